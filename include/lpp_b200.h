@@ -356,6 +356,52 @@ lpp_status lpp_op_sample_static(float* d_logits, int vocab_size, float temperatu
                                 const int* d_history, int history_len, float r, int* d_sampled_token,
                                 void* stream);
 
+/* ---- attention operators beyond the reference's: prompts of several sequences, and a cache held in 4 bits -------------------
+ *
+ * No counterpart in the reference, which runs one sequence with an FP16 cache (src/model.cpp:121-209).  Device pointers, work is
+ * queued on `stream`, nothing is allocated or synchronised; the current device is the one that holds the memory.
+ *
+ * The 4-bit cache of a layer is two arrays (keys, values) [batch][n_kv_heads][capacity] of rows of
+ * lpp_op_kv4_row_bytes(head_size) bytes, on 16-byte boundaries, capacity a multiple of 4.  A row holds groups of 32 dimensions
+ * (ceil(head_size / 32) of them; 8 where that is 5 to 7), lo and hi being the least and the largest value of a group:
+ *     scale = fp16((hi - lo) / 15), zero = fp16(lo + 8 scale), code = clamp(round((x - zero) / scale) + 8, 0, 15)
+ * (half to even; 8 where scale is 0), and the code stands for zero + scale (code - 8).  First the codes of all groups, two a
+ * byte, the lower dimension in the lower half; then (scale, zero) of every group.  A NaN is written as 0, a value beyond the FP16
+ * range as +-65504.  Dimensions that the head does not have carry code 8. */
+
+int64_t lpp_op_kv4_row_bytes(int head_size); /* -1: head sizes are 1 to 256 */
+
+/* Writes n_tokens rows of keys and values [token][n_kv_heads][head_size] (dtype F32, F16 or BF16; *_stride elements from one token to
+ * the next) at the slots d_slots[token] = sequence * capacity + position.  A token whose slot lies outside [0, batch *
+ * capacity) is left out.  The slots of one call differ from one another.  lpp_op_kv4_read gets rows back as values; where the slot lies
+ * outside, the token's place is left as it was. */
+lpp_status lpp_op_kv4_write(void* d_k_cache, void* d_v_cache, const void* d_k, const void* d_v, const int64_t* d_slots, int n_tokens, int batch,
+                            int n_kv_heads, int64_t capacity, int head_size, int64_t k_stride, int64_t v_stride, int dtype, void* stream);
+lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const void* d_v_cache, const int64_t* d_slots, int n_tokens, int batch,
+                           int n_kv_heads, int64_t capacity, int head_size, int64_t k_stride, int64_t v_stride, int dtype, void* stream);
+
+/* Attention of one query token per sequence over the first d_lens[b] positions (clamped to [0, capacity]) of the 4-bit cache:
+ * out[b][h] = sum_j softmax_j(scale q[b][h] . k[b][h / (n_heads / n_kv_heads)][j]) v[...][j]; zeros for a sequence of no positions.
+ * q and out are [batch][n_heads][head_size] of dtype, *_stride elements from one sequence to the next.  FP32 queries and results are worked
+ * with in FP32 precision, others with probabilities rounded to FP16.
+ * d_sums_out (may be NULL) gets the running sums of attention weight that lpp_op_kv4_evict goes by, [batch][n_kv_heads][capacity]:
+ * d_sums_in (NULL = zeros; may be the same array) plus, per position, the sum of the softmax over the query heads of the key/value
+ * head.  Positions from the length on are left as they were.
+ * scratch: lpp_op_kv4_attention_scratch_bytes(...) bytes on a 256-byte boundary, of any content; calls that may overlap need their own. */
+int64_t lpp_op_kv4_attention_scratch_bytes(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int with_sums);
+lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_out, const void* d_q, const void* d_k_cache, const void* d_v_cache,
+                                const int* d_lens, const float* d_sums_in, float* d_sums_out, float scale, int batch, int n_heads, int n_kv_heads,
+                                int64_t capacity, int head_size, int64_t out_stride, int64_t q_stride, int dtype, void* stream);
+
+/* Moves the rows that matter into a shorter cache (another pair of arrays, of capacity_out >= keep positions).  A sequence longer
+ * than `keep` keeps, head by head, its `recent` last rows (recent <= keep) and of the others those with the largest sums, the lowest
+ * position first among equals, a NaN counting as -infinity; a shorter one keeps everything.  Rows stay in their order.  d_kept
+ * [batch][n_kv_heads][keep] gets the old positions, d_sums_out [batch][n_kv_heads][capacity_out] their sums, d_lens_out [batch]
+ * the new lengths min(length, keep); what lies behind them is left as it was. */
+lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int* d_kept, int* d_lens_out, const void* d_k_cache,
+                            const void* d_v_cache, const float* d_sums, const int* d_lens, int batch, int n_kv_heads, int64_t capacity,
+                            int64_t capacity_out, int head_size, int keep, int recent, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,261 @@
+// C-ABI entry points of the stand-alone attention operators: whole packed prompts, and a cache held in 4 bits with what writes it, reads
+// it back, attends to it and makes it shorter.  Device pointers in and out, nothing synchronised or allocated; scratch comes from the
+// caller and may hold anything.
+#include <cuda_runtime.h>
+#include <stdio.h>
+
+#include "../../include/lpp_b200.h"
+#include "common.cuh"
+#include "kv4.cuh"
+#include "op_launch.cuh"
+
+using namespace lpp;
+
+void lpp_internal_set_error(const char* msg);  // engine.cu: text behind lpp_last_error()
+
+namespace {
+
+lpp_status refuse(const char* what, lpp_status s = LPP_ERR_INVALID_ARG) {
+    lpp_internal_set_error(what);
+    return s;
+}
+lpp_status launched(const char* what, lpp_status s) { return s == LPP_OK ? s : refuse(what, s); }
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return 0;
+    }
+    return sms;
+}
+
+// Calls f with a constant for the groups of a row (1 - 4 or 8; 5 - 7 groups are held as 8).
+int kv4_held_groups(int head_size) {
+    const int g = kv4_groups(head_size);
+    return g > 4 ? 8 : g;
+}
+template <int N>
+struct Int {
+    static constexpr int value = N;
+};
+template <typename F>
+lpp_status with_groups(int groups, F f) {
+    switch (groups) {
+        case 1: return f(Int<1>());
+        case 2: return f(Int<2>());
+        case 3: return f(Int<3>());
+        case 4: return f(Int<4>());
+        default: return f(Int<8>());
+    }
+}
+template <typename F>
+lpp_status with_type(int dtype, F f) {
+    if (dtype == LPP_F16) return f((__half*)nullptr);
+    if (dtype == LPP_BF16) return f((__nv_bfloat16*)nullptr);
+    return f((float*)nullptr);
+}
+bool is_dtype(int dtype) { return dtype == LPP_F32 || dtype == LPP_F16 || dtype == LPP_BF16; }
+
+// What every call on a 4-bit cache wants of it; NULL = nothing wrong.
+const char* size_fault(int batch, int kv_heads, int64_t capacity, int head_size) {
+    if (batch <= 0 || kv_heads <= 0 || capacity <= 0 || batch > 65535 || kv_heads > 65535) return "4-bit cache: sizes out of range";
+    if (capacity % 4 || capacity > (1 << 30)) return "4-bit cache: the capacity is a multiple of 4, at most 2^30";
+    if (head_size <= 0 || head_size > 256) return "4-bit cache: head sizes are 1 to 256";
+    return nullptr;
+}
+const char* cache_fault(const void* k, const void* v, int batch, int kv_heads, int64_t capacity, int head_size) {
+    if (!k || !v) return "4-bit cache: null pointer";
+    if (((uintptr_t)k | (uintptr_t)v) & 15) return "4-bit cache: the caches start on a 16-byte boundary";
+    return size_fault(batch, kv_heads, capacity, head_size);
+}
+
+// Shared by writing and reading rows.
+template <typename Launch>
+lpp_status rows_op(const char* name, const void* k, const void* v, const int64_t* slots, const void* kc, const void* vc, int n, int batch, int kv_heads, int64_t capacity,
+                   int head_size, int64_t k_stride, int64_t v_stride, int dtype, Launch launch) {
+    if (const char* f = cache_fault(kc, vc, batch, kv_heads, capacity, head_size)) return refuse(f);
+    if (!is_dtype(dtype)) return refuse("4-bit cache: rows are F32, F16 or BF16");
+    if (n < 0 || (long long)n * kv_heads > 0x7fffffffll) return refuse("4-bit cache: too many rows");
+    if (n == 0) return LPP_OK;
+    if (!k || !v || !slots) return refuse("4-bit cache: null pointer");
+    const int element = dtype == LPP_F32 ? 4 : 2;
+    if (((uintptr_t)k | (uintptr_t)v) & (element - 1) || (uintptr_t)slots & 7) return refuse("4-bit cache: a pointer is not aligned to its type");
+    const int64_t dense = (int64_t)kv_heads * head_size;
+    if (k_stride < dense || v_stride < dense) return refuse("4-bit cache: a token's rows overlap the next one's");
+    // eight values at once where every row starts on a 16-byte boundary
+    const bool wide = head_size % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) && k_stride * element % 16 == 0 && v_stride * element % 16 == 0;
+    Kv4Cache c = {(unsigned char*)kc, (unsigned char*)vc, capacity, (long long)batch * capacity, kv_heads};
+    const int groups = kv4_held_groups(head_size), rows = n * kv_heads;
+    const long long ctas = ((long long)rows * 4 * groups + kKv4RowThreads - 1) / kKv4RowThreads;
+    return launched(name, launch(c, groups, dim3((unsigned)ctas, 2), rows, wide));
+}
+
+// ---- attention over the 4-bit cache: runs of work (one CTA an SM) and the scratch
+int attn_runs(int batch, int n_heads, int n_kv_heads, int64_t capacity, int sms) {
+    const int head_tiles = (n_heads / n_kv_heads + kKv4Heads - 1) / kKv4Heads;
+    return (int)std::min<long long>(sms, (long long)batch * n_kv_heads * head_tiles * ((capacity + kKv4Unit - 1) / kKv4Unit));
+}
+struct AttnLayout {
+    size_t whole, ml, part, scores, total;
+};
+AttnLayout attn_layout(int runs, int batch, int n_heads, int64_t capacity, int groups, bool sums) {
+    auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+    AttnLayout L = {};
+    L.ml = up(sums ? (size_t)batch * n_heads * 8 : 0);
+    L.part = L.ml + up((size_t)runs * 2 * kKv4Heads * 8);
+    L.scores = L.part + up((size_t)runs * 2 * kKv4Heads * groups * 32 * 4);
+    L.total = L.scores + up(sums ? (size_t)batch * n_heads * capacity * 4 : 0);
+    return L;
+}
+const char* attn_fault(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size) {
+    if (const char* f = size_fault(batch, n_kv_heads, capacity, head_size)) return f;
+    if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 1024) return "4-bit attention: the key/value heads divide the heads, at most 1024 to one";
+    return nullptr;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t lpp_op_kv4_row_bytes(int head_size) { return head_size <= 0 || head_size > 256 ? -1 : kv4_row_bytes(kv4_held_groups(head_size)); }
+
+lpp_status lpp_op_kv4_write(void* d_k_cache, void* d_v_cache, const void* d_k, const void* d_v, const int64_t* d_slots, int n_tokens, int batch, int n_kv_heads,
+                            int64_t capacity, int head_size, int64_t k_stride, int64_t v_stride, int dtype, void* stream) {
+    return rows_op("lpp_op_kv4_write: the launch failed", d_k, d_v, d_slots, d_k_cache, d_v_cache, n_tokens, batch, n_kv_heads, capacity, head_size, k_stride, v_stride, dtype,
+                   [&](const Kv4Cache& c, int groups, dim3 grid, int rows, bool wide) {
+                       return with_groups(groups, [&](auto ng) {
+                           return with_type(dtype, [&](auto* t) {
+                               using T = std::remove_pointer_t<decltype(t)>;
+                               return launch_op(kv4_write_kernel<T, ng.value>, grid, kKv4RowThreads, 0, S(stream), c, (const T*)d_k, (const T*)d_v, (const long long*)d_slots,
+                                                rows, head_size, (long long)k_stride, (long long)v_stride, wide);
+                           });
+                       });
+                   });
+}
+
+lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const void* d_v_cache, const int64_t* d_slots, int n_tokens, int batch, int n_kv_heads,
+                           int64_t capacity, int head_size, int64_t k_stride, int64_t v_stride, int dtype, void* stream) {
+    return rows_op("lpp_op_kv4_read: the launch failed", d_k, d_v, d_slots, d_k_cache, d_v_cache, n_tokens, batch, n_kv_heads, capacity, head_size, k_stride, v_stride, dtype,
+                   [&](const Kv4Cache& c, int groups, dim3 grid, int rows, bool wide) {
+                       return with_groups(groups, [&](auto ng) {
+                           return with_type(dtype, [&](auto* t) {
+                               using T = std::remove_pointer_t<decltype(t)>;
+                               return launch_op(kv4_read_kernel<T, ng.value>, grid, kKv4RowThreads, 0, S(stream), c, (T*)d_k, (T*)d_v, (const long long*)d_slots, rows, head_size,
+                                                (long long)k_stride, (long long)v_stride, wide);
+                           });
+                       });
+                   });
+}
+
+int64_t lpp_op_kv4_attention_scratch_bytes(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int with_sums) {
+    const int sms = sm_count();
+    if (sms <= 0 || attn_fault(batch, n_heads, n_kv_heads, capacity, head_size)) return -1;
+    return (int64_t)attn_layout(attn_runs(batch, n_heads, n_kv_heads, capacity, sms), batch, n_heads, capacity, kv4_held_groups(head_size), with_sums != 0).total;
+}
+
+lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_out, const void* d_q, const void* d_k_cache, const void* d_v_cache, const int* d_lens,
+                                const float* d_sums_in, float* d_sums_out, float scale, int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size,
+                                int64_t out_stride, int64_t q_stride, int dtype, void* stream) {
+    if (const char* f = cache_fault(d_k_cache, d_v_cache, batch, n_kv_heads, capacity, head_size)) return refuse(f);
+    if (const char* f = attn_fault(batch, n_heads, n_kv_heads, capacity, head_size)) return refuse(f);
+    if (!scratch || ((uintptr_t)scratch & 255) || !d_out || !d_q || !d_lens) return refuse("4-bit attention: null pointer, or scratch not on a 256-byte boundary");
+    if (!is_dtype(dtype)) return refuse("4-bit attention: queries are F32, F16 or BF16");
+    const int element = dtype == LPP_F32 ? 4 : 2;
+    if (((uintptr_t)d_out | (uintptr_t)d_q) & (element - 1) || ((uintptr_t)d_lens | (uintptr_t)d_sums_in | (uintptr_t)d_sums_out) & 3)
+        return refuse("4-bit attention: a pointer is not aligned to its type");
+    if (out_stride < (int64_t)n_heads * head_size || q_stride < (int64_t)n_heads * head_size) return refuse("4-bit attention: a sequence's heads overlap the next one's");
+    if (!(scale > 0.f) || scale > 3.4e38f) return refuse("4-bit attention: the scale is positive and finite");
+    if (d_sums_in && !d_sums_out) return refuse("4-bit attention: sums go in but not out");
+    const int sms = sm_count();
+    if (sms <= 0) return refuse("4-bit attention: no CUDA device", LPP_ERR_NO_DEVICE);
+    const int groups = kv4_held_groups(head_size), runs = attn_runs(batch, n_heads, n_kv_heads, capacity, sms);
+    const AttnLayout L = attn_layout(runs, batch, n_heads, capacity, groups, d_sums_out != nullptr);
+    if (scratch_bytes < (int64_t)L.total) return refuse("4-bit attention: scratch is smaller than lpp_op_kv4_attention_scratch_bytes() says");
+    char* w = (char*)scratch;
+    Kv4AttnArgs a = {};
+    a.k = (const unsigned char*)d_k_cache;
+    a.v = (const unsigned char*)d_v_cache;
+    a.q = d_q;
+    a.out = d_out;
+    a.lens = d_lens;
+    a.sums_in = d_sums_in;
+    a.sums_out = d_sums_out;
+    a.scores = d_sums_out ? (float*)(w + L.scores) : nullptr;
+    a.whole_ml = d_sums_out ? (float2*)(w + L.whole) : nullptr;
+    a.part_ml = (float2*)(w + L.ml);
+    a.part_o = (float*)(w + L.part);
+    a.capacity = capacity;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.batch = batch;
+    a.heads = n_heads;
+    a.kv_heads = n_kv_heads;
+    a.gqa = n_heads / n_kv_heads;
+    a.head_size = head_size;
+    a.head_tiles = (a.gqa + kKv4Heads - 1) / kKv4Heads;
+    a.runs = runs;
+    a.dtype = dtype;
+    a.rate = scale * 1.4426950408889634f;
+    return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
+                        constexpr int NG = ng.value;
+                        constexpr int smem = kv4_attn_smem<NG>();
+                        auto kernel = dtype == LPP_F32 ? kv4_attn_kernel<NG, true> : kv4_attn_kernel<NG, false>;
+                        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+                            (void)cudaGetLastError();
+                            return LPP_ERR_CUDA;
+                        }
+                        const lpp_status st = launch_op(kernel, dim3(runs), kKv4Threads, smem, S(stream), a);
+                        if (st != LPP_OK) return st;
+                        const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;
+                        return launch_op(kv4_finish_kernel<NG>, dim3((unsigned)std::max<long long>(a.gqa, rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)a.gqa * 8, S(stream),
+                                         a);
+                    }));
+}
+
+lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int* d_kept, int* d_lens_out, const void* d_k_cache, const void* d_v_cache, const float* d_sums,
+                            const int* d_lens, int batch, int n_kv_heads, int64_t capacity, int64_t capacity_out, int head_size, int keep, int recent, void* stream) {
+    if (const char* f = cache_fault(d_k_cache, d_v_cache, batch, n_kv_heads, capacity, head_size)) return refuse(f);
+    if (const char* f = cache_fault(d_k_out, d_v_out, batch, n_kv_heads, capacity_out, head_size)) return refuse(f);
+    if (!d_sums_out || !d_kept || !d_lens_out || !d_sums || !d_lens) return refuse("eviction: null pointer");
+    if (((uintptr_t)d_sums_out | (uintptr_t)d_kept | (uintptr_t)d_lens_out | (uintptr_t)d_sums | (uintptr_t)d_lens) & 3) return refuse("eviction: a pointer is not aligned to its type");
+    if (keep <= 0 || keep > capacity_out || recent < 0 || recent > keep) return refuse("eviction: 0 <= recent <= keep <= capacity of the new cache, keep > 0");
+    // rows move to other places while others are read: the old and the new cache are two
+    auto apart = [](const void* x, size_t nx, const void* y, size_t ny) { return (uintptr_t)x + nx <= (uintptr_t)y || (uintptr_t)y + ny <= (uintptr_t)x; };
+    const int row = kv4_row_bytes(kv4_held_groups(head_size));
+    const size_t heads = (size_t)batch * n_kv_heads, in = heads * capacity * row, out = heads * capacity_out * row;
+    const void *ins[2] = {d_k_cache, d_v_cache}, *outs[2] = {d_k_out, d_v_out};
+    for (const void* i : ins)
+        for (const void* o : outs)
+            if (!apart(i, in, o, out)) return refuse("eviction: the new cache overlaps the old one");
+    if (!apart(d_k_out, out, d_v_out, out) || !apart(d_sums, heads * capacity * 4, d_sums_out, heads * capacity_out * 4) || !apart(d_lens, (size_t)batch * 4, d_lens_out, (size_t)batch * 4))
+        return refuse("eviction: the new cache overlaps the old one");
+    const int sms = sm_count();
+    if (sms <= 0) return refuse("eviction: no CUDA device", LPP_ERR_NO_DEVICE);
+    Kv4EvictArgs a = {};
+    a.k = (const unsigned char*)d_k_cache;
+    a.v = (const unsigned char*)d_v_cache;
+    a.k_out = (unsigned char*)d_k_out;
+    a.v_out = (unsigned char*)d_v_out;
+    a.sums = d_sums;
+    a.sums_out = d_sums_out;
+    a.kept = d_kept;
+    a.lens_out = d_lens_out;
+    a.lens = d_lens;
+    a.capacity = capacity;
+    a.capacity_out = capacity_out;
+    a.kv_heads = n_kv_heads;
+    a.keep = keep;
+    a.recent = recent;
+    a.row_bytes = row;
+    lpp_status st = launch_op(kv4_select_kernel, dim3(n_kv_heads, batch), kKv4EvictThreads, 0, S(stream), a);
+    if (st != LPP_OK) return launched("lpp_op_kv4_evict: the launch failed", st);
+    const int vec = row % 16 == 0 ? 16 : row % 8 == 0 ? 8 : 4;
+    const long long per_head = ((long long)keep * (row / vec) + 255) / 256;
+    const dim3 grid((unsigned)std::min<long long>(per_head, std::max<long long>(1, 8ll * sms / (long long)heads)), n_kv_heads, batch);
+    st = vec == 16 ? launch_op(kv4_move_kernel<uint4>, grid, 256, 0, S(stream), a)
+                   : vec == 8 ? launch_op(kv4_move_kernel<uint2>, grid, 256, 0, S(stream), a) : launch_op(kv4_move_kernel<uint32_t>, grid, 256, 0, S(stream), a);
+    return launched("lpp_op_kv4_evict: the launch failed", st);
+}
+
+}  // extern "C"

@@ -6,7 +6,7 @@ set -e
 HERE="$(cd "$(dirname "$0")" && pwd)"
 OUT="${LPP_OUT:-$HERE/../liblpp_b200.so}"
 NVCC="${NVCC:-/usr/local/cuda/bin/nvcc}"
-"$NVCC" -gencode arch=compute_100a,code=sm_100a -lineinfo -O3 -std=c++17 --threads 2 \
+"$NVCC" -gencode arch=compute_100a,code=sm_100a -lineinfo -O3 -std=c++17 --threads 3 \
     -ccbin "${HOSTCXX:-g++}" --shared -Xcompiler -fPIC -Xptxas -v \
-    -o "$OUT" "$HERE/engine.cu" "$HERE/ops_api.cu" -ldl "$@"
+    -o "$OUT" "$HERE/engine.cu" "$HERE/ops_api.cu" "$HERE/attention_api.cu" -ldl "$@"
 echo "built $OUT"

@@ -135,6 +135,11 @@ __device__ __forceinline__ float act_gate_arg(int act, float z) {
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Allow the dependent grid to start launching (it still waits in pdl_wait for our completion).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// First statement of every operator kernel: nothing of the kernel before may be touched ahead of it.
+__device__ __forceinline__ void op_begin() {
+    pdl_launch_dependents();
+    pdl_wait();
+}
 
 // ------------------------------------------------------------------ mbarrier + bulk async copy
 

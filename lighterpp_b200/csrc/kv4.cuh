@@ -1,0 +1,780 @@
+// A key/value cache held in 4 bits: writing rows into it, reading them back, attention of one token per sequence over it, and
+// moving the rows that matter into a shorter cache.  No counterpart in the reference, whose cache is FP16 (src/model.h:108-109); the
+// layout follows its order [kv head][position] (src/scatter_kv.cu:15-16) with one more dimension for the sequence.
+//
+// A row holds the keys (or values) of one head at one position in groups of 32 dimensions.  With lo and hi the least and the largest
+// value of a group:
+//     scale = fp16((hi - lo) / 15),  zero = fp16(lo + 8 scale),  code = clamp(round((x - zero) / scale) + 8, 0, 15)   (half to even;
+// 8 where scale is 0), and the code stands for zero + scale (code - 8).  The bytes of a row: 16 per group with two codes each (the lower
+// dimension in the lower half), then 4 per group with scale and zero.  The dimensions that fill the last group up have code 8 and
+// count neither for lo nor for hi.  A NaN is written as 0, values beyond the FP16 range as +-65504.
+#pragma once
+#include "common.cuh"
+
+namespace lpp {
+
+constexpr int kKv4Group = 32;
+__host__ __device__ constexpr int kv4_groups(int head_size) { return (head_size + kKv4Group - 1) / kKv4Group; }
+__host__ __device__ constexpr int kv4_row_bytes(int groups) { return groups * (kKv4Group / 2 + 4); }
+
+// The caches of one layer: [batch][kv_heads][capacity] rows.
+struct Kv4Cache {
+    unsigned char *k, *v;
+    long long capacity, slots;  // slots: batch * capacity
+    int kv_heads;
+};
+
+// ------------------------------------------------------------------ writing and reading rows
+//
+// Four threads a group, eight dimensions (one 32-bit word of codes) each; bound by the bytes of the values.
+
+constexpr int kKv4RowThreads = 256;
+
+// Eight consecutive values; `n` of them exist.
+template <typename T>
+__device__ __forceinline__ void kv4_load8(const T* p, int n, bool wide, float (&x)[8]) {
+    if (wide && n >= 8) {
+        if constexpr (sizeof(T) == 4) {
+            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
+            const uint4 a = *reinterpret_cast<const uint4*>(p);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2<T>(w[i]);
+                x[2 * i] = f.x;
+                x[2 * i + 1] = f.y;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
+    }
+}
+
+// a - b = d + e exactly (Knuth's two-sum)
+__device__ __forceinline__ float exact_sub(float a, float b, float& e) {
+    const float d = __fsub_rn(a, b), bb = __fsub_rn(d, a);
+    e = __fsub_rn(__fsub_rn(a, __fsub_rn(d, bb)), __fadd_rn(b, bb));
+    return d;
+}
+
+// The code of x - 8: round((x - zero) / scale) to even, in [-8, 7].  `inv` is about 1 / scale; next to a border between two codes the
+// exact remainder decides, so that the code is that of the exact quotient.
+__device__ __forceinline__ int kv4_code(float x, float zero, float scale, float inv) {
+    const float t = fminf(fmaxf((x - zero) * inv, -8.f), 7.f);
+    float r = rintf(t);
+    if (fabsf(t - r) > 0.4999f) {  // (the quotient's error is below 8 * 2^-21)
+        float e;
+        const float d = exact_sub(x, zero, e), border = floorf(t) + 0.5f;  // border * scale: 5 + 11 bits, exact
+        const float rest = __fadd_rn(__fsub_rn(d, border * scale), e);      // the subtraction is exact so near the border
+        r = rest > 0.f ? border + 0.5f : rest < 0.f ? border - 0.5f : rintf(border);
+    }
+    return (int)fminf(fmaxf(r, -8.f), 7.f);
+}
+
+template <typename T, int NG>
+static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(Kv4Cache c, const T* k, const T* v, const long long* slots, int n_rows,
+                                                                          int head_size, long long k_stride, long long v_stride, bool wide) {
+    op_begin();
+    constexpr int kLanes = 4 * NG;  // threads of a row
+    const long long i = (long long)blockIdx.x * kKv4RowThreads + threadIdx.x;
+    const long long row = i / kLanes;
+    if ((i - (threadIdx.x & 31)) / kLanes >= n_rows) return;  // (whole warps: the shuffles below need all lanes)
+    const int lane = (int)(i - row * kLanes), d0 = lane * 8;
+    const int token = (int)min(row, (long long)n_rows - 1) / c.kv_heads, head = (int)min(row, (long long)n_rows - 1) - token * c.kv_heads;
+    const long long slot = slots[token];
+    const bool valid = row < n_rows && slot >= 0 && slot < c.slots;
+    float x[8];
+    const int n = head_size - d0;
+    const T* src = blockIdx.y ? v + token * v_stride : k + token * k_stride;
+    kv4_load8(src + (long long)head * head_size + d0, n, wide, x);
+    float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
+        if (j < n) {
+            lo = fminf(lo, x[j]);
+            hi = fmaxf(hi, x[j]);
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    if (lo > hi) lo = hi = 0.f;  // no dimension of the head lies in this group
+    // (hi - lo) / 15 as the exact difference's quotient rounded once to FP32, then to FP16
+    float e;
+    const float d = exact_sub(hi, lo, e), q = __fdiv_rn(d, 15.f), rest = __fadd_rn(__fmaf_rn(-15.f, q, d), e);
+    const __half scale_h = __float2half_rn(__fadd_rn(q, rest * (1.f / 15.f)));
+    const float scale = __half2float(scale_h);
+    const __half zero_h = __float2half_rn(__fmaf_rn(8.f, scale, lo));
+    const float zero = __half2float(zero_h), inv = __fdiv_rn(1.f, scale);
+    uint32_t word = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int code = j < n && scale > 0.f ? kv4_code(x[j], zero, scale, inv) : 0;
+        word |= (uint32_t)(code + 8) << (4 * j);
+    }
+    if (!valid) return;
+    const long long b = slot / c.capacity, p = slot - b * c.capacity;
+    unsigned char* dst = (blockIdx.y ? c.v : c.k) + ((b * c.kv_heads + head) * c.capacity + p) * kv4_row_bytes(NG);
+    *reinterpret_cast<uint32_t*>(dst + lane * 4) = word;
+    if ((lane & 3) == 0)
+        *reinterpret_cast<uint32_t*>(dst + NG * 16 + lane) = (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(zero_h) << 16;
+}
+
+template <typename T, int NG>
+static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(Kv4Cache c, T* k, T* v, const long long* slots, int n_rows, int head_size,
+                                                                         long long k_stride, long long v_stride, bool wide) {
+    op_begin();
+    constexpr int kLanes = 4 * NG;
+    const long long i = (long long)blockIdx.x * kKv4RowThreads + threadIdx.x;
+    const long long row = i / kLanes;
+    if (row >= n_rows) return;
+    const int lane = (int)(i - row * kLanes), d0 = lane * 8, n = head_size - d0;
+    const int token = (int)row / c.kv_heads, head = (int)row - token * c.kv_heads;
+    const long long slot = slots[token];
+    if (n <= 0 || slot < 0 || slot >= c.slots) return;
+    const long long b = slot / c.capacity, p = slot - b * c.capacity;
+    const unsigned char* src = (blockIdx.y ? c.v : c.k) + ((b * c.kv_heads + head) * c.capacity + p) * kv4_row_bytes(NG);
+    const uint32_t word = *reinterpret_cast<const uint32_t*>(src + lane * 4);
+    const float2 sz = half2_bits_to_float2(*reinterpret_cast<const uint32_t*>(src + NG * 16 + (lane & ~3)));
+    T* dst = (blockIdx.y ? v + token * v_stride : k + token * k_stride) + (long long)head * head_size + d0;
+    __align__(16) T y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = from_float<T>(__fadd_rn(sz.y, sz.x * (float)((int)(word >> (4 * j) & 15) - 8)));  // (the product is exact)
+    if (wide && n >= 8) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
+    } else {
+        for (int j = 0; j < n && j < 8; ++j) dst[j] = y[j];
+    }
+}
+
+// ------------------------------------------------------------------ attention of one token per sequence
+//
+// out = sum_j p_j v_j, p = softmax(scale q . k_j) over the positions below the sequence's length.  Units of 128 positions of one
+// key/value head, in the order [sequence][head][position], are dealt out to the CTAs in equal runs, whatever the lengths; the eight
+// warps of a CTA take 16 positions of a unit each and keep running sums of their own, which are put together where a run goes on to
+// the next head or ends.  Heads that lie in several runs are put together by the finishing kernel.
+//
+// Products on the tensor cores (mma.sync.m16n8k16, FP32 sums), cache rows as the 16-row operand and up to eight query heads of the
+// key/value head as the 8-column one.  The codes themselves are the operand: as FP16 bit patterns, 0 .. 15 are the subnormals
+// n 2^-24, and the same bits four places up are 16 n 2^-24, so a mask makes two elements of an operand register (the query elements of
+// the second kind are divided by 16).  Sums are kept apart by group and multiplied with the group's scale in FP32:
+//     q . k = sum_g scale_g (sum_d q_d n_d - 8 Q_g) + zero_g Q_g,  Q_g = sum_d q_d;
+// -8 Q_g is where the accumulator starts.  For the values the scale goes to the probability before that is rounded to FP16, the codes
+// become n - 8 (rounding errors then are those of values around their middle), and sum_j p_j zero_jg is added in FP32.
+//
+// Reference of the exponentials: not the running maximum of the scores but a bound on the largest p * scale, which has to stay in the
+// FP16 range: probabilities are 2^(x - M) with M far enough below the largest x + log2(scale) seen when M was set that they keep their
+// bits, and M moves only when a product would leave the range.  So a tile needs no maximum over lanes, only a vote.
+//
+// FP32 queries and FP32 results go in as two FP16 operands each (hi + lo), the sums of either added up.
+constexpr int kKv4Warps = 8, kKv4Threads = kKv4Warps * 32;
+constexpr int kKv4Tile = 16;     // positions of a warp's tile
+constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
+constexpr int kKv4Heads = 8;     // query heads of a CTA
+constexpr float kKv4Limit = 32768.f;  // of p * scale
+template <int NG>
+constexpr int kKv4Stages = NG > 4 ? 3 : 6;  // tiles in flight per warp
+
+struct Kv4AttnArgs {
+    const unsigned char *k, *v;
+    const void* q;
+    void* out;
+    const int* lens;
+    const float* sums_in;   // NULL = zeros
+    float* sums_out;        // NULL = no sums
+    float* scores;          // [batch][kv_heads][capacity][gqa], base-2 exponents (with sums)
+    float2* whole_ml;       // [batch][heads]: reference and sum of heads that lie in one run (with sums)
+    float2* part_ml;        // [runs][2][8]: the same of parts of a head: [0] one that began in an earlier run, [1] one that begins here
+    float* part_o;          // [runs][2][8][NG * 32]
+    long long capacity, q_stride, out_stride;
+    int batch, heads, kv_heads, gqa, head_size, head_tiles, runs;
+    int dtype;
+    float rate;             // scale * log2(e)
+};
+
+__device__ __forceinline__ int kv4_len(const Kv4AttnArgs& a, int b) { return (int)max(0ll, min((long long)a.lens[b], a.capacity)); }
+__device__ __forceinline__ int kv4_units(int len) { return max(1, (len + kKv4Unit - 1) / kKv4Unit); }  // (an empty sequence has results to write)
+// Units of all sequences for one head, by a warp.
+__device__ __forceinline__ long long kv4_total(const Kv4AttnArgs& a) {
+    long long n = 0;
+    for (int b = threadIdx.x & 31; b < a.batch; b += 32) n += kv4_units(kv4_len(a, b));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n;
+}
+// Sequence that holds unit `unit` of all, and its first unit, by a warp; `heads` counts a key/value head once per eight query heads.
+__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, long long unit, long long& first) {
+    const int lane = threadIdx.x & 31;
+    long long base = 0;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+        const long long own = b0 + lane < a.batch ? (long long)kv4_units(kv4_len(a, b0 + lane)) * heads : 0;
+        long long x = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const unsigned there = __ballot_sync(0xffffffffu, base + x > unit);
+        if (there) {
+            const int at = __ffs(there) - 1;
+            first = base + __shfl_sync(0xffffffffu, x - own, at);
+            return b0 + at;
+        }
+        base += __shfl_sync(0xffffffffu, x, 31);
+    }
+    first = base;
+    return a.batch;
+}
+
+template <int NG>
+constexpr int kKv4RingBytes = kKv4Warps * kKv4Stages<NG> * 2 * kKv4Tile * kv4_row_bytes(NG);
+template <int NG>
+constexpr int kKv4Pitch = NG * 32 + 4;
+template <int NG>
+constexpr int kv4_attn_smem() {  // rings, barriers, sums of the warps
+    return kKv4RingBytes<NG> + kKv4Warps * kKv4Stages<NG> * 8 + kKv4Warps * kKv4Heads * kKv4Pitch<NG> * 4;
+}
+
+__device__ __forceinline__ float load_typed(const void* p, long long i, int dtype) {
+    if (dtype == 1) return __half2float(reinterpret_cast<const __half*>(p)[i]);
+    if (dtype == 2) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+    return reinterpret_cast<const float*>(p)[i];
+}
+__device__ __forceinline__ void store_typed(void* p, long long i, int dtype, float x) {
+    if (dtype == 1)
+        reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
+    else if (dtype == 2)
+        reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
+    else
+        reinterpret_cast<float*>(p)[i] = x;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// d = a . b + c
+__device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
+                                        float c3) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 matrix of 16-bit elements spread over a warp
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t a) {
+    uint16_t r;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(a));
+    return r;
+}
+// (n - 8) of the codes in bits 0-3 and 16-19, and in bits 4-7 and 20-23: 1024 + n - 1032, (1024 + 16 n) / 16 - 72, both exact
+__device__ __forceinline__ uint32_t kv4_low(uint32_t x) {
+    const uint32_t b = (x & 0x000f000fu) | 0x64006400u, off = 0x64086408u;
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t kv4_high(uint32_t x) {
+    const uint32_t b = (x & 0x00f000f0u) | 0x64006400u, f = 0x2c002c00u /* 1/16 */, off = 0xd480d480u /* -72 */;
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&f), *reinterpret_cast<const __half2*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+template <int NG, bool SPLIT>
+static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const Kv4AttnArgs a) {
+    constexpr int kRow = kv4_row_bytes(NG), kTileBytes = kKv4Tile * kRow, kParts = SPLIT ? 2 : 1, kStages = kKv4Stages<NG>, kPitch = kKv4Pitch<NG>;
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ float s_m[kKv4Warps][kKv4Heads], s_l[kKv4Warps][kKv4Heads];
+    __shared__ int s_fail;
+    op_begin();
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int heads8 = a.kv_heads * a.head_tiles;
+    const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);  // (no run is empty)
+    if (blockIdx.x >= runs) return;
+    const long long begin = all * blockIdx.x / runs, end = all * (blockIdx.x + 1) / runs;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kKv4RingBytes<NG>) + warp * kStages;
+    float* so = reinterpret_cast<float*>(smem + kKv4RingBytes<NG> + kKv4Warps * kStages * 8);
+    unsigned char* ring = smem + warp * kStages * 2 * kTileBytes;
+    if (tid == 0) s_fail = 0;
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
+        mbar_fence_init();
+    }
+    __syncthreads();
+    long long first = 0;
+    int b = kv4_find(a, heads8, begin, first), len = kv4_len(a, b), units = kv4_units(len);
+    int head = (int)((begin - first) / units), unit = (int)(begin - first - (long long)head * units);
+    const int here = (int)(end - begin);
+
+    // lane 0: requests this warp's tiles in their order, as far as the ring reaches
+    int ahead_b = b, ahead_len = len, ahead_units = units, ahead_head = head, ahead_unit = unit, ahead_left = here, asked = 0, used = 0;
+    auto request = [&]() {
+        while (ahead_left > 0 && asked - used < kStages) {
+            const int at = ahead_unit * kKv4Unit + warp * kKv4Tile;
+            if (at < ahead_len) {
+                const int stage = asked % kStages;
+                const long long row = ((long long)ahead_b * a.kv_heads + ahead_head / a.head_tiles) * a.capacity + at;
+                const uint32_t bytes = (uint32_t)min((long long)kKv4Tile, a.capacity - at) * kRow;  // (a multiple of four rows)
+                mbar_arrive_expect_tx(&bars[stage], 2 * bytes);
+                bulk_g2s(ring + stage * 2 * kTileBytes, a.k + row * kRow, bytes, &bars[stage]);
+                bulk_g2s(ring + stage * 2 * kTileBytes + kTileBytes, a.v + row * kRow, bytes, &bars[stage]);
+                ++asked;
+            }
+            --ahead_left;
+            if (++ahead_unit == ahead_units) {
+                ahead_unit = 0;
+                if (++ahead_head == heads8 && ahead_left > 0) {
+                    ahead_head = 0;
+                    ahead_len = kv4_len(a, ++ahead_b);
+                    ahead_units = kv4_units(ahead_len);
+                }
+            }
+        }
+    };
+    if (lane == 0) request();
+    bool ok = true;
+
+    for (int left = here; left > 0;) {
+    const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
+    const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
+    const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
+    const int mine = min(units - unit, left), p1 = len;
+    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^13 .. 2^14
+    uint32_t qf[kParts][NG][4];
+    float qs[NG][2], rate[2];  // sums of a group and factor of the scores, heads 2 t and 2 t + 1
+    {
+        float x[NG][8], top = 0.f;
+        const bool some = g < n_heads;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int d = i * 32 + t * 8 + j;
+                x[i][j] = some && d < a.head_size ? load_typed(a.q, (long long)b * a.q_stride + (long long)(h0 + g) * a.head_size + d, a.dtype) : 0.f;
+                top = fmaxf(top, fabsf(x[i][j]));
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // exponents of 2 in two halves, either within the normal range
+        const int e = top > 0.f && top < INFINITY ? 13 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
+        const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
+        float sums[NG];
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+            float sum = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16
+                const float f = (j & 1) ? 1.f / 16.f : 1.f;
+                const float u = x[i][j] * f0 * f1, w = x[i][j + 4] * f0 * f1;
+                const __half2 hi = __floats2half2_rn(u * f, w * f);
+                const float2 hf = __half22float2(hi);
+                qf[0][i][j] = *reinterpret_cast<const uint32_t*>(&hi);
+                sum += (hf.x + hf.y) * ((j & 1) ? 16.f : 1.f);
+                if constexpr (SPLIT) {
+                    const __half2 lo = __floats2half2_rn(u * f - hf.x, w * f - hf.y);
+                    const float2 lf = __half22float2(lo);
+                    qf[1][i][j] = *reinterpret_cast<const uint32_t*>(&lo);
+                    sum += (lf.x + lf.y) * ((j & 1) ? 16.f : 1.f);
+                }
+            }
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            sums[i] = sum * 0x1p-24f;  // the codes' factor
+        }
+        // 2^24 / 2^e, back from the operands' factors
+        const float back = __int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * 0x1p24f * a.rate;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int from = (2 * t + j) * 4;
+            rate[j] = __shfl_sync(0xffffffffu, back, from);
+#pragma unroll
+            for (int i = 0; i < NG; ++i) qs[i][j] = __shfl_sync(0xffffffffu, sums[i], from);
+        }
+    }
+
+    float o[2 * NG][4], z[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) z[i][0] = z[i][1] = 0.f;
+
+    for (int i = 0; i < mine; ++i) {
+        const int at = (unit + i) * kKv4Unit + warp * kKv4Tile, stage = used % kStages;
+        if (at >= p1) continue;
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&bars[stage], (uint32_t)(used / kStages) & 1u, nullptr));
+        if (!ok) {  // a copy that never came: the results of this run say so
+            m[0] = m[1] = NAN;
+            s_fail = 1;
+            break;
+        }
+        const uint32_t sk = smem_u32(ring + stage * 2 * kTileBytes), sv = sk + kTileBytes;
+        // ---- scores of rows g and g + 8
+        float s[4] = {};
+        {
+            const uint32_t r0 = sk + g * kRow, r1 = r0 + 8 * kRow;
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                const uint32_t w0 = lds32(r0 + gr * 16 + t * 4), w1 = lds32(r1 + gr * 16 + t * 4);
+                const float2 sz0 = half2_bits_to_float2(lds32(r0 + NG * 16 + gr * 4)), sz1 = half2_bits_to_float2(lds32(r1 + NG * 16 + gr * 4));
+                const float c0 = -8.f * qs[gr][0], c1 = -8.f * qs[gr][1];
+                float acc[4];
+                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
+                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], c0, c1, c0, c1);
+                kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[0][gr][2], qf[0][gr][3], acc[0], acc[1], acc[2], acc[3]);
+                if constexpr (SPLIT) {
+                    kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[0], acc[1], acc[2], acc[3]);
+                    kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[1][gr][2], qf[1][gr][3], acc[0], acc[1], acc[2], acc[3]);
+                }
+                s[0] = fmaf(sz0.y, qs[gr][0], fmaf(sz0.x, acc[0], s[0]));
+                s[1] = fmaf(sz0.y, qs[gr][1], fmaf(sz0.x, acc[1], s[1]));
+                s[2] = fmaf(sz1.y, qs[gr][0], fmaf(sz1.x, acc[2], s[2]));
+                s[3] = fmaf(sz1.y, qs[gr][1], fmaf(sz1.x, acc[3], s[3]));
+            }
+        }
+        const bool in0 = at + g < p1, in1 = at + g + 8 < p1;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = (j < 2 ? in0 : in1) ? s[j] * rate[j & 1] : -INFINITY;
+        if (a.scores) {
+            float* dst = a.scores + (row0 + at) * a.gqa + tile8 * kKv4Heads + 2 * t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) dst[(long long)(g + (j >> 1) * 8) * a.gqa + (j & 1)] = s[j];
+        }
+        // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
+        float vs[2][NG], vz[2][NG], top[2] = {0x1p-24f, 0x1p-24f};
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                const uint32_t w = lds32(sv + (g + r * 8) * kRow + NG * 16 + gr * 4);
+                const float2 f = half2_bits_to_float2((r ? in1 : in0) ? w : 0u);
+                vs[r][gr] = f.x;
+                vz[r][gr] = f.y;
+                top[r] = fmaxf(top[r], f.x);
+            }
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? in0 : in1) ? exp2_fast(s[j] - m[j & 1]) : 0.f;
+        if (__any_sync(0xffffffffu, !(fmaxf(p[0], p[1]) * top[0] <= kKv4Limit) || !(fmaxf(p[2], p[3]) * top[1] <= kKv4Limit))) {
+            // move the reference: the largest product becomes 2^8 .. 2^9
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                float x = fmaxf(s[j] + (float)(ilogbf(top[0]) - 8), s[j + 2] + (float)(ilogbf(top[1]) - 8));
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                const float next = fmaxf(m[j], x), f = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - next);
+                m[j] = next;
+                l[j] *= f;
+#pragma unroll
+                for (int k = 0; k < 2 * NG; ++k) {
+                    o[k][j] *= f;
+                    o[k][j + 2] *= f;
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k) z[k][j] *= f;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? in0 : in1) ? exp2_fast(s[j] - m[j & 1]) : 0.f;
+        }
+        l[0] += p[0] + p[2];
+        l[1] += p[1] + p[3];
+        // ---- values
+        const uint32_t c0 = sv + 2 * t * kRow + g * 2;
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+            z[gr][0] = fmaf(p[2], vz[1][gr], fmaf(p[0], vz[0][gr], z[gr][0]));
+            z[gr][1] = fmaf(p[3], vz[1][gr], fmaf(p[1], vz[0][gr], z[gr][1]));
+            const float y0 = p[0] * vs[0][gr], y1 = p[1] * vs[0][gr], y2 = p[2] * vs[1][gr], y3 = p[3] * vs[1][gr];
+            const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
+            const uint32_t b0 = transpose8(*reinterpret_cast<const uint32_t*>(&ha)), b1 = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
+            const uint32_t ca = c0 + gr * 16;
+            const uint32_t xa = lds16(ca) | lds16(ca + kRow) << 16, xb = lds16(ca + 8 * kRow) | lds16(ca + 9 * kRow) << 16;
+            const uint32_t ya = xa >> 8, yb = xb >> 8;
+            const uint32_t a0 = kv4_low(xa), a1 = kv4_high(xa), a2 = kv4_low(xb), a3 = kv4_high(xb);
+            const uint32_t d0 = kv4_low(ya), d1 = kv4_high(ya), d2 = kv4_low(yb), d3 = kv4_high(yb);
+            float(&oa)[4] = o[2 * gr];
+            float(&ob)[4] = o[2 * gr + 1];
+            kv4_mma(oa, a0, a1, a2, a3, b0, b1, oa[0], oa[1], oa[2], oa[3]);
+            kv4_mma(ob, d0, d1, d2, d3, b0, b1, ob[0], ob[1], ob[2], ob[3]);
+            if constexpr (SPLIT) {
+                const float2 fa = __half22float2(ha), fb = __half22float2(hb);
+                const __half2 la = __floats2half2_rn(y0 - fa.x, y1 - fa.y), lb = __floats2half2_rn(y2 - fb.x, y3 - fb.y);
+                const uint32_t l0 = transpose8(*reinterpret_cast<const uint32_t*>(&la)), l1 = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
+                kv4_mma(oa, a0, a1, a2, a3, l0, l1, oa[0], oa[1], oa[2], oa[3]);
+                kv4_mma(ob, d0, d1, d2, d3, l0, l1, ob[0], ob[1], ob[2], ob[3]);
+            }
+        }
+        __syncwarp();
+        ++used;
+        if (lane == 0) request();
+    }
+    // ---- the warp's sums over its lanes, then the CTA's over its warps
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
+#pragma unroll
+        for (int k = 0; k < NG; ++k)
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) z[k][j] += __shfl_xor_sync(0xffffffffu, z[k][j], d);
+        if (g == 0) {
+            s_m[warp][2 * t + j] = m[j];
+            s_l[warp][2 * t + j] = l[j];
+        }
+    }
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j)  // tile 2 gr + k: rows g and g + 8 are dimensions 4 g + 2 k and the one after
+                so[(warp * kKv4Heads + 2 * t + (j & 1)) * kPitch + gr * 32 + 4 * g + 2 * k + (j >> 1)] = o[2 * gr + k][j] + z[gr][j & 1];
+    __syncthreads();
+    const bool whole = unit == 0 && mine == units;  // the head lies in this run; else a part: [1] begins here, [0] began earlier
+    const long long part = (long long)blockIdx.x * 2 + (unit == 0 ? 1 : 0);
+    for (int i = tid; i < n_heads * NG * 32; i += kKv4Threads) {
+        const int h = i / (NG * 32), d = i - h * (NG * 32);
+        float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, s_m[w][h]);
+#pragma unroll
+        for (int w = 0; w < kKv4Warps; ++w) {
+            const float f = s_m[w][h] == -INFINITY ? 0.f : exp2_fast(s_m[w][h] - top);
+            sum = fmaf(f, s_l[w][h], sum);
+            y = fmaf(f, so[(w * kKv4Heads + h) * kPitch + d], y);
+        }
+        const long long bh = (long long)b * a.heads + h0 + h;
+        if (!whole) {
+            a.part_o[(part * kKv4Heads + h) * (NG * 32) + d] = y;
+            if (d == 0) a.part_ml[part * kKv4Heads + h] = make_float2(top, sum);
+        } else {
+            if (d < a.head_size) store_typed(a.out, (long long)b * a.out_stride + (long long)(h0 + h) * a.head_size + d, a.dtype, len > 0 ? __fdiv_rn(y, sum) : 0.f);
+            if (d == 0 && a.whole_ml) a.whole_ml[bh] = make_float2(top, sum);
+        }
+    }
+    __syncthreads();  // the sums have been read
+    left -= mine;
+    unit += mine;
+    if (unit == units && left > 0) {
+        unit = 0;
+        if (++head == heads8) {
+            head = 0;
+            len = kv4_len(a, ++b);
+            units = kv4_units(len);
+        }
+    }
+    }
+    if (s_fail) {  // copies may still be in flight: a bounded time to land
+        const long long c0 = clock64();
+        while (clock64() - c0 < (1 << 17)) __nanosleep(1000);
+    }
+}
+
+// Puts the parts of heads together that lie in several runs, and adds the probabilities of a key/value head's queries to the sums of
+// its positions.  Grid (max(gqa, blocks of positions), kv_heads, batch).
+constexpr int kKv4FinishThreads = 256, kKv4FinishRows = 1024;
+template <int NG>
+static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(const Kv4AttnArgs a) {
+    extern __shared__ float s_fin[];  // [gqa][2]: reference, 1 / sum
+    op_begin();
+    const int tid = threadIdx.x, lane = tid & 31, kvh = blockIdx.y, b = blockIdx.z, heads8 = a.kv_heads * a.head_tiles;
+    const int len = kv4_len(a, b), units = kv4_units(len);
+    const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);
+    long long before = 0;
+    for (int i = lane; i < b; i += 32) before += kv4_units(kv4_len(a, i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    // runs that hold the first and the last unit of a head
+    auto runs_of = [&](int tile8, int& r0, int& r1) {
+        const long long u0 = before * heads8 + (long long)(kvh * a.head_tiles + tile8) * units, u1 = u0 + units - 1;
+        r0 = (int)(((u0 + 1) * runs - 1) / all);
+        r1 = (int)(((u1 + 1) * runs - 1) / all);
+    };
+    auto part_of = [&](int r, int r0, int h) { return ((long long)r * 2 + (r == r0 ? 1 : 0)) * kKv4Heads + h % kKv4Heads; };
+    for (int h = tid >> 5; h < a.gqa; h += kKv4FinishThreads / 32) {
+        int r0, r1;
+        runs_of(h / kKv4Heads, r0, r1);
+        float top = -INFINITY, sum = 0.f;
+        if (r0 == r1) {
+            if (a.whole_ml) {
+                const float2 ml = a.whole_ml[(long long)b * a.heads + kvh * a.gqa + h];
+                top = ml.x;
+                sum = ml.y;
+            }
+        } else {
+            for (int r = r0 + lane; r <= r1; r += 32) top = fmaxf(top, a.part_ml[part_of(r, r0, h)].x);
+            top = warp_max(top);
+            for (int r = r0 + lane; r <= r1; r += 32) {
+                const float2 ml = a.part_ml[part_of(r, r0, h)];
+                sum = fmaf(exp2_fast(ml.x - top), ml.y, sum);
+            }
+            sum = warp_sum(sum);
+        }
+        if (lane == 0) {
+            s_fin[2 * h] = top;
+            s_fin[2 * h + 1] = __fdiv_rn(1.f, sum);
+        }
+    }
+    __syncthreads();
+    if (blockIdx.x < a.gqa) {
+        const int h = blockIdx.x;
+        int r0, r1;
+        runs_of(h / kKv4Heads, r0, r1);
+        if (r0 < r1)
+            for (int d = tid; d < a.head_size; d += kKv4FinishThreads) {
+                float y = 0.f;
+                for (int r = r0; r <= r1; ++r) {
+                    const long long part = part_of(r, r0, h);
+                    y = fmaf(exp2_fast(a.part_ml[part].x - s_fin[2 * h]), a.part_o[part * (NG * 32) + d], y);
+                }
+                store_typed(a.out, (long long)b * a.out_stride + (long long)(kvh * a.gqa + h) * a.head_size + d, a.dtype, y * s_fin[2 * h + 1]);
+            }
+    }
+    if (a.sums_out) {
+        const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
+        const int end = (int)min((long long)len, (long long)(blockIdx.x + 1) * kKv4FinishRows);
+        for (int p = blockIdx.x * kKv4FinishRows + tid; p < end; p += kKv4FinishThreads) {
+            const float* x = a.scores + (row0 + p) * a.gqa;
+            float sum = 0.f;
+            for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - s_fin[2 * h]), s_fin[2 * h + 1], sum);
+            a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
+        }
+    }
+}
+
+// ------------------------------------------------------------------ eviction
+//
+// Keeps the `recent` last rows of every head and, of the rows before them, those with the largest sums (the lowest position first among
+// equals; a NaN counts as -infinity), in their order.  One CTA per head finds the smallest sum that stays, digit by digit, and writes
+// the list of kept rows; a second kernel moves them.
+constexpr int kKv4EvictThreads = 1024;
+
+struct Kv4EvictArgs {
+    const unsigned char *k, *v;
+    unsigned char *k_out, *v_out;
+    const float* sums;
+    float* sums_out;
+    int *kept, *lens_out;
+    const int* lens;
+    long long capacity, capacity_out;
+    int kv_heads, keep, recent, row_bytes;
+};
+
+// Order of the sums as unsigned integers
+__device__ __forceinline__ uint32_t kv4_rank(float x) {
+    const uint32_t u = x != x ? 0xff800000u : __float_as_uint(x + 0.f);  // (-0 becomes 0)
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_select_kernel(const Kv4EvictArgs a) {
+    __shared__ uint32_t hist[2048], warp_sums[32], s_digit, s_left;
+    op_begin();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.x, b = blockIdx.y;
+    const int len = (int)max(0ll, min((long long)a.lens[b], a.capacity)), stay = min(len, a.keep), old = max(0, len - a.recent);
+    const long long head = (long long)b * a.kv_heads + kvh;
+    const float* sums = a.sums + head * a.capacity;
+    int* kept = a.kept + head * a.keep;
+    if (kvh == 0 && tid == 0) a.lens_out[b] = stay;
+    const uint32_t choose = (uint32_t)max(0, stay - (len - old));  // of the `old` first rows
+    // the choose-th largest rank: digits of 11, 11 and 10 bits
+    uint32_t prefix = 0, mask = 0, left = choose;
+    if (choose > 0 && choose < (uint32_t)old) {
+        for (int pass = 0; pass < 3; ++pass) {
+            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+            const uint32_t digits = pass == 2 ? 1023u : 2047u;
+            for (int i = tid; i < 2048; i += kKv4EvictThreads) hist[i] = 0;
+            __syncthreads();
+            for (int i = tid; i < old; i += kKv4EvictThreads) {
+                const uint32_t r = kv4_rank(sums[i]);
+                if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & digits], 1u);
+            }
+            __syncthreads();
+            // digits from the top, two a thread
+            const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
+            uint32_t x = c0 + c1;
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+                if (lane >= d) x += y;
+            }
+            if (lane == 31) warp_sums[warp] = x;
+            __syncthreads();
+            for (int w = 0; w < warp; ++w) x += warp_sums[w];
+            const uint32_t before = x - c0 - c1;
+            if (before < left && left <= x) {
+                const bool first = left <= before + c0;
+                s_digit = (uint32_t)(first ? 2047 - 2 * tid : 2046 - 2 * tid);
+                s_left = left - before - (first ? 0u : c0);
+            }
+            __syncthreads();
+            prefix |= s_digit << shift;
+            mask |= digits << shift;
+            left = s_left;
+        }
+    }
+    // rows with a larger rank stay, of those that equal it the first `left`
+    const bool all = choose >= (uint32_t)old;
+    uint32_t n = 0, equal = 0;  // rows kept and equals seen so far
+    for (int i0 = 0; i0 < old; i0 += kKv4EvictThreads) {
+        const int i = i0 + tid;
+        const uint32_t r = i < old ? kv4_rank(sums[i]) : 0u;
+        const bool same = i < old && choose > 0 && !all && r == prefix, more = i < old && choose > 0 && (all || r > prefix);
+        uint32_t x = (same ? 1u << 16 : 0u) + (more ? 1u : 0u);
+        const uint32_t own = x;
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+            if (lane >= d) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sums[warp] = x;
+        __syncthreads();
+        uint32_t total = 0;
+        for (int w = 0; w < 32; ++w) {
+            if (w < warp) x += warp_sums[w];
+            total += warp_sums[w];
+        }
+        x -= own;
+        const uint32_t eq = equal + (x >> 16);  // equals before this row
+        const uint32_t at = n + (x & 0xffffu) + (all ? 0u : min(eq, left) - min(equal, left));
+        if (more || (same && eq < left)) kept[at] = i;
+        n += (total & 0xffffu) + (all ? 0u : min(equal + (total >> 16), left) - min(equal, left));
+        equal += total >> 16;
+    }
+    for (int i = tid; i < len - old && i < stay; i += kKv4EvictThreads) kept[stay - (len - old) + i] = old + i;
+}
+
+// V: bytes a thread moves at once (16, 8 or 4, by the row's size)
+template <typename V>
+static __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a) {
+    op_begin();
+    const int kvh = blockIdx.y, b = blockIdx.z, units = a.row_bytes / (int)sizeof(V);
+    const long long head = (long long)b * a.kv_heads + kvh;
+    const int stay = (int)max(0ll, min(min((long long)a.lens[b], a.capacity), (long long)a.keep));
+    const int* kept = a.kept + head * a.keep;
+    const V *k = reinterpret_cast<const V*>(a.k + head * a.capacity * a.row_bytes), *v = reinterpret_cast<const V*>(a.v + head * a.capacity * a.row_bytes);
+    V *ko = reinterpret_cast<V*>(a.k_out + head * a.capacity_out * a.row_bytes), *vo = reinterpret_cast<V*>(a.v_out + head * a.capacity_out * a.row_bytes);
+    const long long step = (long long)gridDim.x * blockDim.x, total = (long long)stay * units;
+    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
+        const int row = (int)(i / units), unit = (int)(i - (long long)row * units), from = kept[row];
+        ko[i] = k[(long long)from * units + unit];
+        vo[i] = v[(long long)from * units + unit];
+        if (unit == 0) a.sums_out[head * a.capacity_out + row] = a.sums[head * a.capacity + from];
+    }
+}
+
+}  // namespace lpp

@@ -1,0 +1,50 @@
+// Launching stand-alone operator kernels: shared by the files that hold their entry points.
+#pragma once
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "../../include/lpp_b200.h"
+
+namespace {
+
+inline lpp_status chk() { return cudaGetLastError() == cudaSuccess ? LPP_OK : LPP_ERR_CUDA; }
+inline cudaStream_t S(void* s) { return (cudaStream_t)s; }
+inline int blocks(long long n, int t) { return (int)std::max<long long>(1, (n + t - 1) / t); }
+
+// Launches an operator kernel.  It may start while the kernel before it in the stream ends (it waits for it in op_begin):
+// 18 operators of a layer one after the other take about a microsecond less each.  A stream that is being captured gets a plain
+// launch, because what comes before it in the graph need not be a kernel.  cluster: CTAs of a cluster along x.
+template <typename... KArgs, typename... Args>
+lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, Args... args) {
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &capturing) != cudaSuccess) {
+        (void)cudaGetLastError();
+        capturing = cudaStreamCaptureStatusActive;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2] = {};
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs].val.clusterDim.x = cluster;
+        attr[cfg.numAttrs].val.clusterDim.y = 1;
+        attr[cfg.numAttrs++].val.clusterDim.z = 1;
+    }
+    if (capturing == cudaStreamCaptureStatusNone) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    cfg.attrs = attr;
+    cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
+    return chk();
+}
+template <typename... KArgs, typename... Args>
+lpp_status launch_op(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+    return launch_op_cluster(kernel, grid, threads, smem, 1, s, args...);
+}
+
+}  // namespace

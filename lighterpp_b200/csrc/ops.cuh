@@ -10,12 +10,6 @@
 
 namespace lpp {
 
-// First statement of every operator kernel: nothing of the kernel before may be touched ahead of it.
-__device__ __forceinline__ void op_begin() {
-    pdl_launch_dependents();
-    pdl_wait();
-}
-
 // src/matmul.cu:150-161
 static __global__ void convert_f32_to_f16_kernel(__half* dst, const float* src, long long n) {
     op_begin();

@@ -10,6 +10,7 @@
 #include "../../include/lpp_b200.h"
 #include "common.cuh"
 #include "gemv.cuh"
+#include "op_launch.cuh"
 #include "ops.cuh"
 #include "sampler.cuh"
 #include "sampler_exact.cuh"
@@ -17,34 +18,6 @@
 using namespace lpp;
 
 namespace {
-
-inline lpp_status chk() { return cudaGetLastError() == cudaSuccess ? LPP_OK : LPP_ERR_CUDA; }
-inline cudaStream_t S(void* s) { return (cudaStream_t)s; }
-inline int blocks(long long n, int t) { return (int)std::max<long long>(1, (n + t - 1) / t); }
-
-// Launches an operator kernel.  It may start while the kernel before it in the stream ends (it waits for it in op_begin):
-// 18 operators of a layer one after the other take about a microsecond less each.  A stream that is being captured gets a plain
-// launch, because what comes before it in the graph need not be a kernel.
-template <typename... KArgs, typename... Args>
-lpp_status launch_op(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
-    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(s, &capturing) != cudaSuccess) {
-        (void)cudaGetLastError();
-        capturing = cudaStreamCaptureStatusActive;
-    }
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr = {};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = capturing == cudaStreamCaptureStatusNone ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
-    return chk();
-}
 
 // Any-shape fallback for the stand-alone GEMV: one warp per row, scalar loads.
 template <typename WT>
