@@ -359,8 +359,20 @@ lpp_status lpp_op_sample_static(float* d_logits, int vocab_size, float temperatu
 /* ---- attention operators beyond the reference's: prompts of several sequences, and a cache held in 4 bits -------------------
  *
  * No counterpart in the reference, which runs one sequence with an FP16 cache (src/model.cpp:121-209).  Device pointers, work is
- * queued on `stream`, nothing is allocated or synchronised; the current device is the one that holds the memory.
- *
+ * queued on `stream`, nothing is allocated or synchronised; the current device is the one that holds the memory. */
+
+/* Causal attention of n_sequences whole prompts that lie behind one another, d_offsets[n_sequences + 1] (on the device, ascending from
+ * 0; equal neighbours are empty prompts) being their first tokens and the end of the last: for a token i of a prompt
+ *     out[i][h] = sum_j softmax_j(scale q[i][h] . k[j][h / (n_heads / n_kv_heads)]) v[j][...] over its tokens j <= i.
+ * q and out are [token][n_heads][head_size], k and v [token][n_kv_heads][head_size], F16 or BF16, *_stride elements from one token to the
+ * next (a multiple of 8, at least a token's elements), on 16-byte boundaries; head sizes are multiples of 8 up to 128.  The arrays hold n_tokens tokens:
+ * results of those from d_offsets[n_sequences] on are left as they were, and their queries, keys and values are not looked at.  Scores and
+ * sums are FP32, probabilities are rounded to the type. */
+lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k, const void* d_v, const int* d_offsets, int n_sequences, int n_tokens,
+                                   int n_heads, int n_kv_heads, int head_size, int64_t out_stride, int64_t q_stride, int64_t k_stride,
+                                   int64_t v_stride, float scale, int dtype, void* stream);
+
+/*
  * The 4-bit cache of a layer is two arrays (keys, values) [batch][n_kv_heads][capacity] of rows of
  * lpp_op_kv4_row_bytes(head_size) bytes, on 16-byte boundaries, capacity a multiple of 4.  A row holds groups of 32 dimensions
  * (ceil(head_size / 32) of them; 8 where that is 5 to 7), lo and hi being the least and the largest value of a group:

@@ -8,6 +8,8 @@
 #include "common.cuh"
 #include "kv4.cuh"
 #include "op_launch.cuh"
+#include "prompt_attention.cuh"
+#include "tensor_map.h"
 
 using namespace lpp;
 
@@ -117,6 +119,61 @@ const char* attn_fault(int batch, int n_heads, int n_kv_heads, int64_t capacity,
 }  // namespace
 
 extern "C" {
+
+lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k, const void* d_v, const int* d_offsets, int n_sequences, int n_tokens, int n_heads,
+                                   int n_kv_heads, int head_size, int64_t out_stride, int64_t q_stride, int64_t k_stride, int64_t v_stride, float scale, int dtype, void* stream) {
+    if (n_sequences < 0 || n_tokens < 0 || n_tokens > (1 << 30)) return refuse("prompt attention: sizes out of range");
+    if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535) return refuse("prompt attention: the key/value heads divide the heads");
+    if (head_size <= 0 || head_size % 8 || head_size > 128) return refuse("prompt attention: head sizes are multiples of 8 up to 128");
+    if (dtype != LPP_F16 && dtype != LPP_BF16) return refuse("prompt attention: F16 or BF16");
+    if (!(scale > 0.f) || scale > 3.4e38f) return refuse("prompt attention: the scale is positive and finite");
+    if (n_sequences == 0 || n_tokens == 0) return LPP_OK;
+    if (!d_out || !d_q || !d_k || !d_v || !d_offsets) return refuse("prompt attention: null pointer");
+    if (((uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v) & 15 || (uintptr_t)d_offsets & 3)
+        return refuse("prompt attention: queries, keys, values and results start on 16-byte boundaries");
+    const int64_t rows = (int64_t)n_heads * head_size, kv_rows = (int64_t)n_kv_heads * head_size;
+    if (out_stride < rows || q_stride < rows || k_stride < kv_rows || v_stride < kv_rows || (out_stride | q_stride | k_stride | v_stride) % 8 ||
+        std::max(std::max(out_stride, q_stride), std::max(k_stride, v_stride)) > (1ll << 32))
+        return refuse("prompt attention: a token's heads fit its stride, a multiple of 8 elements");
+    const encode_tiled_fn encode = tensor_map_encoder();
+    if (!encode) return refuse("prompt attention: no CUDA device, or cuTensorMapEncodeTiled is not available from this driver", LPP_ERR_NO_DEVICE);
+    CUtensorMap q_map, k_map, v_map;
+    auto make = [&](CUtensorMap* m, const void* p, int heads, int64_t stride) {  // 128 tokens x 64 dimensions of a head a copy
+        const cuuint64_t dims[3] = {(cuuint64_t)head_size, (cuuint64_t)heads, (cuuint64_t)n_tokens};
+        const cuuint64_t strides[2] = {(cuuint64_t)head_size * 2, (cuuint64_t)stride * 2};
+        const cuuint32_t box[3] = {64u, 1u, (cuuint32_t)kPaRows}, estr[3] = {1, 1, 1};
+        return encode(m, dtype == LPP_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(p), dims, strides, box, estr,
+                      CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    };
+    if (!make(&q_map, d_q, n_heads, q_stride) || !make(&k_map, d_k, n_kv_heads, k_stride) || !make(&v_map, d_v, n_kv_heads, v_stride))
+        return refuse("prompt attention: cuTensorMapEncodeTiled failed", LPP_ERR_CUDA);
+    PromptAttnArgs a = {};
+    a.out = d_out;
+    a.v = d_v;
+    a.offsets = d_offsets;
+    a.out_stride = out_stride;
+    a.v_stride = v_stride;
+    a.n_sequences = n_sequences;
+    a.n_tokens = n_tokens;
+    a.heads = n_heads;
+    a.gqa = n_heads / n_kv_heads;
+    a.head_size = head_size;
+    a.pair_heads = a.gqa % 2 == 0;
+    const int cta_rows = a.pair_heads ? kPaRows : 2 * kPaRows, per_tile = a.pair_heads ? n_heads / 2 : n_heads;
+    a.tiles = (n_tokens + cta_rows - 1) / cta_rows;
+    a.rate = scale * 1.4426950408889634f;
+    if ((long long)a.tiles * per_tile > 0x7fffffffll) return refuse("prompt attention: too many tokens", LPP_ERR_TOO_LARGE);
+    auto go = [&](auto kernel, int smem) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+            (void)cudaGetLastError();
+            return LPP_ERR_CUDA;
+        }
+        return launch_op(kernel, dim3(a.tiles * per_tile), kPaThreads, smem, S(stream), q_map, k_map, v_map, a);
+    };
+    return launched("lpp_op_prompt_attention: the launch failed",
+                    head_size <= 64 ? (dtype == LPP_F16 ? go(prompt_attention_kernel<64, __half>, kPaSmem<64>) : go(prompt_attention_kernel<64, __nv_bfloat16>, kPaSmem<64>))
+                                    : (dtype == LPP_F16 ? go(prompt_attention_kernel<128, __half>, kPaSmem<128>) : go(prompt_attention_kernel<128, __nv_bfloat16>, kPaSmem<128>)));
+}
 
 int64_t lpp_op_kv4_row_bytes(int head_size) { return head_size <= 0 || head_size > 256 ? -1 : kv4_row_bytes(kv4_held_groups(head_size)); }
 

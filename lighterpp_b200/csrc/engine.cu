@@ -48,6 +48,7 @@
 #include "sampler.cuh"
 #include "sampler_exact.cuh"
 #include "shared_kv.cuh"
+#include "tensor_map.h"
 
 using namespace lpp;
 
@@ -2397,22 +2398,6 @@ extern "C" lpp_status lpp_sample_logits(lpp_engine* e, const float* h_logits, co
 }
 
 // ------------------------------------------------------------------ batched prompt path
-
-typedef CUresult (*encode_tiled_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                    const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static encode_tiled_fn tensor_map_encoder() {
-    static encode_tiled_fn encode = nullptr;
-    if (!encode) {
-        cudaDriverEntryPointQueryResult qr;
-        void* fn = nullptr;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &qr) == cudaSuccess && fn &&
-            qr == cudaDriverEntryPointSuccess)
-            encode = (encode_tiled_fn)fn;
-    }
-    return encode;
-}
 
 // Tensor maps over row-major FP16 matrices of THIS GPU's memory, cut into pieces of 64 inputs (128 bytes, stored with
 // the 128-byte swizzle: the K-major operand layout of the MMA descriptors).  cols must be a multiple of 64; elements

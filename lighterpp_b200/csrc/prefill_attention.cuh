@@ -59,7 +59,6 @@ __device__ __forceinline__ uint64_t fa_desc_mn(uint32_t smem_addr) {
 __host__ __device__ constexpr uint32_t fa_idesc(int n, bool b_mn_major) {  // as umma_idesc, FP16, M = 128
     return (1u << 4) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 template <int HS>
 static __global__ void __launch_bounds__(kFaThreads, 1) prefill_attention_umma_kernel(const __grid_constant__ CUtensorMap k_map,

@@ -44,6 +44,7 @@ def _lib():
         lib.lpp_op_sample_on.argtypes = [vp, i64, vp, i, f, f, vp, i, f, vp, vp]
         lib.lpp_op_sample_scratch_bytes.argtypes = [i]
         lib.lpp_op_sample_scratch_bytes.restype = i64
+        lib.lpp_op_prompt_attention.argtypes = [vp, vp, vp, vp, vp, i, i, i, i, i, i64, i64, i64, i64, f, i, vp]
         lib.lpp_op_kv4_row_bytes.argtypes = [i]
         lib.lpp_op_kv4_row_bytes.restype = i64
         lib.lpp_op_kv4_write.argtypes = [vp, vp, vp, vp, vp, i, i, i, i64, i, i64, i64, i, vp]
@@ -169,6 +170,21 @@ def _cache(what, k, v, head_size):
     _want(what, k, torch.uint8, tuple(k.shape[:3]) + (row,))
     _want(what, v, torch.uint8, k.shape)
     return k.shape[:3]
+
+
+def cuda_prompt_attention(d_out, d_q, d_k, d_v, d_offsets, scale):
+    """Causal attention of packed prompts: ``d_q``, ``d_out`` [tokens, heads, head_size], ``d_k``, ``d_v`` [tokens, kv heads, head_size] (F16
+    or BF16); ``d_offsets`` (int32, prompts + 1) has the first token of each prompt and the end of the last.  Tokens behind are left as they were."""
+    with _same_device(d_q, d_out, d_k, d_v, d_offsets):
+        qs = _heads("cuda_prompt_attention", d_q)
+        outs = _heads("cuda_prompt_attention", d_out, d_q.dtype, d_q.shape)
+        ks = _heads("cuda_prompt_attention", d_k, d_q.dtype)
+        vs = _heads("cuda_prompt_attention", d_v, d_q.dtype, d_k.shape)
+        if d_k.shape[0] != d_q.shape[0] or d_k.shape[2] != d_q.shape[2] or d_offsets.dim() != 1 or d_offsets.shape[0] < 1:
+            raise ValueError("cuda_prompt_attention: as many keys as queries, of one head size, and offsets of prompts + 1")
+        _want("cuda_prompt_attention", d_offsets, torch.int32, d_offsets.shape)
+        _check(_lib().lpp_op_prompt_attention(_raw(d_out), _raw(d_q), _raw(d_k), _raw(d_v), _raw(d_offsets), d_offsets.shape[0] - 1, d_q.shape[0], d_q.shape[1], d_k.shape[1],
+                                              d_q.shape[2], outs, qs, ks, vs, float(scale), _DTYPES[d_q.dtype], _s()), "cuda_prompt_attention")
 
 
 def kv4_row_bytes(head_size):
