@@ -93,8 +93,9 @@ lpp_status rows_op(const char* name, const void* k, const void* v, const int64_t
     return launched(name, launch(c, groups, dim3((unsigned)ctas, 2), rows, wide));
 }
 
-// ---- attention over the 4-bit cache: runs of work (one CTA an SM) and the scratch
-int attn_runs(int batch, int n_heads, int n_kv_heads, int64_t capacity, int sms) {
+// ---- attention over the 4-bit cache: runs of work (one a CTA, as many CTAs as the SMs hold) and the scratch
+int attn_runs(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int sms) {
+    sms *= kv4_held_groups(head_size) > 4 ? kKv4Ctas<8> : kKv4Ctas<4>;
     const int head_tiles = (n_heads / n_kv_heads + kKv4Heads - 1) / kKv4Heads;
     return (int)std::min<long long>(sms, (long long)batch * n_kv_heads * head_tiles * ((capacity + kKv4Unit - 1) / kKv4Unit));
 }
@@ -208,7 +209,7 @@ lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const vo
 int64_t lpp_op_kv4_attention_scratch_bytes(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int with_sums) {
     const int sms = sm_count();
     if (sms <= 0 || attn_fault(batch, n_heads, n_kv_heads, capacity, head_size)) return -1;
-    return (int64_t)attn_layout(attn_runs(batch, n_heads, n_kv_heads, capacity, sms), batch, n_heads, capacity, kv4_held_groups(head_size), with_sums != 0).total;
+    return (int64_t)attn_layout(attn_runs(batch, n_heads, n_kv_heads, capacity, head_size, sms), batch, n_heads, capacity, kv4_held_groups(head_size), with_sums != 0).total;
 }
 
 lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_out, const void* d_q, const void* d_k_cache, const void* d_v_cache, const int* d_lens,
@@ -226,7 +227,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     if (d_sums_in && !d_sums_out) return refuse("4-bit attention: sums go in but not out");
     const int sms = sm_count();
     if (sms <= 0) return refuse("4-bit attention: no CUDA device", LPP_ERR_NO_DEVICE);
-    const int groups = kv4_held_groups(head_size), runs = attn_runs(batch, n_heads, n_kv_heads, capacity, sms);
+    const int groups = kv4_held_groups(head_size), runs = attn_runs(batch, n_heads, n_kv_heads, capacity, head_size, sms);
     const AttnLayout L = attn_layout(runs, batch, n_heads, capacity, groups, d_sums_out != nullptr);
     if (scratch_bytes < (int64_t)L.total) return refuse("4-bit attention: scratch is smaller than lpp_op_kv4_attention_scratch_bytes() says");
     char* w = (char*)scratch;
@@ -265,8 +266,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
                         const lpp_status st = launch_op(kernel, dim3(runs), kKv4Threads, smem, S(stream), a);
                         if (st != LPP_OK) return st;
                         const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;
-                        return launch_op(kv4_finish_kernel<NG>, dim3((unsigned)std::max<long long>(a.gqa, rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)a.gqa * 8, S(stream),
-                                         a);
+                        return launch_op(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + runs) * 4, S(stream), a);
                     }));
 }
 

@@ -166,7 +166,8 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(Kv4Cach
 // n 2^-24, and the same bits four places up are 16 n 2^-24, so a mask makes two elements of an operand register (the query elements of
 // the second kind are divided by 16).  Sums are kept apart by group and multiplied with the group's scale in FP32:
 //     q . k = sum_g scale_g (sum_d q_d n_d - 8 Q_g) + zero_g Q_g,  Q_g = sum_d q_d;
-// -8 Q_g is where the accumulator starts.  For the values the scale goes to the probability before that is rounded to FP16, the codes
+// -8 Q_g is where the accumulator starts, and the zeros' part is one more product, of the (scale, zero) pairs as they lie in the row with
+// (0, Q_g), Q_g as two FP16 operands.  For the values the scale goes to the probability before that is rounded to FP16, the codes
 // become n - 8 (rounding errors then are those of values around their middle), and sum_j p_j zero_jg is added in FP32.
 //
 // Reference of the exponentials: not the running maximum of the scores but a bound on the largest p * scale, which has to stay in the
@@ -180,7 +181,9 @@ constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
 constexpr int kKv4Heads = 8;     // query heads of a CTA
 constexpr float kKv4Limit = 32768.f;  // of p * scale
 template <int NG>
-constexpr int kKv4Stages = NG > 4 ? 3 : 6;  // tiles in flight per warp
+constexpr int kKv4Stages = NG > 3 ? 3 : 4;  // tiles in flight per warp
+template <int NG>
+constexpr int kKv4Ctas = NG > 4 ? 1 : 2;    // of an SM
 
 struct Kv4AttnArgs {
     const unsigned char *k, *v;
@@ -201,31 +204,35 @@ struct Kv4AttnArgs {
 
 __device__ __forceinline__ int kv4_len(const Kv4AttnArgs& a, int b) { return (int)max(0ll, min((long long)a.lens[b], a.capacity)); }
 __device__ __forceinline__ int kv4_units(int len) { return max(1, (len + kKv4Unit - 1) / kKv4Unit); }  // (an empty sequence has results to write)
-// Units of all sequences for one head, by a warp.
+// What a head weighs where work is dealt out: its units, and as many again as loading its queries and putting its warps together take.
+// Point kKv4Head + u of a head stands for unit u, the points before for its beginning.
+constexpr int kKv4Head = 4;
+__device__ __forceinline__ int kv4_weight(int len) { return kv4_units(len) + kKv4Head; }
+// Weight of all sequences for one head, by a warp.
 __device__ __forceinline__ long long kv4_total(const Kv4AttnArgs& a) {
     long long n = 0;
-    for (int b = threadIdx.x & 31; b < a.batch; b += 32) n += kv4_units(kv4_len(a, b));
+    for (int b = threadIdx.x & 31; b < a.batch; b += 32) n += kv4_weight(kv4_len(a, b));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
     return n;
 }
-// Sequence that holds unit `unit` of all, and its first unit, by a warp; `heads` counts a key/value head once per eight query heads.
-__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, long long unit, long long& first) {
+// Sequence that holds point `at` of all, and its first point, by a warp; `heads` counts a key/value head once per eight query heads.
+__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, long long at, long long& first) {
     const int lane = threadIdx.x & 31;
     long long base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const long long own = b0 + lane < a.batch ? (long long)kv4_units(kv4_len(a, b0 + lane)) * heads : 0;
+        const long long own = b0 + lane < a.batch ? (long long)kv4_weight(kv4_len(a, b0 + lane)) * heads : 0;
         long long x = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        const unsigned there = __ballot_sync(0xffffffffu, base + x > unit);
+        const unsigned there = __ballot_sync(0xffffffffu, base + x > at);
         if (there) {
-            const int at = __ffs(there) - 1;
-            first = base + __shfl_sync(0xffffffffu, x - own, at);
-            return b0 + at;
+            const int from = __ffs(there) - 1;
+            first = base + __shfl_sync(0xffffffffu, x - own, from);
+            return b0 + from;
         }
         base += __shfl_sync(0xffffffffu, x, 31);
     }
@@ -282,6 +289,49 @@ __device__ __forceinline__ uint32_t lds16(uint32_t a) {
     asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(a));
     return r;
 }
+// Scales and zeros of a row, a word a group
+template <int NG>
+__device__ __forceinline__ void kv4_params(uint32_t a, uint32_t (&w)[NG]) {
+    if constexpr (NG % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < NG; i += 4) asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "r"(a + i * 4));
+    } else if constexpr (NG == 2) {
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    } else {
+#pragma unroll
+        for (int i = 0; i < NG; ++i) w[i] = lds32(a + i * 4);
+    }
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t a, uint32_t (&r)[4]) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a));
+}
+// Words of the codes of a tile, [group][half of the rows].  Keys: word t of rows g and g + 8.  Values: 16-bit piece g of rows 2 t (lower
+// half) and 2 t + 1, and of the rows 8 further.
+template <int NG, bool VALUES>
+__device__ __forceinline__ void kv4_codes(uint32_t tile, int lane, uint32_t (&w)[NG][2]) {
+    constexpr int kRow = kv4_row_bytes(NG);
+    if constexpr (kRow % 16 == 0) {
+        const uint32_t a = tile + ((lane & 7) + (lane & 8)) * kRow + (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < NG; i += 2) {
+            uint32_t r[4];
+            ldmatrix4<VALUES>(a + i * 16, r);
+            w[i][0] = r[0], w[i][1] = r[1], w[i + 1][0] = r[2], w[i + 1][1] = r[3];
+        }
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+        const uint32_t a = VALUES ? tile + 2 * t * kRow + g * 2 : tile + g * kRow + t * 4;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                w[i][h] = VALUES ? lds16(a + i * 16 + h * 8 * kRow) | lds16(a + i * 16 + (h * 8 + 1) * kRow) << 16 : lds32(a + i * 16 + h * 8 * kRow);
+    }
+}
 // (n - 8) of the codes in bits 0-3 and 16-19, and in bits 4-7 and 20-23: 1024 + n - 1032, (1024 + 16 n) / 16 - 72, both exact
 __device__ __forceinline__ uint32_t kv4_low(uint32_t x) {
     const uint32_t b = (x & 0x000f000fu) | 0x64006400u, off = 0x64086408u;
@@ -295,17 +345,33 @@ __device__ __forceinline__ uint32_t kv4_high(uint32_t x) {
 }
 
 template <int NG, bool SPLIT>
-static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const Kv4AttnArgs a) {
+static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int kRow = kv4_row_bytes(NG), kTileBytes = kKv4Tile * kRow, kParts = SPLIT ? 2 : 1, kStages = kKv4Stages<NG>, kPitch = kKv4Pitch<NG>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kKv4Warps][kKv4Heads], s_l[kKv4Warps][kKv4Heads];
     __shared__ int s_fail;
-    op_begin();
+    pdl_wait();
+    pdl_launch_dependents();  // (after the wait: what the finishing kernel reads of the lengths is there when it starts)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int heads8 = a.kv_heads * a.head_tiles;
     const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);  // (no run is empty)
     if (blockIdx.x >= runs) return;
-    const long long begin = all * blockIdx.x / runs, end = all * (blockIdx.x + 1) / runs;
+    // (sequence, head, unit) of a point
+    struct Place {
+        int b, len, head, unit;
+    };
+    auto place = [&](long long at) {
+        long long first = 0;
+        Place p;
+        p.b = kv4_find(a, heads8, at, first);
+        p.len = p.b < a.batch ? kv4_len(a, p.b) : 0;
+        const int weight = kv4_weight(p.len);
+        p.head = (int)((at - first) / weight);
+        p.unit = max(0, (int)(at - first - (long long)p.head * weight) - kKv4Head);
+        return p;
+    };
+    const Place p_begin = place(all * blockIdx.x / runs), p_end = place(all * (blockIdx.x + 1) / runs);
+    if (p_begin.b == p_end.b && p_begin.head == p_end.head && p_begin.unit == p_end.unit) return;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kKv4RingBytes<NG>) + warp * kStages;
     float* so = reinterpret_cast<float*>(smem + kKv4RingBytes<NG> + kKv4Warps * kStages * 8);
     unsigned char* ring = smem + warp * kStages * 2 * kTileBytes;
@@ -315,47 +381,55 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
         mbar_fence_init();
     }
     __syncthreads();
-    long long first = 0;
-    int b = kv4_find(a, heads8, begin, first), len = kv4_len(a, b), units = kv4_units(len);
-    int head = (int)((begin - first) / units), unit = (int)(begin - first - (long long)head * units);
-    const int here = (int)(end - begin);
+    int b = p_begin.b, len = p_begin.len, units = kv4_units(len), head = p_begin.head, unit = p_begin.unit;
 
-    // lane 0: requests this warp's tiles in their order, as far as the ring reaches
-    int ahead_b = b, ahead_len = len, ahead_units = units, ahead_head = head, ahead_unit = unit, ahead_left = here, asked = 0, used = 0;
+    // lane 0: requests this warp's next tile, if there is one
+    int ahead_b = b, ahead_len = len, ahead_end = units * kKv4Unit, ahead_head = head, ahead_at = unit * kKv4Unit + warp * kKv4Tile, put = 0;
+    auto head_row = [&](int seq, int h8) { return ((long long)seq * a.kv_heads + h8 / a.head_tiles) * a.capacity; };
+    long long ahead_row = head_row(b, head);
     auto request = [&]() {
-        while (ahead_left > 0 && asked - used < kStages) {
-            const int at = ahead_unit * kKv4Unit + warp * kKv4Tile;
-            if (at < ahead_len) {
-                const int stage = asked % kStages;
-                const long long row = ((long long)ahead_b * a.kv_heads + ahead_head / a.head_tiles) * a.capacity + at;
+        for (;;) {
+            const int at = ahead_at;
+            const bool last = ahead_b == p_end.b && ahead_head == p_end.head;
+            if (ahead_b > p_end.b || (last && at >= p_end.unit * kKv4Unit)) return;
+            const bool there = at < ahead_len;
+            if (there) {
+                const long long from = (ahead_row + at) * kRow;
                 const uint32_t bytes = (uint32_t)min((long long)kKv4Tile, a.capacity - at) * kRow;  // (a multiple of four rows)
-                mbar_arrive_expect_tx(&bars[stage], 2 * bytes);
-                bulk_g2s(ring + stage * 2 * kTileBytes, a.k + row * kRow, bytes, &bars[stage]);
-                bulk_g2s(ring + stage * 2 * kTileBytes + kTileBytes, a.v + row * kRow, bytes, &bars[stage]);
-                ++asked;
+                unsigned char* to = ring + put * 2 * kTileBytes;
+                mbar_arrive_expect_tx(&bars[put], 2 * bytes);
+                bulk_g2s(to, a.k + from, bytes, &bars[put]);
+                bulk_g2s(to + kTileBytes, a.v + from, bytes, &bars[put]);
+                if (++put == kStages) put = 0;
             }
-            --ahead_left;
-            if (++ahead_unit == ahead_units) {
-                ahead_unit = 0;
-                if (++ahead_head == heads8 && ahead_left > 0) {
+            if ((ahead_at += kKv4Unit) >= ahead_end) {  // the next head
+                ahead_at = warp * kKv4Tile;
+                if (++ahead_head == heads8) {
                     ahead_head = 0;
-                    ahead_len = kv4_len(a, ++ahead_b);
-                    ahead_units = kv4_units(ahead_len);
+                    if (++ahead_b < a.batch) ahead_len = kv4_len(a, ahead_b);
+                    ahead_end = kv4_units(ahead_len) * kKv4Unit;
                 }
+                ahead_row = head_row(ahead_b, ahead_head);
             }
+            if (there) break;
         }
     };
-    if (lane == 0) request();
+    if (lane == 0)
+        for (int i = 0; i < kStages; ++i) request();
     bool ok = true;
+    int stage = 0;
+    uint32_t phase = 0;
 
-    for (int left = here; left > 0;) {
+    while (b < p_end.b || (b == p_end.b && (head < p_end.head || (head == p_end.head && unit < p_end.unit)))) {
     const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
     const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
     const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
-    const int mine = min(units - unit, left), p1 = len;
-    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^13 .. 2^14
+    const int mine = (b == p_end.b && head == p_end.head ? p_end.unit : units) - unit, p1 = len;
+    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^9 .. 2^10 (their sums
+    // over a group stay in the FP16 range)
     uint32_t qf[kParts][NG][4];
-    float qs[NG][2], rate[2];  // sums of a group and factor of the scores, heads 2 t and 2 t + 1
+    float start[NG][2], rate[2];  // where a group's accumulator starts, and factor of the scores, heads 2 t and 2 t + 1
+    uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of the zeros, head g: (0, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
     {
         float x[NG][8], top = 0.f;
         const bool some = g < n_heads;
@@ -370,7 +444,7 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // exponents of 2 in two halves, either within the normal range
-        const int e = top > 0.f && top < INFINITY ? 13 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
+        const int e = top > 0.f && top < INFINITY ? 9 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
         const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
         float sums[NG];
 #pragma unroll
@@ -393,7 +467,7 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sums[i] = sum * 0x1p-24f;  // the codes' factor
+            sums[i] = sum;
         }
         // 2^24 / 2^e, back from the operands' factors
         const float back = __int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * 0x1p24f * a.rate;
@@ -402,7 +476,17 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
             const int from = (2 * t + j) * 4;
             rate[j] = __shfl_sync(0xffffffffu, back, from);
 #pragma unroll
-            for (int i = 0; i < NG; ++i) qs[i][j] = __shfl_sync(0xffffffffu, sums[i], from);
+            for (int i = 0; i < NG; ++i) start[i][j] = -8.f * 0x1p-24f * __shfl_sync(0xffffffffu, sums[i], from);
+        }
+        float own[NG > 4 ? 2 : 1] = {};
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+            if ((i & 3) == t) own[i >> 2] = sums[i];
+#pragma unroll
+        for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
+            const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
+            zf[0][i] = (uint32_t)__half_as_ushort(hi) << 16;
+            zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = (uint32_t)__half_as_ushort(lo) << 16;
         }
     }
 
@@ -414,10 +498,9 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
 #pragma unroll
     for (int i = 0; i < NG; ++i) z[i][0] = z[i][1] = 0.f;
 
-    for (int i = 0; i < mine; ++i) {
-        const int at = (unit + i) * kKv4Unit + warp * kKv4Tile, stage = used % kStages;
-        if (at >= p1) continue;
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&bars[stage], (uint32_t)(used / kStages) & 1u, nullptr));
+    float* scores = a.scores ? a.scores + (row0 + unit * kKv4Unit + warp * kKv4Tile + g) * a.gqa + tile8 * kKv4Heads + 2 * t : nullptr;
+    for (int i = 0, at = unit * kKv4Unit + warp * kKv4Tile; i < mine && at < p1; ++i, at += kKv4Unit) {
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&bars[stage], phase, nullptr));
         if (!ok) {  // a copy that never came: the results of this run say so
             m[0] = m[1] = NAN;
             s_fail = 1;
@@ -425,49 +508,64 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
         }
         const uint32_t sk = smem_u32(ring + stage * 2 * kTileBytes), sv = sk + kTileBytes;
         // ---- scores of rows g and g + 8
-        float s[4] = {};
+        float s[4];
         {
-            const uint32_t r0 = sk + g * kRow, r1 = r0 + 8 * kRow;
+            uint32_t w[NG][2], p0[NG], p1w[NG];
+            kv4_codes<NG, false>(sk, lane, w);
+            const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
+            kv4_params<NG>(r0, p0);
+            kv4_params<NG>(r1, p1w);
+            // zeros first: rows of (scale, zero) pairs as they lie there times (0, Q)
+            float acc[4];
+            if constexpr (NG > 4) {
+                const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
+                kv4_mma(acc, a0, a1, a2, a3, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+                kv4_mma(acc, a0, a1, a2, a3, zf[1][0], zf[1][1], acc[0], acc[1], acc[2], acc[3]);
+            } else {
+                const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
+                kv4_mma(acc, a0, a1, a0, a1, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] = acc[j] * 0x1p-24f;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const uint32_t w0 = lds32(r0 + gr * 16 + t * 4), w1 = lds32(r1 + gr * 16 + t * 4);
-                const float2 sz0 = half2_bits_to_float2(lds32(r0 + NG * 16 + gr * 4)), sz1 = half2_bits_to_float2(lds32(r1 + NG * 16 + gr * 4));
-                const float c0 = -8.f * qs[gr][0], c1 = -8.f * qs[gr][1];
-                float acc[4];
-                const uint32_t v0 = w0 >> 8, v1 = w1 >> 8;
-                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], c0, c1, c0, c1);
+                const uint32_t w0 = w[gr][0], w1 = w[gr][1], v0 = w0 >> 8, v1 = w1 >> 8;
+                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], start[gr][0], start[gr][1], start[gr][0], start[gr][1]);
                 kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[0][gr][2], qf[0][gr][3], acc[0], acc[1], acc[2], acc[3]);
                 if constexpr (SPLIT) {
                     kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[0], acc[1], acc[2], acc[3]);
                     kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[1][gr][2], qf[1][gr][3], acc[0], acc[1], acc[2], acc[3]);
                 }
-                s[0] = fmaf(sz0.y, qs[gr][0], fmaf(sz0.x, acc[0], s[0]));
-                s[1] = fmaf(sz0.y, qs[gr][1], fmaf(sz0.x, acc[1], s[1]));
-                s[2] = fmaf(sz1.y, qs[gr][0], fmaf(sz1.x, acc[2], s[2]));
-                s[3] = fmaf(sz1.y, qs[gr][1], fmaf(sz1.x, acc[3], s[3]));
+                const float s0 = __half2float(__ushort_as_half((unsigned short)p0[gr])), s1 = __half2float(__ushort_as_half((unsigned short)p1w[gr]));
+                s[0] = fmaf(s0, acc[0], s[0]);
+                s[1] = fmaf(s0, acc[1], s[1]);
+                s[2] = fmaf(s1, acc[2], s[2]);
+                s[3] = fmaf(s1, acc[3], s[3]);
             }
         }
         const bool in0 = at + g < p1, in1 = at + g + 8 < p1;
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[j] = (j < 2 ? in0 : in1) ? s[j] * rate[j & 1] : -INFINITY;
         if (a.scores) {
-            float* dst = a.scores + (row0 + at) * a.gqa + tile8 * kKv4Heads + 2 * t;
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) dst[(long long)(g + (j >> 1) * 8) * a.gqa + (j & 1)] = s[j];
+                if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) scores[(j >> 1) * 8 * a.gqa + (j & 1)] = s[j];
+            scores += (long long)kKv4Unit * a.gqa;
         }
         // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
         float vs[2][NG], vz[2][NG], top[2] = {0x1p-24f, 0x1p-24f};
 #pragma unroll
-        for (int r = 0; r < 2; ++r)
+        for (int r = 0; r < 2; ++r) {
+            uint32_t w[NG];
+            kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, w);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const uint32_t w = lds32(sv + (g + r * 8) * kRow + NG * 16 + gr * 4);
-                const float2 f = half2_bits_to_float2((r ? in1 : in0) ? w : 0u);
+                const float2 f = half2_bits_to_float2((r ? in1 : in0) ? w[gr] : 0u);
                 vs[r][gr] = f.x;
                 vz[r][gr] = f.y;
                 top[r] = fmaxf(top[r], f.x);
             }
+        }
         float p[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? in0 : in1) ? exp2_fast(s[j] - m[j & 1]) : 0.f;
@@ -495,7 +593,8 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
         l[0] += p[0] + p[2];
         l[1] += p[1] + p[3];
         // ---- values
-        const uint32_t c0 = sv + 2 * t * kRow + g * 2;
+        uint32_t codes[NG][2];
+        kv4_codes<NG, true>(sv, lane, codes);
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
             z[gr][0] = fmaf(p[2], vz[1][gr], fmaf(p[0], vz[0][gr], z[gr][0]));
@@ -503,8 +602,7 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
             const float y0 = p[0] * vs[0][gr], y1 = p[1] * vs[0][gr], y2 = p[2] * vs[1][gr], y3 = p[3] * vs[1][gr];
             const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
             const uint32_t b0 = transpose8(*reinterpret_cast<const uint32_t*>(&ha)), b1 = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
-            const uint32_t ca = c0 + gr * 16;
-            const uint32_t xa = lds16(ca) | lds16(ca + kRow) << 16, xb = lds16(ca + 8 * kRow) | lds16(ca + 9 * kRow) << 16;
+            const uint32_t xa = codes[gr][0], xb = codes[gr][1];
             const uint32_t ya = xa >> 8, yb = xb >> 8;
             const uint32_t a0 = kv4_low(xa), a1 = kv4_high(xa), a2 = kv4_low(xb), a3 = kv4_high(xb);
             const uint32_t d0 = kv4_low(ya), d1 = kv4_high(ya), d2 = kv4_low(yb), d3 = kv4_high(yb);
@@ -521,8 +619,11 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
             }
         }
         __syncwarp();
-        ++used;
         if (lane == 0) request();
+        if (++stage == kStages) {
+            stage = 0;
+            phase ^= 1u;
+        }
     }
     // ---- the warp's sums over its lanes, then the CTA's over its warps
 #pragma unroll
@@ -569,15 +670,16 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
         }
     }
     __syncthreads();  // the sums have been read
-    left -= mine;
     unit += mine;
-    if (unit == units && left > 0) {
+    if (unit == units) {
         unit = 0;
         if (++head == heads8) {
             head = 0;
-            len = kv4_len(a, ++b);
+            if (++b < a.batch) len = kv4_len(a, b);
             units = kv4_units(len);
         }
+    } else {
+        break;
     }
     }
     if (s_fail) {  // copies may still be in flight: a bounded time to land
@@ -586,29 +688,39 @@ static __global__ void __launch_bounds__(kKv4Threads, 1) kv4_attn_kernel(const K
     }
 }
 
-// Puts the parts of heads together that lie in several runs, and adds the probabilities of a key/value head's queries to the sums of
-// its positions.  Grid (max(gqa, blocks of positions), kv_heads, batch).
-constexpr int kKv4FinishThreads = 256, kKv4FinishRows = 1024;
+// Puts the parts of heads together that lie in several runs (the first gqa blocks of a key/value head), and adds the probabilities of its
+// queries to the sums of its positions (the others).  Grid (gqa + blocks of positions, kv_heads, batch).
+constexpr int kKv4FinishThreads = 256, kKv4FinishRows = 512;
 template <int NG>
 static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(const Kv4AttnArgs a) {
-    extern __shared__ float s_fin[];  // [gqa][2]: reference, 1 / sum
-    op_begin();
-    const int tid = threadIdx.x, lane = tid & 31, kvh = blockIdx.y, b = blockIdx.z, heads8 = a.kv_heads * a.head_tiles;
-    const int len = kv4_len(a, b), units = kv4_units(len);
+    extern __shared__ float s_fin[];  // [gqa][2]: reference, 1 / sum; then [runs]: weights of the parts
+    __shared__ float s_part[kKv4FinishThreads / 32][NG * 32];
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, b = blockIdx.z, heads8 = a.kv_heads * a.head_tiles;
+    const int len = kv4_len(a, b), units = kv4_units(len), weight = kv4_weight(len), row_block = (int)blockIdx.x - a.gqa;
     const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);
     long long before = 0;
-    for (int i = lane; i < b; i += 32) before += kv4_units(kv4_len(a, i));
+    for (int i = lane; i < b; i += 32) before += kv4_weight(kv4_len(a, i));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
     // runs that hold the first and the last unit of a head
     auto runs_of = [&](int tile8, int& r0, int& r1) {
-        const long long u0 = before * heads8 + (long long)(kvh * a.head_tiles + tile8) * units, u1 = u0 + units - 1;
+        const long long u0 = before * heads8 + (long long)(kvh * a.head_tiles + tile8) * weight + kKv4Head, u1 = u0 + units - 1;
         r0 = (int)(((u0 + 1) * runs - 1) / all);
         r1 = (int)(((u1 + 1) * runs - 1) / all);
     };
     auto part_of = [&](int r, int r0, int h) { return ((long long)r * 2 + (r == r0 ? 1 : 0)) * kKv4Heads + h % kKv4Heads; };
-    for (int h = tid >> 5; h < a.gqa; h += kKv4FinishThreads / 32) {
-        int r0, r1;
+    int r0, r1;
+    if (row_block < 0) {
+        runs_of((int)blockIdx.x / kKv4Heads, r0, r1);
+        if (r0 == r1) {
+            pdl_wait();
+            return;  // written already
+        }
+    }
+    pdl_wait();
+    // reference and sum of the head, or of all heads where their probabilities are wanted
+    for (int h = row_block < 0 ? (int)blockIdx.x + warp : warp; h < (row_block < 0 ? (int)blockIdx.x + 1 : a.gqa); h += kKv4FinishThreads / 32) {
         runs_of(h / kKv4Heads, r0, r1);
         float top = -INFINITY, sum = 0.f;
         if (r0 == r1) {
@@ -618,11 +730,19 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
                 sum = ml.y;
             }
         } else {
-            for (int r = r0 + lane; r <= r1; r += 32) top = fmaxf(top, a.part_ml[part_of(r, r0, h)].x);
+            float2 ml = make_float2(-INFINITY, 0.f);
+            if (r0 + lane <= r1) ml = a.part_ml[part_of(r0 + lane, r0, h)];
+            top = ml.x;
+            for (int r = r0 + 32 + lane; r <= r1; r += 32) top = fmaxf(top, a.part_ml[part_of(r, r0, h)].x);
             top = warp_max(top);
-            for (int r = r0 + lane; r <= r1; r += 32) {
-                const float2 ml = a.part_ml[part_of(r, r0, h)];
-                sum = fmaf(exp2_fast(ml.x - top), ml.y, sum);
+            const float w = exp2_fast(ml.x - top);
+            sum = w * ml.y;
+            if (row_block < 0 && r0 + lane <= r1) s_fin[2 * a.gqa + lane] = w;
+            for (int r = r0 + 32 + lane; r <= r1; r += 32) {
+                const float2 more = a.part_ml[part_of(r, r0, h)];
+                const float x = exp2_fast(more.x - top);
+                sum = fmaf(x, more.y, sum);
+                if (row_block < 0) s_fin[2 * a.gqa + r - r0] = x;
             }
             sum = warp_sum(sum);
         }
@@ -632,29 +752,45 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
         }
     }
     __syncthreads();
-    if (blockIdx.x < a.gqa) {
+    if (row_block < 0) {  // a warp takes every eighth part, a lane NG dimensions
         const int h = blockIdx.x;
-        int r0, r1;
         runs_of(h / kKv4Heads, r0, r1);
-        if (r0 < r1)
-            for (int d = tid; d < a.head_size; d += kKv4FinishThreads) {
-                float y = 0.f;
-                for (int r = r0; r <= r1; ++r) {
-                    const long long part = part_of(r, r0, h);
-                    y = fmaf(exp2_fast(a.part_ml[part].x - s_fin[2 * h]), a.part_o[part * (NG * 32) + d], y);
-                }
-                store_typed(a.out, (long long)b * a.out_stride + (long long)(kvh * a.gqa + h) * a.head_size + d, a.dtype, y * s_fin[2 * h + 1]);
-            }
-    }
-    if (a.sums_out) {
-        const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
-        const int end = (int)min((long long)len, (long long)(blockIdx.x + 1) * kKv4FinishRows);
-        for (int p = blockIdx.x * kKv4FinishRows + tid; p < end; p += kKv4FinishThreads) {
-            const float* x = a.scores + (row0 + p) * a.gqa;
-            float sum = 0.f;
-            for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - s_fin[2 * h]), s_fin[2 * h + 1], sum);
-            a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
+        float y[NG] = {};
+#pragma unroll 4
+        for (int r = r0 + warp; r <= r1; r += kKv4FinishThreads / 32) {
+            const float w = s_fin[2 * a.gqa + r - r0];
+            const float* po = a.part_o + part_of(r, r0, h) * (NG * 32) + lane;
+#pragma unroll
+            for (int k = 0; k < NG; ++k) y[k] = fmaf(w, po[k * 32], y[k]);
         }
+#pragma unroll
+        for (int k = 0; k < NG; ++k) s_part[warp][k * 32 + lane] = y[k];
+        __syncthreads();
+        for (int d = tid; d < a.head_size; d += kKv4FinishThreads) {
+            float x = 0.f;
+#pragma unroll
+            for (int w = 0; w < kKv4FinishThreads / 32; ++w) x += s_part[w][d];
+            store_typed(a.out, (long long)b * a.out_stride + (long long)(kvh * a.gqa + h) * a.head_size + d, a.dtype, x * s_fin[2 * h + 1]);
+        }
+        return;
+    }
+    const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
+    const int end = (int)min((long long)len, (long long)(row_block + 1) * kKv4FinishRows);
+    for (int p = row_block * kKv4FinishRows + tid; p < end; p += kKv4FinishThreads) {
+        const float* x = a.scores + (row0 + p) * a.gqa;
+        float sum = 0.f;
+        if (a.gqa % 4 == 0) {
+            for (int h = 0; h < a.gqa; h += 4) {
+                const float4 v = *reinterpret_cast<const float4*>(x + h);
+                sum = fmaf(exp2_fast(v.x - s_fin[2 * h]), s_fin[2 * h + 1], sum);
+                sum = fmaf(exp2_fast(v.y - s_fin[2 * h + 2]), s_fin[2 * h + 3], sum);
+                sum = fmaf(exp2_fast(v.z - s_fin[2 * h + 4]), s_fin[2 * h + 5], sum);
+                sum = fmaf(exp2_fast(v.w - s_fin[2 * h + 6]), s_fin[2 * h + 7], sum);
+            }
+        } else {
+            for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - s_fin[2 * h]), s_fin[2 * h + 1], sum);
+        }
+        a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
     }
 }
 

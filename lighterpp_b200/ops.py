@@ -6,6 +6,7 @@ queued on torch's current stream; nothing here synchronises.  There is no CPU pa
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -131,62 +132,90 @@ def cuda_sample(d_logits, vocab_size, temperature, penalty, d_history, history_l
 
 # ---- operators beyond the reference's: sizes come from the tensors, work is queued on the current stream of their device.  One
 # sequence's (or token's) heads lie behind one another; from one to the next there may be a gap (a view of a wider tensor).
+#
+# A small call takes the GPU less time than the host, so the checks here look at every tensor once.  (With a device guard around every
+# call, sizes asked of the library each time and shapes compared as tuples a call took 22 - 26 us of host time.)
 
 _DTYPES = {torch.float32: LPP_F32, torch.float16: LPP_F16, torch.bfloat16: LPP_BF16}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _same_device(*tensors):
-    first = tensors[0]
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device != first.device):
-            raise ValueError("expected CUDA tensors on one device")
-    return torch.cuda.device(first.device)
+def _call(what, entry, device, *args):
+    """Queues the call on the current stream of ``device``."""
+    if torch.cuda.current_device() == device:
+        st = entry(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            st = entry(*args, _raw_stream(device))
+    if st:
+        _check(st, what)
 
 
-def _want(what, t, dtype, shape):
-    if t.dtype != dtype or tuple(t.shape) != tuple(shape) or not t.is_contiguous():
-        raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+def _device(what, first, *others):
+    device = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != device:
+            raise ValueError(f"{what}: expected CUDA tensors on one device")
+    if device < 0:
+        raise ValueError(f"{what}: expected CUDA tensors on one device")
+    return device
 
 
-def _heads(what, t, dtype=None, shape=None):
+def _want(what, t, dtype, *shape):
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what}: expected a contiguous {dtype} tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
+
+
+def _heads(what, t, dtype, shape):
     """Elements from one token of ``t`` [tokens, heads, head_size] to the next."""
-    if t.dim() != 3 or t.dtype not in _DTYPES or (dtype is not None and t.dtype != dtype) or (shape is not None and tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{what}: got {t.dtype} {tuple(t.shape)}" + (f", expected {dtype} {tuple(shape)}" if shape is not None else ""))
-    if t.numel() and ((t.shape[2] > 1 and t.stride(2) != 1) or (t.shape[1] > 1 and t.stride(1) != t.shape[2])):
+    if t.dtype is not dtype or t.shape != shape or len(shape) != 3:
+        raise ValueError(f"{what}: got {t.dtype} {tuple(t.shape)}, expected {dtype} [tokens, heads, head_size]" + (f" = {tuple(shape)}" if t.shape != shape else ""))
+    tokens, heads, size = shape
+    if t.is_contiguous():
+        return heads * size
+    if (size > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != size):
         raise ValueError(f"{what}: the heads of a token lie behind one another")
-    dense = t.shape[1] * t.shape[2]
-    return t.stride(0) if t.shape[0] > 1 else dense
+    return t.stride(0) if tokens > 1 else heads * size
 
 
-def _raw(t):
-    return C.c_void_p(t.data_ptr() if t is not None else None)
+def _type(what, t):
+    dtype = _DTYPES.get(t.dtype)
+    if dtype is None:
+        raise ValueError(f"{what}: {t.dtype} is none of F32, F16 and BF16")
+    return dtype
+
+
+def _ptr(t):
+    return t.data_ptr() if t is not None else None
 
 
 def _cache(what, k, v, head_size):
     """(batch, kv heads, capacity) of a 4-bit cache."""
+    shape = k.shape
     row = kv4_row_bytes(head_size)
-    if k.dim() != 4:
-        raise ValueError(f"{what}: a 4-bit cache is [batch, kv heads, capacity, {row}] bytes")
-    _want(what, k, torch.uint8, tuple(k.shape[:3]) + (row,))
-    _want(what, v, torch.uint8, k.shape)
-    return k.shape[:3]
+    if len(shape) != 4 or shape[3] != row or v.shape != shape or k.dtype is not torch.uint8 or v.dtype is not torch.uint8 or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError(f"{what}: a 4-bit cache is two contiguous [batch, kv heads, capacity, {row}] tensors of bytes, got {tuple(shape)} and {tuple(v.shape)}")
+    return shape[:3]
 
 
 def cuda_prompt_attention(d_out, d_q, d_k, d_v, d_offsets, scale):
     """Causal attention of packed prompts: ``d_q``, ``d_out`` [tokens, heads, head_size], ``d_k``, ``d_v`` [tokens, kv heads, head_size] (F16
     or BF16); ``d_offsets`` (int32, prompts + 1) has the first token of each prompt and the end of the last.  Tokens behind are left as they were."""
-    with _same_device(d_q, d_out, d_k, d_v, d_offsets):
-        qs = _heads("cuda_prompt_attention", d_q)
-        outs = _heads("cuda_prompt_attention", d_out, d_q.dtype, d_q.shape)
-        ks = _heads("cuda_prompt_attention", d_k, d_q.dtype)
-        vs = _heads("cuda_prompt_attention", d_v, d_q.dtype, d_k.shape)
-        if d_k.shape[0] != d_q.shape[0] or d_k.shape[2] != d_q.shape[2] or d_offsets.dim() != 1 or d_offsets.shape[0] < 1:
-            raise ValueError("cuda_prompt_attention: as many keys as queries, of one head size, and offsets of prompts + 1")
-        _want("cuda_prompt_attention", d_offsets, torch.int32, d_offsets.shape)
-        _check(_lib().lpp_op_prompt_attention(_raw(d_out), _raw(d_q), _raw(d_k), _raw(d_v), _raw(d_offsets), d_offsets.shape[0] - 1, d_q.shape[0], d_q.shape[1], d_k.shape[1],
-                                              d_q.shape[2], outs, qs, ks, vs, float(scale), _DTYPES[d_q.dtype], _s()), "cuda_prompt_attention")
+    what = "cuda_prompt_attention"
+    device = _device(what, d_q, d_out, d_k, d_v, d_offsets)
+    dtype, shape, kv_shape = d_q.dtype, d_q.shape, d_k.shape
+    qs, outs = _heads(what, d_q, dtype, shape), _heads(what, d_out, dtype, shape)
+    ks, vs = _heads(what, d_k, dtype, kv_shape), _heads(what, d_v, dtype, kv_shape)
+    n, heads, size = shape
+    if kv_shape[0] != n or kv_shape[2] != size or d_offsets.dim() != 1 or d_offsets.shape[0] < 1:
+        raise ValueError(f"{what}: as many keys as queries, of one head size, and offsets of prompts + 1")
+    prompts = d_offsets.shape[0] - 1
+    _want(what, d_offsets, torch.int32, prompts + 1)
+    _call(what, _lib().lpp_op_prompt_attention, device, d_out.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_offsets.data_ptr(), prompts, n, heads, kv_shape[1],
+          size, outs, qs, ks, vs, float(scale), _type(what, d_q))
 
 
+@functools.lru_cache(maxsize=None)
 def kv4_row_bytes(head_size):
     """Bytes of a row of the 4-bit cache: ``torch.zeros(batch, kv_heads, capacity, kv4_row_bytes(head_size), dtype=torch.uint8)`` is one."""
     n = _lib().lpp_op_kv4_row_bytes(int(head_size))
@@ -195,71 +224,82 @@ def kv4_row_bytes(head_size):
     return n
 
 
+def _kv4_rows(what, entry, first, second, k, v, caches, slots):
+    device = _device(what, k, v, slots, *caches)
+    shape = k.shape
+    ks, vs = _heads(what, k, k.dtype, shape), _heads(what, v, k.dtype, shape)
+    n, heads, size = shape
+    batch, kv, capacity = _cache(what, *caches, size)
+    _want(what, slots, torch.int64, n)
+    if heads != kv:
+        raise ValueError(f"{what}: the cache has another number of heads")
+    _call(what, entry, device, first[0].data_ptr(), first[1].data_ptr(), second[0].data_ptr(), second[1].data_ptr(), slots.data_ptr(), n, batch, kv, capacity, size, ks, vs,
+          _type(what, k))
+
+
 def cuda_kv4_write(d_k_cache, d_v_cache, d_k, d_v, d_slots):
     """Rows ``d_k``, ``d_v`` [tokens, kv heads, head_size] into the 4-bit cache at ``d_slots`` (int64; sequence * capacity + position,
     all different; a token whose slot is negative, or beyond the cache, is left out)."""
-    with _same_device(d_k_cache, d_v_cache, d_k, d_v, d_slots):
-        ks = _heads("cuda_kv4_write", d_k)
-        vs = _heads("cuda_kv4_write", d_v, d_k.dtype, d_k.shape)
-        b, kv, cap = _cache("cuda_kv4_write", d_k_cache, d_v_cache, d_k.shape[2])
-        _want("cuda_kv4_write", d_slots, torch.int64, d_k.shape[:1])
-        if d_k.shape[1] != kv:
-            raise ValueError("cuda_kv4_write: the cache has another number of heads")
-        _check(_lib().lpp_op_kv4_write(_raw(d_k_cache), _raw(d_v_cache), _raw(d_k), _raw(d_v), _raw(d_slots), d_k.shape[0], b, kv, cap, d_k.shape[2], ks, vs,
-                                       _DTYPES[d_k.dtype], _s()), "cuda_kv4_write")
+    caches, rows = (d_k_cache, d_v_cache), (d_k, d_v)
+    _kv4_rows("cuda_kv4_write", _lib().lpp_op_kv4_write, caches, rows, d_k, d_v, caches, d_slots)
 
 
 def cuda_kv4_read(d_k, d_v, d_k_cache, d_v_cache, d_slots):
     """The values that the cache holds at ``d_slots``; a token whose slot is negative, or beyond the cache, is left as it was."""
-    with _same_device(d_k_cache, d_v_cache, d_k, d_v, d_slots):
-        ks = _heads("cuda_kv4_read", d_k)
-        vs = _heads("cuda_kv4_read", d_v, d_k.dtype, d_k.shape)
-        b, kv, cap = _cache("cuda_kv4_read", d_k_cache, d_v_cache, d_k.shape[2])
-        _want("cuda_kv4_read", d_slots, torch.int64, d_k.shape[:1])
-        if d_k.shape[1] != kv:
-            raise ValueError("cuda_kv4_read: the cache has another number of heads")
-        _check(_lib().lpp_op_kv4_read(_raw(d_k), _raw(d_v), _raw(d_k_cache), _raw(d_v_cache), _raw(d_slots), d_k.shape[0], b, kv, cap, d_k.shape[2], ks, vs,
-                                      _DTYPES[d_k.dtype], _s()), "cuda_kv4_read")
+    caches, rows = (d_k_cache, d_v_cache), (d_k, d_v)
+    _kv4_rows("cuda_kv4_read", _lib().lpp_op_kv4_read, rows, caches, d_k, d_v, caches, d_slots)
+
+
+@functools.lru_cache(maxsize=None)
+def _kv4_scratch_bytes(device, *sizes):
+    with torch.cuda.device(device):
+        return _lib().lpp_op_kv4_attention_scratch_bytes(*sizes)
 
 
 def cuda_kv4_attention(d_out, d_q, d_k_cache, d_v_cache, d_lens, scale, d_sums_in=None, d_sums_out=None):
     """Attention of one token per sequence, ``d_q`` [batch, heads, head_size], over the first ``d_lens`` (int32) positions of the 4-bit
     cache.  ``d_sums_out`` [batch, kv heads, capacity] (FP32) = ``d_sums_in`` (None: zeros) + the softmax summed over a key/value head's queries."""
-    with _same_device(d_q, d_out, d_k_cache, d_v_cache, d_lens, d_sums_in, d_sums_out):
-        qs = _heads("cuda_kv4_attention", d_q)
-        outs = _heads("cuda_kv4_attention", d_out, d_q.dtype, d_q.shape)
-        n, heads, size = d_q.shape
-        b, kv, cap = _cache("cuda_kv4_attention", d_k_cache, d_v_cache, size)
-        _want("cuda_kv4_attention", d_lens, torch.int32, (n,))
-        if b != n:
-            raise ValueError("cuda_kv4_attention: one query token per sequence of the cache")
-        for t in (d_sums_in, d_sums_out):
-            if t is not None:
-                _want("cuda_kv4_attention", t, torch.float32, (b, kv, cap))
-        lib = _lib()
-        bytes_ = lib.lpp_op_kv4_attention_scratch_bytes(b, heads, kv, cap, size, d_sums_out is not None)
-        # torch's allocator hands blocks on in stream order, so the scratch may be let go as soon as the work is queued
-        scratch = torch.empty(max(bytes_, 1), dtype=torch.uint8, device=d_q.device)
-        _check(lib.lpp_op_kv4_attention(_raw(scratch), bytes_, _raw(d_out), _raw(d_q), _raw(d_k_cache), _raw(d_v_cache), _raw(d_lens), _raw(d_sums_in), _raw(d_sums_out),
-                                        float(scale), b, heads, kv, cap, size, outs, qs, _DTYPES[d_q.dtype], _s()), "cuda_kv4_attention")
+    what = "cuda_kv4_attention"
+    device = _device(what, d_q, d_out, d_k_cache, d_v_cache, d_lens, d_sums_in, d_sums_out)
+    dtype, shape = d_q.dtype, d_q.shape
+    qs, outs = _heads(what, d_q, dtype, shape), _heads(what, d_out, dtype, shape)
+    n, heads, size = shape
+    batch, kv, capacity = _cache(what, d_k_cache, d_v_cache, size)
+    _want(what, d_lens, torch.int32, n)
+    if batch != n:
+        raise ValueError(f"{what}: one query token per sequence of the cache")
+    if d_sums_in is not None:
+        _want(what, d_sums_in, torch.float32, batch, kv, capacity)
+    if d_sums_out is not None:
+        _want(what, d_sums_out, torch.float32, batch, kv, capacity)
+    room = _kv4_scratch_bytes(device, batch, heads, kv, capacity, size, d_sums_out is not None)
+    # torch's allocator hands blocks on in stream order, so the scratch may be let go as soon as the work is queued
+    scratch = torch.empty(max(room, 1), dtype=torch.uint8, device=d_q.device)
+    _call(what, _lib().lpp_op_kv4_attention, device, scratch.data_ptr(), room, d_out.data_ptr(), d_q.data_ptr(), d_k_cache.data_ptr(), d_v_cache.data_ptr(), d_lens.data_ptr(),
+          _ptr(d_sums_in), _ptr(d_sums_out), float(scale), batch, heads, kv, capacity, size, outs, qs, _type(what, d_q))
+
+
+_KV4_SIZES = {}  # row bytes -> a head size that has them
 
 
 def cuda_kv4_evict(d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_k_cache, d_v_cache, d_sums, d_lens, keep, recent):
     """Moves ``keep`` rows of every head into a shorter cache: the ``recent`` last ones and those with the largest ``d_sums``.  ``d_kept``
     [batch, kv heads, keep] (int32) gets their old positions, ``d_lens_out`` (int32) the new lengths."""
-    with _same_device(d_k_cache, d_v_cache, d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_sums, d_lens):
-        lib = _lib()
-        if d_k_cache.dim() != 4 or d_k_out.dim() != 4:
-            raise ValueError("cuda_kv4_evict: a 4-bit cache is [batch, kv heads, capacity, row] bytes")
-        b, kv, cap, row = d_k_cache.shape
-        size = next((s for s in (32, 64, 96, 128, 256) if lib.lpp_op_kv4_row_bytes(s) == row), 0)  # (rows are moved whole)
-        cap_out = d_k_out.shape[2]
-        for t, shape in ((d_k_cache, (b, kv, cap, row)), (d_v_cache, (b, kv, cap, row)), (d_k_out, (b, kv, cap_out, row)), (d_v_out, (b, kv, cap_out, row))):
-            _want("cuda_kv4_evict", t, torch.uint8, shape)
-        _want("cuda_kv4_evict", d_sums, torch.float32, (b, kv, cap))
-        _want("cuda_kv4_evict", d_sums_out, torch.float32, (b, kv, cap_out))
-        _want("cuda_kv4_evict", d_kept, torch.int32, (b, kv, int(keep)))
-        _want("cuda_kv4_evict", d_lens, torch.int32, (b,))
-        _want("cuda_kv4_evict", d_lens_out, torch.int32, (b,))
-        _check(lib.lpp_op_kv4_evict(_raw(d_k_out), _raw(d_v_out), _raw(d_sums_out), _raw(d_kept), _raw(d_lens_out), _raw(d_k_cache), _raw(d_v_cache), _raw(d_sums),
-                                    _raw(d_lens), b, kv, cap, cap_out, size, int(keep), int(recent), _s()), "cuda_kv4_evict")
+    what, keep, recent = "cuda_kv4_evict", int(keep), int(recent)
+    device = _device(what, d_k_cache, d_v_cache, d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_sums, d_lens)
+    if not _KV4_SIZES:
+        _KV4_SIZES.update((kv4_row_bytes(s), s) for s in (32, 64, 96, 128, 256))
+    size = _KV4_SIZES.get(d_k_cache.shape[-1], 0)  # (rows are moved whole)
+    if not size:
+        raise ValueError(f"{what}: no head has rows of {d_k_cache.shape[-1]} bytes")
+    batch, kv, capacity = _cache(what, d_k_cache, d_v_cache, size)
+    batch_out, kv_out, capacity_out = _cache(what, d_k_out, d_v_out, size)
+    if batch_out != batch or kv_out != kv:
+        raise ValueError(f"{what}: the new cache has other sequences or heads")
+    _want(what, d_sums, torch.float32, batch, kv, capacity)
+    _want(what, d_sums_out, torch.float32, batch, kv, capacity_out)
+    _want(what, d_kept, torch.int32, batch, kv, keep)
+    _want(what, d_lens, torch.int32, batch)
+    _want(what, d_lens_out, torch.int32, batch)
+    _call(what, _lib().lpp_op_kv4_evict, device, d_k_out.data_ptr(), d_v_out.data_ptr(), d_sums_out.data_ptr(), d_kept.data_ptr(), d_lens_out.data_ptr(), d_k_cache.data_ptr(),
+          d_v_cache.data_ptr(), d_sums.data_ptr(), d_lens.data_ptr(), batch, kv, capacity, capacity_out, size, keep, recent)

@@ -231,7 +231,7 @@ def test_captured_replayed_and_on_another_stream(T, scratch_fill):
     scratch = T.full((n,), scratch_fill, dtype=T.uint8, device="cuda")
 
     def call():
-        st = lib.lpp_op_kv4_attention(ops._raw(scratch), n, ops._raw(out), ops._raw(q), ops._raw(kc), ops._raw(vc), ops._raw(dl), None, ops._raw(sums), 0.125, 2, 8, 2, 640, 64,
+        st = lib.lpp_op_kv4_attention(ops._ptr(scratch), n, ops._ptr(out), ops._ptr(q), ops._ptr(kc), ops._ptr(vc), ops._ptr(dl), None, ops._ptr(sums), 0.125, 2, 8, 2, 640, 64,
                                       512, 512, 1, ops._s())
         assert st == 0
 
@@ -263,7 +263,7 @@ def test_scratch_that_is_too_small_is_refused(T):
     n = lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 640, 64, 0)
     assert 0 < n < lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 640, 64, 1)
     x = T.zeros(1 << 20, dtype=T.uint8, device="cuda")
-    p = ops._raw(x)
+    p = ops._ptr(x)
     assert lib.lpp_op_kv4_attention(p, n - 1, p, p, p, p, p, None, None, 0.1, 1, 8, 2, 640, 64, 512, 512, 1, ops._s()) == 1
     assert lib.lpp_op_kv4_attention(p, n, p, p, p, p, p, None, p, 0.1, 1, 8, 2, 640, 64, 512, 512, 1, ops._s()) == 1  # sums want more
 
