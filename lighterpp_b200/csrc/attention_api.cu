@@ -257,7 +257,10 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.rate = scale * 1.4426950408889634f;
     return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
                         constexpr int NG = ng.value;
-                        constexpr int smem = kv4_attn_smem<NG>();
+                        // as many units in flight as the shared memory holds beside the warps' sums
+                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = (227 * 1024) / kKv4Ctas<NG> - 2048 - sums;
+                        a.stages = std::min(kKv4MaxStages, room / kKv4StageBytes<NG>);
+                        const int smem = a.stages * kKv4StageBytes<NG> + sums;
                         auto kernel = dtype == LPP_F32 ? kv4_attn_kernel<NG, true> : kv4_attn_kernel<NG, false>;
                         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
                             (void)cudaGetLastError();

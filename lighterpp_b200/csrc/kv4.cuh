@@ -165,9 +165,8 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(Kv4Cach
 // key/value head as the 8-column one.  The codes themselves are the operand: as FP16 bit patterns, 0 .. 15 are the subnormals
 // n 2^-24, and the same bits four places up are 16 n 2^-24, so a mask makes two elements of an operand register (the query elements of
 // the second kind are divided by 16).  Sums are kept apart by group and multiplied with the group's scale in FP32:
-//     q . k = sum_g scale_g (sum_d q_d n_d - 8 Q_g) + zero_g Q_g,  Q_g = sum_d q_d;
-// -8 Q_g is where the accumulator starts, and the zeros' part is one more product, of the (scale, zero) pairs as they lie in the row with
-// (0, Q_g), Q_g as two FP16 operands.  For the values the scale goes to the probability before that is rounded to FP16, the codes
+//     q . k = sum_g scale_g sum_d q_d n_d + (zero_g - 8 scale_g) Q_g,  Q_g = sum_d q_d;
+// the second part is one more product, of the (scale, zero) pairs as they lie in the row with (-8 Q_g, Q_g), Q_g as two FP16 operands.  For the values the scale goes to the probability before that is rounded to FP16, the codes
 // become n - 8 (rounding errors then are those of values around their middle), and sum_j p_j zero_jg is added in FP32.
 //
 // Reference of the exponentials: not the running maximum of the scores but a bound on the largest p * scale, which has to stay in the
@@ -180,8 +179,7 @@ constexpr int kKv4Tile = 16;     // positions of a warp's tile
 constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
 constexpr int kKv4Heads = 8;     // query heads of a CTA
 constexpr float kKv4Limit = 32768.f;  // of p * scale
-template <int NG>
-constexpr int kKv4Stages = NG > 3 ? 3 : 4;  // tiles in flight per warp
+constexpr int kKv4MaxStages = 8;  // units in flight per CTA
 template <int NG>
 constexpr int kKv4Ctas = NG > 4 ? 1 : 2;    // of an SM
 
@@ -197,7 +195,7 @@ struct Kv4AttnArgs {
     float2* part_ml;        // [runs][2][8]: the same of parts of a head: [0] one that began in an earlier run, [1] one that begins here
     float* part_o;          // [runs][2][8][NG * 32]
     long long capacity, q_stride, out_stride;
-    int batch, heads, kv_heads, gqa, head_size, head_tiles, runs;
+    int batch, heads, kv_heads, gqa, head_size, head_tiles, runs, stages;
     int dtype;
     float rate;             // scale * log2(e)
 };
@@ -241,12 +239,12 @@ __device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, long lo
 }
 
 template <int NG>
-constexpr int kKv4RingBytes = kKv4Warps * kKv4Stages<NG> * 2 * kKv4Tile * kv4_row_bytes(NG);
+constexpr int kKv4StageBytes = 2 * kKv4Unit * kv4_row_bytes(NG);  // keys, then values
 template <int NG>
 constexpr int kKv4Pitch = NG * 32 + 4;
 template <int NG>
-constexpr int kv4_attn_smem() {  // rings, barriers, sums of the warps
-    return kKv4RingBytes<NG> + kKv4Warps * kKv4Stages<NG> * 8 + kKv4Warps * kKv4Heads * kKv4Pitch<NG> * 4;
+constexpr int kv4_sums_bytes(int heads) {  // of the warps, for up to eight heads
+    return kKv4Warps * heads * kKv4Pitch<NG> * 4;
 }
 
 __device__ __forceinline__ float load_typed(const void* p, long long i, int dtype) {
@@ -332,27 +330,36 @@ __device__ __forceinline__ void kv4_codes(uint32_t tile, int lane, uint32_t (&w)
                 w[i][h] = VALUES ? lds16(a + i * 16 + h * 8 * kRow) | lds16(a + i * 16 + (h * 8 + 1) * kRow) << 16 : lds32(a + i * 16 + h * 8 * kRow);
     }
 }
-// (n - 8) of the codes in bits 0-3 and 16-19, and in bits 4-7 and 20-23: 1024 + n - 1032, (1024 + 16 n) / 16 - 72, both exact
-__device__ __forceinline__ uint32_t kv4_low(uint32_t x) {
-    const uint32_t b = (x & 0x000f000fu) | 0x64006400u, off = 0x64086408u;
+// (n - 8) of the codes in bits 0-3 and 16-19, and in bits 4-7 and 20-23: 1024 + n - 1032, (1024 + 16 n) / 16 - 72, both exact.  The
+// constants travel in registers of unknown content: as immediates mask and exponent would be two instructions.
+struct Kv4Magic {
+    uint32_t exponent = 0x64006400u, f = 0x2c002c00u /* 1/16 */, off = 0xd480d480u /* -72 */;
+    __device__ __forceinline__ void hide() { asm volatile("" : "+r"(exponent), "+r"(f), "+r"(off)); }
+};
+__device__ __forceinline__ uint32_t kv4_low(uint32_t x, const Kv4Magic& c) {
+    uint32_t b;
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(b) : "r"(x), "r"(c.exponent));  // (x & mask) | exponent
+    const uint32_t off = 0x64086408u;
     const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&off));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t kv4_high(uint32_t x) {
-    const uint32_t b = (x & 0x00f000f0u) | 0x64006400u, f = 0x2c002c00u /* 1/16 */, off = 0xd480d480u /* -72 */;
-    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&f), *reinterpret_cast<const __half2*>(&off));
+__device__ __forceinline__ uint32_t kv4_high(uint32_t x, const Kv4Magic& c) {
+    uint32_t b;
+    asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xea;" : "=r"(b) : "r"(x), "r"(c.exponent));
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c.f), *reinterpret_cast<const __half2*>(&c.off));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 template <int NG, bool SPLIT>
 static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_kernel(const Kv4AttnArgs a) {
-    constexpr int kRow = kv4_row_bytes(NG), kTileBytes = kKv4Tile * kRow, kParts = SPLIT ? 2 : 1, kStages = kKv4Stages<NG>, kPitch = kKv4Pitch<NG>;
+    constexpr int kRow = kv4_row_bytes(NG), kStage = kKv4StageBytes<NG>, kParts = SPLIT ? 2 : 1, kPitch = kKv4Pitch<NG>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kKv4Warps][kKv4Heads], s_l[kKv4Warps][kKv4Heads];
+    __shared__ uint64_t full[kKv4MaxStages], empty[kKv4MaxStages];
     __shared__ int s_fail;
     pdl_wait();
     pdl_launch_dependents();  // (after the wait: what the finishing kernel reads of the lengths is there when it starts)
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int heads8 = a.kv_heads * a.head_tiles;
     const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);  // (no run is empty)
     if (blockIdx.x >= runs) return;
@@ -372,38 +379,38 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     };
     const Place p_begin = place(all * blockIdx.x / runs), p_end = place(all * (blockIdx.x + 1) / runs);
     if (p_begin.b == p_end.b && p_begin.head == p_end.head && p_begin.unit == p_end.unit) return;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kKv4RingBytes<NG>) + warp * kStages;
-    float* so = reinterpret_cast<float*>(smem + kKv4RingBytes<NG> + kKv4Warps * kStages * 8);
-    unsigned char* ring = smem + warp * kStages * 2 * kTileBytes;
-    if (tid == 0) s_fail = 0;
-    if (lane == 0) {
-        for (int i = 0; i < kStages; ++i) mbar_init(&bars[i], 1);
+    float* so = reinterpret_cast<float*>(smem + a.stages * kStage);
+    if (tid == 0) {
+        s_fail = 0;
+        for (int i = 0; i < a.stages; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], kKv4Warps);
+        }
         mbar_fence_init();
     }
     __syncthreads();
     int b = p_begin.b, len = p_begin.len, units = kv4_units(len), head = p_begin.head, unit = p_begin.unit;
 
-    // lane 0: requests this warp's next tile, if there is one
-    int ahead_b = b, ahead_len = len, ahead_end = units * kKv4Unit, ahead_head = head, ahead_at = unit * kKv4Unit + warp * kKv4Tile, put = 0;
+    // first thread: requests the next unit that has positions
+    int ahead_b = b, ahead_len = len, ahead_end = units * kKv4Unit, ahead_head = head, ahead_at = unit * kKv4Unit, put = 0;
     auto head_row = [&](int seq, int h8) { return ((long long)seq * a.kv_heads + h8 / a.head_tiles) * a.capacity; };
     long long ahead_row = head_row(b, head);
     auto request = [&]() {
         for (;;) {
             const int at = ahead_at;
-            const bool last = ahead_b == p_end.b && ahead_head == p_end.head;
-            if (ahead_b > p_end.b || (last && at >= p_end.unit * kKv4Unit)) return;
+            if (ahead_b > p_end.b || (ahead_b == p_end.b && (ahead_head > p_end.head || (ahead_head == p_end.head && at >= p_end.unit * kKv4Unit)))) return;
             const bool there = at < ahead_len;
             if (there) {
                 const long long from = (ahead_row + at) * kRow;
-                const uint32_t bytes = (uint32_t)min((long long)kKv4Tile, a.capacity - at) * kRow;  // (a multiple of four rows)
-                unsigned char* to = ring + put * 2 * kTileBytes;
-                mbar_arrive_expect_tx(&bars[put], 2 * bytes);
-                bulk_g2s(to, a.k + from, bytes, &bars[put]);
-                bulk_g2s(to + kTileBytes, a.v + from, bytes, &bars[put]);
-                if (++put == kStages) put = 0;
+                const uint32_t bytes = (uint32_t)(min(kKv4Unit, (ahead_len - at + 3) & ~3) * kRow);  // (the capacity is a multiple of four rows)
+                unsigned char* to = smem + put * kStage;
+                mbar_arrive_expect_tx(&full[put], 2 * bytes);
+                bulk_g2s(to, a.k + from, bytes, &full[put]);
+                bulk_g2s(to + kStage / 2, a.v + from, bytes, &full[put]);
+                if (++put == a.stages) put = 0;
             }
             if ((ahead_at += kKv4Unit) >= ahead_end) {  // the next head
-                ahead_at = warp * kKv4Tile;
+                ahead_at = 0;
                 if (++ahead_head == heads8) {
                     ahead_head = 0;
                     if (++ahead_b < a.batch) ahead_len = kv4_len(a, ahead_b);
@@ -411,25 +418,27 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 }
                 ahead_row = head_row(ahead_b, ahead_head);
             }
-            if (there) break;
+            if (there) return;
         }
     };
-    if (lane == 0)
-        for (int i = 0; i < kStages; ++i) request();
+    if (tid == 0)
+        for (int i = 0; i < a.stages; ++i) request();
+    Kv4Magic magic;
+    magic.hide();
     bool ok = true;
-    int stage = 0;
-    uint32_t phase = 0;
+    int stage = 0, stage_before = -1;
+    uint32_t phase = 0, phase_before = 0;
 
     while (b < p_end.b || (b == p_end.b && (head < p_end.head || (head == p_end.head && unit < p_end.unit)))) {
     const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
     const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
     const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
     const int mine = (b == p_end.b && head == p_end.head ? p_end.unit : units) - unit, p1 = len;
-    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^9 .. 2^10 (their sums
-    // over a group stay in the FP16 range)
+    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^6 .. 2^7 (eight times
+    // their sums over a group stay in the FP16 range)
     uint32_t qf[kParts][NG][4];
-    float start[NG][2], rate[2];  // where a group's accumulator starts, and factor of the scores, heads 2 t and 2 t + 1
-    uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of the zeros, head g: (0, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
+    float rate[2];  // factor of the scores, heads 2 t and 2 t + 1
+    uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of (scale, zero), head g: (-8 Q, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
     {
         float x[NG][8], top = 0.f;
         const bool some = g < n_heads;
@@ -444,7 +453,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // exponents of 2 in two halves, either within the normal range
-        const int e = top > 0.f && top < INFINITY ? 9 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
+        const int e = top > 0.f && top < INFINITY ? 6 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
         const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
         float sums[NG];
 #pragma unroll
@@ -475,8 +484,6 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         for (int j = 0; j < 2; ++j) {
             const int from = (2 * t + j) * 4;
             rate[j] = __shfl_sync(0xffffffffu, back, from);
-#pragma unroll
-            for (int i = 0; i < NG; ++i) start[i][j] = -8.f * 0x1p-24f * __shfl_sync(0xffffffffu, sums[i], from);
         }
         float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
@@ -485,8 +492,9 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
 #pragma unroll
         for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
             const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
-            zf[0][i] = (uint32_t)__half_as_ushort(hi) << 16;
-            zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = (uint32_t)__half_as_ushort(lo) << 16;
+            const __half2 both = __halves2half2(__hmul(hi, __float2half_rn(-8.f)), hi), rest = __halves2half2(__hmul(lo, __float2half_rn(-8.f)), lo);
+            zf[0][i] = *reinterpret_cast<const uint32_t*>(&both);
+            zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = *reinterpret_cast<const uint32_t*>(&rest);
         }
     }
 
@@ -499,14 +507,10 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     for (int i = 0; i < NG; ++i) z[i][0] = z[i][1] = 0.f;
 
     float* scores = a.scores ? a.scores + (row0 + unit * kKv4Unit + warp * kKv4Tile + g) * a.gqa + tile8 * kKv4Heads + 2 * t : nullptr;
-    for (int i = 0, at = unit * kKv4Unit + warp * kKv4Tile; i < mine && at < p1; ++i, at += kKv4Unit) {
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&bars[stage], phase, nullptr));
-        if (!ok) {  // a copy that never came: the results of this run say so
-            m[0] = m[1] = NAN;
-            s_fail = 1;
-            break;
-        }
-        const uint32_t sk = smem_u32(ring + stage * 2 * kTileBytes), sv = sk + kTileBytes;
+    auto tile = [&](auto whole, int at) {  // whole: every row lies below the length
+        constexpr bool kWhole = decltype(whole)::value;
+        const bool in0 = kWhole || at + g < p1, in1 = kWhole || at + g + 8 < p1;
+        const uint32_t sk = smem_u32(smem + stage * kStage) + warp * kKv4Tile * kRow, sv = sk + kStage / 2;
         // ---- scores of rows g and g + 8
         float s[4];
         {
@@ -515,7 +519,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
             kv4_params<NG>(r0, p0);
             kv4_params<NG>(r1, p1w);
-            // zeros first: rows of (scale, zero) pairs as they lie there times (0, Q)
+            // rows of (scale, zero) pairs as they lie there times (-8 Q, Q)
             float acc[4];
             if constexpr (NG > 4) {
                 const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
@@ -530,7 +534,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 const uint32_t w0 = w[gr][0], w1 = w[gr][1], v0 = w0 >> 8, v1 = w1 >> 8;
-                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], start[gr][0], start[gr][1], start[gr][0], start[gr][1]);
+                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], 0.f, 0.f, 0.f, 0.f);
                 kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[0][gr][2], qf[0][gr][3], acc[0], acc[1], acc[2], acc[3]);
                 if constexpr (SPLIT) {
                     kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[0], acc[1], acc[2], acc[3]);
@@ -543,13 +547,22 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 s[3] = fmaf(s1, acc[3], s[3]);
             }
         }
-        const bool in0 = at + g < p1, in1 = at + g + 8 < p1;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = (j < 2 ? in0 : in1) ? s[j] * rate[j & 1] : -INFINITY;
-        if (a.scores) {
+        for (int j = 0; j < 4; ++j) s[j] *= rate[j & 1];
+        if constexpr (!kWhole) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) scores[(j >> 1) * 8 * a.gqa + (j & 1)] = s[j];
+                if (!(j < 2 ? in0 : in1)) s[j] = -INFINITY;
+        }
+        if (a.scores) {
+            if (2 * t + 1 < n_heads && a.gqa % 2 == 0) {
+                if (in0) *reinterpret_cast<float2*>(scores) = make_float2(s[0], s[1]);
+                if (in1) *reinterpret_cast<float2*>(scores + 8 * a.gqa) = make_float2(s[2], s[3]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) scores[(j >> 1) * 8 * a.gqa + (j & 1)] = s[j];
+            }
             scores += (long long)kKv4Unit * a.gqa;
         }
         // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
@@ -558,17 +571,21 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         for (int r = 0; r < 2; ++r) {
             uint32_t w[NG];
             kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, w);
+            if (!(r ? in1 : in0)) {
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) w[gr] = 0u;
+            }
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const float2 f = half2_bits_to_float2((r ? in1 : in0) ? w[gr] : 0u);
+                const float2 f = half2_bits_to_float2(w[gr]);
                 vs[r][gr] = f.x;
                 vz[r][gr] = f.y;
                 top[r] = fmaxf(top[r], f.x);
             }
         }
-        float p[4];
+        float p[4];  // (a row beyond the end: 0, or NaN while there is no reference, which the vote takes)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? in0 : in1) ? exp2_fast(s[j] - m[j & 1]) : 0.f;
+        for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
         if (__any_sync(0xffffffffu, !(fmaxf(p[0], p[1]) * top[0] <= kKv4Limit) || !(fmaxf(p[2], p[3]) * top[1] <= kKv4Limit))) {
             // move the reference: the largest product becomes 2^8 .. 2^9
 #pragma unroll
@@ -588,7 +605,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 for (int k = 0; k < NG; ++k) z[k][j] *= f;
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? in0 : in1) ? exp2_fast(s[j] - m[j & 1]) : 0.f;
+            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
         }
         l[0] += p[0] + p[2];
         l[1] += p[1] + p[3];
@@ -604,8 +621,8 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             const uint32_t b0 = transpose8(*reinterpret_cast<const uint32_t*>(&ha)), b1 = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
             const uint32_t xa = codes[gr][0], xb = codes[gr][1];
             const uint32_t ya = xa >> 8, yb = xb >> 8;
-            const uint32_t a0 = kv4_low(xa), a1 = kv4_high(xa), a2 = kv4_low(xb), a3 = kv4_high(xb);
-            const uint32_t d0 = kv4_low(ya), d1 = kv4_high(ya), d2 = kv4_low(yb), d3 = kv4_high(yb);
+            const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
+            const uint32_t d0 = kv4_low(ya, magic), d1 = kv4_high(ya, magic), d2 = kv4_low(yb, magic), d3 = kv4_high(yb, magic);
             float(&oa)[4] = o[2 * gr];
             float(&ob)[4] = o[2 * gr + 1];
             kv4_mma(oa, a0, a1, a2, a3, b0, b1, oa[0], oa[1], oa[2], oa[3]);
@@ -618,9 +635,30 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 kv4_mma(ob, d0, d1, d2, d3, l0, l1, ob[0], ob[1], ob[2], ob[3]);
             }
         }
+    };
+    const int unit_end = min(p1, (unit + mine) * kKv4Unit);
+    for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
+        const int at = unit_at + warp * kKv4Tile;
+        if (!__all_sync(0xffffffffu, mbar_try_wait(&full[stage], phase))) ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase, nullptr));
+        if (!ok) {  // a copy that never came: the results of this run say so
+            m[0] = m[1] = NAN;
+            s_fail = 1;
+            break;
+        }
+        if (at + kKv4Tile <= p1)
+            tile(std::true_type(), at);
+        else if (at < p1)
+            tile(std::false_type(), at);
         __syncwarp();
-        if (lane == 0) request();
-        if (++stage == kStages) {
+        if (lane == 0) mbar_arrive(&empty[stage]);
+        // the unit before has been read by all warps but late ones: its place takes the next
+        if (warp == 0 && stage_before >= 0) {
+            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[stage_before], phase_before, nullptr));
+            if (lane == 0 && ok) request();
+        }
+        stage_before = stage;
+        phase_before = phase;
+        if (++stage == a.stages) {
             stage = 0;
             phase ^= 1u;
         }
@@ -645,7 +683,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j)  // tile 2 gr + k: rows g and g + 8 are dimensions 4 g + 2 k and the one after
-                so[(warp * kKv4Heads + 2 * t + (j & 1)) * kPitch + gr * 32 + 4 * g + 2 * k + (j >> 1)] = o[2 * gr + k][j] + z[gr][j & 1];
+                if (2 * t + (j & 1) < n_heads) so[(warp * n_heads + 2 * t + (j & 1)) * kPitch + gr * 32 + 4 * g + 2 * k + (j >> 1)] = o[2 * gr + k][j] + z[gr][j & 1];
     __syncthreads();
     const bool whole = unit == 0 && mine == units;  // the head lies in this run; else a part: [1] begins here, [0] began earlier
     const long long part = (long long)blockIdx.x * 2 + (unit == 0 ? 1 : 0);
@@ -658,7 +696,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         for (int w = 0; w < kKv4Warps; ++w) {
             const float f = s_m[w][h] == -INFINITY ? 0.f : exp2_fast(s_m[w][h] - top);
             sum = fmaf(f, s_l[w][h], sum);
-            y = fmaf(f, so[(w * kKv4Heads + h) * kPitch + d], y);
+            y = fmaf(f, so[(w * n_heads + h) * kPitch + d], y);
         }
         const long long bh = (long long)b * a.heads + h0 + h;
         if (!whole) {
