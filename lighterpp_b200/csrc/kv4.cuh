@@ -268,13 +268,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // d = a . b + c
 __device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
                                         float c3) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                  : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 matrix of 16-bit elements spread over a warp
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t a) {
@@ -350,12 +350,17 @@ __device__ __forceinline__ uint32_t kv4_high(uint32_t x, const Kv4Magic& c) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+struct Kv4Ahead {
+    int b, len, head, at, put;  // the next unit to be requested, and its place in the ring
+};
+
 template <int NG, bool SPLIT>
 static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int kRow = kv4_row_bytes(NG), kStage = kKv4StageBytes<NG>, kParts = SPLIT ? 2 : 1, kPitch = kKv4Pitch<NG>;
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kKv4Warps][kKv4Heads], s_l[kKv4Warps][kKv4Heads];
     __shared__ uint64_t full[kKv4MaxStages], empty[kKv4MaxStages];
+    __shared__ Kv4Ahead ahead;
     __shared__ int s_fail;
     pdl_wait();
     pdl_launch_dependents();  // (after the wait: what the finishing kernel reads of the lengths is there when it starts)
@@ -391,43 +396,43 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     __syncthreads();
     int b = p_begin.b, len = p_begin.len, units = kv4_units(len), head = p_begin.head, unit = p_begin.unit;
 
-    // first thread: requests the next unit that has positions
-    int ahead_b = b, ahead_len = len, ahead_end = units * kKv4Unit, ahead_head = head, ahead_at = unit * kKv4Unit, put = 0;
-    auto head_row = [&](int seq, int h8) { return ((long long)seq * a.kv_heads + h8 / a.head_tiles) * a.capacity; };
-    long long ahead_row = head_row(b, head);
+    // one lane: requests the next unit that has positions.  The warps take turns (one that always did it would hold the others up); how far
+    // the requests are stands in shared memory.
     auto request = [&]() {
-        for (;;) {
-            const int at = ahead_at;
-            if (ahead_b > p_end.b || (ahead_b == p_end.b && (ahead_head > p_end.head || (ahead_head == p_end.head && at >= p_end.unit * kKv4Unit)))) return;
-            const bool there = at < ahead_len;
-            if (there) {
-                const long long from = (ahead_row + at) * kRow;
-                const uint32_t bytes = (uint32_t)(min(kKv4Unit, (ahead_len - at + 3) & ~3) * kRow);  // (the capacity is a multiple of four rows)
-                unsigned char* to = smem + put * kStage;
-                mbar_arrive_expect_tx(&full[put], 2 * bytes);
-                bulk_g2s(to, a.k + from, bytes, &full[put]);
-                bulk_g2s(to + kStage / 2, a.v + from, bytes, &full[put]);
-                if (++put == a.stages) put = 0;
+        Kv4Ahead x = ahead;
+        bool done = false;
+        while (!done && (x.b < p_end.b || (x.b == p_end.b && (x.head < p_end.head || (x.head == p_end.head && x.at < p_end.unit * kKv4Unit))))) {
+            if (x.at < x.len) {
+                const long long from = (((long long)x.b * a.kv_heads + x.head / a.head_tiles) * a.capacity + x.at) * kRow;
+                const uint32_t bytes = (uint32_t)(min(kKv4Unit, (x.len - x.at + 3) & ~3) * kRow);  // (the capacity is a multiple of four rows)
+                unsigned char* to = smem + x.put * kStage;
+                mbar_arrive_expect_tx(&full[x.put], 2 * bytes);
+                bulk_g2s(to, a.k + from, bytes, &full[x.put]);
+                bulk_g2s(to + kStage / 2, a.v + from, bytes, &full[x.put]);
+                if (++x.put == a.stages) x.put = 0;
+                done = true;
             }
-            if ((ahead_at += kKv4Unit) >= ahead_end) {  // the next head
-                ahead_at = 0;
-                if (++ahead_head == heads8) {
-                    ahead_head = 0;
-                    if (++ahead_b < a.batch) ahead_len = kv4_len(a, ahead_b);
-                    ahead_end = kv4_units(ahead_len) * kKv4Unit;
+            if ((x.at += kKv4Unit) >= x.len) {  // the next head
+                x.at = 0;
+                if (++x.head == heads8) {
+                    x.head = 0;
+                    if (++x.b < a.batch) x.len = kv4_len(a, x.b);
                 }
-                ahead_row = head_row(ahead_b, ahead_head);
             }
-            if (there) return;
         }
+        ahead = x;
     };
-    if (tid == 0)
+    if (tid == 0) {
+        ahead = {b, len, head, unit * kKv4Unit, 0};
         for (int i = 0; i < a.stages; ++i) request();
+    }
+    __syncthreads();
+    bool ok = true;
+    int stage = 0, stage_before = -1, turn = 0;
+    uint32_t phase = 0, phase_before = 0;
+
     Kv4Magic magic;
     magic.hide();
-    bool ok = true;
-    int stage = 0, stage_before = -1;
-    uint32_t phase = 0, phase_before = 0;
 
     while (b < p_end.b || (b == p_end.b && (head < p_end.head || (head == p_end.head && unit < p_end.unit)))) {
     const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
@@ -520,31 +525,42 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             kv4_params<NG>(r0, p0);
             kv4_params<NG>(r1, p1w);
             // rows of (scale, zero) pairs as they lie there times (-8 Q, Q)
-            float acc[4];
+            float zacc[4], acc[NG][4];
             if constexpr (NG > 4) {
                 const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
-                kv4_mma(acc, a0, a1, a2, a3, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
-                kv4_mma(acc, a0, a1, a2, a3, zf[1][0], zf[1][1], acc[0], acc[1], acc[2], acc[3]);
+                kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+                kv4_mma(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1], zacc[0], zacc[1], zacc[2], zacc[3]);
             } else {
                 const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
-                kv4_mma(acc, a0, a1, a0, a1, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+                kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+            }
+            // (the groups' chains of products side by side)
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+                kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], 0.f, 0.f, 0.f, 0.f);
+            if constexpr (SPLIT) {
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr)
+                    kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[gr][0], acc[gr][1],
+                            acc[gr][2], acc[gr][3]);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = acc[j] * 0x1p-24f;
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    const uint32_t v0 = w[gr][0] >> 8, v1 = w[gr][1] >> 8;
+                    kv4_mma(acc[gr], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[part][gr][2], qf[part][gr][3], acc[gr][0], acc[gr][1], acc[gr][2],
+                            acc[gr][3]);
+                }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] = zacc[j] * 0x1p-24f;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const uint32_t w0 = w[gr][0], w1 = w[gr][1], v0 = w0 >> 8, v1 = w1 >> 8;
-                kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], 0.f, 0.f, 0.f, 0.f);
-                kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[0][gr][2], qf[0][gr][3], acc[0], acc[1], acc[2], acc[3]);
-                if constexpr (SPLIT) {
-                    kv4_mma(acc, w0 & 0x000f000fu, w1 & 0x000f000fu, w0 & 0x00f000f0u, w1 & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[0], acc[1], acc[2], acc[3]);
-                    kv4_mma(acc, v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[1][gr][2], qf[1][gr][3], acc[0], acc[1], acc[2], acc[3]);
-                }
                 const float s0 = __half2float(__ushort_as_half((unsigned short)p0[gr])), s1 = __half2float(__ushort_as_half((unsigned short)p1w[gr]));
-                s[0] = fmaf(s0, acc[0], s[0]);
-                s[1] = fmaf(s0, acc[1], s[1]);
-                s[2] = fmaf(s1, acc[2], s[2]);
-                s[3] = fmaf(s1, acc[3], s[3]);
+                s[0] = fmaf(s0, acc[gr][0], s[0]);
+                s[1] = fmaf(s0, acc[gr][1], s[1]);
+                s[2] = fmaf(s1, acc[gr][2], s[2]);
+                s[3] = fmaf(s1, acc[gr][3], s[3]);
             }
         }
 #pragma unroll
@@ -566,22 +582,20 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             scores += (long long)kKv4Unit * a.gqa;
         }
         // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
-        float vs[2][NG], vz[2][NG], top[2] = {0x1p-24f, 0x1p-24f};
+        uint32_t vp[2][NG], codes[NG][2];
+        kv4_codes<NG, true>(sv, lane, codes);
+        float top[2];
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
-            uint32_t w[NG];
-            kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, w);
+            kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, vp[r]);
             if (!(r ? in1 : in0)) {
 #pragma unroll
-                for (int gr = 0; gr < NG; ++gr) w[gr] = 0u;
+                for (int gr = 0; gr < NG; ++gr) vp[r][gr] = 0u;
             }
+            __half2 most = *reinterpret_cast<const __half2*>(&vp[r][0]);
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                const float2 f = half2_bits_to_float2(w[gr]);
-                vs[r][gr] = f.x;
-                vz[r][gr] = f.y;
-                top[r] = fmaxf(top[r], f.x);
-            }
+            for (int gr = 1; gr < NG; ++gr) most = __hmax2(most, *reinterpret_cast<const __half2*>(&vp[r][gr]));
+            top[r] = fmaxf(__low2float(most), 0x1p-24f);
         }
         float p[4];  // (a row beyond the end: 0, or NaN while there is no reference, which the vote takes)
 #pragma unroll
@@ -610,31 +624,33 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         l[0] += p[0] + p[2];
         l[1] += p[1] + p[3];
         // ---- values
-        uint32_t codes[NG][2];
-        kv4_codes<NG, true>(sv, lane, codes);
+        uint32_t pf[kParts][NG][2];  // probabilities times scales as operands: rows as the codes have them
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr) {
-            z[gr][0] = fmaf(p[2], vz[1][gr], fmaf(p[0], vz[0][gr], z[gr][0]));
-            z[gr][1] = fmaf(p[3], vz[1][gr], fmaf(p[1], vz[0][gr], z[gr][1]));
-            const float y0 = p[0] * vs[0][gr], y1 = p[1] * vs[0][gr], y2 = p[2] * vs[1][gr], y3 = p[3] * vs[1][gr];
+            const float2 u = half2_bits_to_float2(vp[0][gr]), w = half2_bits_to_float2(vp[1][gr]);
+            z[gr][0] = fmaf(p[2], w.y, fmaf(p[0], u.y, z[gr][0]));
+            z[gr][1] = fmaf(p[3], w.y, fmaf(p[1], u.y, z[gr][1]));
+            const float y0 = p[0] * u.x, y1 = p[1] * u.x, y2 = p[2] * w.x, y3 = p[3] * w.x;
             const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
-            const uint32_t b0 = transpose8(*reinterpret_cast<const uint32_t*>(&ha)), b1 = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
-            const uint32_t xa = codes[gr][0], xb = codes[gr][1];
-            const uint32_t ya = xa >> 8, yb = xb >> 8;
-            const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
-            const uint32_t d0 = kv4_low(ya, magic), d1 = kv4_high(ya, magic), d2 = kv4_low(yb, magic), d3 = kv4_high(yb, magic);
-            float(&oa)[4] = o[2 * gr];
-            float(&ob)[4] = o[2 * gr + 1];
-            kv4_mma(oa, a0, a1, a2, a3, b0, b1, oa[0], oa[1], oa[2], oa[3]);
-            kv4_mma(ob, d0, d1, d2, d3, b0, b1, ob[0], ob[1], ob[2], ob[3]);
+            pf[0][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&ha));
+            pf[0][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
             if constexpr (SPLIT) {
                 const float2 fa = __half22float2(ha), fb = __half22float2(hb);
                 const __half2 la = __floats2half2_rn(y0 - fa.x, y1 - fa.y), lb = __floats2half2_rn(y2 - fb.x, y3 - fb.y);
-                const uint32_t l0 = transpose8(*reinterpret_cast<const uint32_t*>(&la)), l1 = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
-                kv4_mma(oa, a0, a1, a2, a3, l0, l1, oa[0], oa[1], oa[2], oa[3]);
-                kv4_mma(ob, d0, d1, d2, d3, l0, l1, ob[0], ob[1], ob[2], ob[3]);
+                pf[1][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&la));
+                pf[1][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
             }
         }
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
+                const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
+                float(&y)[4] = o[2 * gr + k];
+#pragma unroll
+                for (int part = 0; part < kParts; ++part) kv4_mma(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1], y[0], y[1], y[2], y[3]);
+            }
     };
     const int unit_end = min(p1, (unit + mine) * kKv4Unit);
     for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
@@ -650,12 +666,14 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         else if (at < p1)
             tile(std::false_type(), at);
         __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[stage]);
         // the unit before has been read by all warps but late ones: its place takes the next
-        if (warp == 0 && stage_before >= 0) {
+        if (turn == warp && stage_before >= 0) {
             ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[stage_before], phase_before, nullptr));
             if (lane == 0 && ok) request();
+            __syncwarp();
         }
+        if (lane == 0) mbar_arrive(&empty[stage]);  // (after the request: who makes the next one sees how far it came)
+        turn = (turn + 1) & (kKv4Warps - 1);
         stage_before = stage;
         phase_before = phase;
         if (++stage == a.stages) {
