@@ -113,6 +113,7 @@ AttnLayout attn_layout(int runs, int batch, int n_heads, int64_t capacity, int g
 }
 const char* attn_fault(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size) {
     if (const char* f = size_fault(batch, n_kv_heads, capacity, head_size)) return f;
+    if ((long long)batch * n_heads * (capacity / kKv4Unit + 1 + kKv4Head) > 0x7fffffffll) return "4-bit attention: more than 2^31 pieces of work";
     if (n_heads <= 0 || n_heads % n_kv_heads || n_heads / n_kv_heads > 1024) return "4-bit attention: the key/value heads divide the heads, at most 1024 to one";
     return nullptr;
 }

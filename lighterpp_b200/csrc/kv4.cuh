@@ -206,24 +206,32 @@ __device__ __forceinline__ int kv4_units(int len) { return max(1, (len + kKv4Uni
 // Point kKv4Head + u of a head stands for unit u, the points before for its beginning.
 constexpr int kKv4Head = 4;
 __device__ __forceinline__ int kv4_weight(int len) { return kv4_units(len) + kKv4Head; }
+// The points of all heads cut into runs as even as they come (fewer than 2^31 points; no run is empty).
+struct Kv4Runs {
+    int runs, each, more;  // the first `more` runs have a point more
+    __device__ __forceinline__ Kv4Runs(int most, int points) : runs(min(most, points)), each(points / runs), more(points - each * runs) {}
+    __device__ __forceinline__ int begin(int i) const { return i * each + min(i, more); }
+    __device__ __forceinline__ int of(int point) const {
+        const int longer = more * (each + 1);
+        return point < longer ? point / (each + 1) : more + (point - longer) / each;
+    }
+};
 // Weight of all sequences for one head, by a warp.
-__device__ __forceinline__ long long kv4_total(const Kv4AttnArgs& a) {
-    long long n = 0;
+__device__ __forceinline__ int kv4_total(const Kv4AttnArgs& a) {
+    int n = 0;
     for (int b = threadIdx.x & 31; b < a.batch; b += 32) n += kv4_weight(kv4_len(a, b));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n;
+    return __reduce_add_sync(0xffffffffu, n);
 }
 // Sequence that holds point `at` of all, and its first point, by a warp; `heads` counts a key/value head once per eight query heads.
-__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, long long at, long long& first) {
+__device__ __forceinline__ int kv4_find(const Kv4AttnArgs& a, int heads, int at, int& first) {
     const int lane = threadIdx.x & 31;
-    long long base = 0;
+    int base = 0;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-        const long long own = b0 + lane < a.batch ? (long long)kv4_weight(kv4_len(a, b0 + lane)) * heads : 0;
-        long long x = own;
+        const int own = b0 + lane < a.batch ? kv4_weight(kv4_len(a, b0 + lane)) * heads : 0;
+        int x = own;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, x, o);
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
         const unsigned there = __ballot_sync(0xffffffffu, base + x > at);
@@ -265,12 +273,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// d = a . b + c
-__device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2,
-                                        float c3) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+// d = a . b
+__device__ __forceinline__ void kv4_mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// d += a . b
+__device__ __forceinline__ void kv4_mma_add(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 matrix of 16-bit elements spread over a warp
     uint32_t r;
@@ -364,25 +377,27 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     __shared__ int s_fail;
     pdl_wait();
     pdl_launch_dependents();  // (after the wait: what the finishing kernel reads of the lengths is there when it starts)
-    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, t = lane & 3;
+    int lane = threadIdx.x & 31;
+    asm volatile("" : "+r"(lane));  // (kept, not made again from the special register in every tile)
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), g = lane >> 2, t = lane & 3;
     const int heads8 = a.kv_heads * a.head_tiles;
-    const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);  // (no run is empty)
-    if (blockIdx.x >= runs) return;
+    const Kv4Runs runs(a.runs, kv4_total(a) * heads8);
+    if ((int)blockIdx.x >= runs.runs) return;
     // (sequence, head, unit) of a point
     struct Place {
         int b, len, head, unit;
     };
-    auto place = [&](long long at) {
-        long long first = 0;
+    auto place = [&](int at) {
+        int first = 0;
         Place p;
         p.b = kv4_find(a, heads8, at, first);
         p.len = p.b < a.batch ? kv4_len(a, p.b) : 0;
         const int weight = kv4_weight(p.len);
-        p.head = (int)((at - first) / weight);
-        p.unit = max(0, (int)(at - first - (long long)p.head * weight) - kKv4Head);
+        p.head = (at - first) / weight;
+        p.unit = max(0, at - first - p.head * weight - kKv4Head);
         return p;
     };
-    const Place p_begin = place(all * blockIdx.x / runs), p_end = place(all * (blockIdx.x + 1) / runs);
+    const Place p_begin = place(runs.begin(blockIdx.x)), p_end = place(runs.begin(blockIdx.x + 1));
     if (p_begin.b == p_end.b && p_begin.head == p_end.head && p_begin.unit == p_end.unit) return;
     float* so = reinterpret_cast<float*>(smem + a.stages * kStage);
     if (tid == 0) {
@@ -426,7 +441,6 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         ahead = {b, len, head, unit * kKv4Unit, 0};
         for (int i = 0; i < a.stages; ++i) request();
     }
-    __syncthreads();
     bool ok = true;
     int stage = 0, stage_before = -1, turn = 0;
     uint32_t phase = 0, phase_before = 0;
@@ -528,35 +542,33 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             float zacc[4], acc[NG][4];
             if constexpr (NG > 4) {
                 const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
-                kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
-                kv4_mma(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1], zacc[0], zacc[1], zacc[2], zacc[3]);
+                kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1]);
+                kv4_mma_add(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1]);
             } else {
                 const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
-                kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1], 0.f, 0.f, 0.f, 0.f);
+                kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1]);
             }
             // (the groups' chains of products side by side)
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr)
-                kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1], 0.f, 0.f, 0.f, 0.f);
+                kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1]);
             if constexpr (SPLIT) {
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr)
-                    kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1], acc[gr][0], acc[gr][1],
-                            acc[gr][2], acc[gr][3]);
+                    kv4_mma_add(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1]);
             }
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr) {
                     const uint32_t v0 = w[gr][0] >> 8, v1 = w[gr][1] >> 8;
-                    kv4_mma(acc[gr], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[part][gr][2], qf[part][gr][3], acc[gr][0], acc[gr][1], acc[gr][2],
-                            acc[gr][3]);
+                    kv4_mma_add(acc[gr], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[part][gr][2], qf[part][gr][3]);
                 }
 #pragma unroll
             for (int j = 0; j < 4; ++j) s[j] = zacc[j] * 0x1p-24f;
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
-                const float s0 = __half2float(__ushort_as_half((unsigned short)p0[gr])), s1 = __half2float(__ushort_as_half((unsigned short)p1w[gr]));
+                const float s0 = half2_bits_to_float2(p0[gr]).x, s1 = half2_bits_to_float2(p1w[gr]).x;
                 s[0] = fmaf(s0, acc[gr][0], s[0]);
                 s[1] = fmaf(s0, acc[gr][1], s[1]);
                 s[2] = fmaf(s1, acc[gr][2], s[2]);
@@ -649,7 +661,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
                 float(&y)[4] = o[2 * gr + k];
 #pragma unroll
-                for (int part = 0; part < kParts; ++part) kv4_mma(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1], y[0], y[1], y[2], y[3]);
+                for (int part = 0; part < kParts; ++part) kv4_mma_add(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1]);
             }
     };
     const int unit_end = min(p1, (unit + mine) * kKv4Unit);
@@ -754,16 +766,15 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, b = blockIdx.z, heads8 = a.kv_heads * a.head_tiles;
     const int len = kv4_len(a, b), units = kv4_units(len), weight = kv4_weight(len), row_block = (int)blockIdx.x - a.gqa;
-    const long long all = kv4_total(a) * heads8, runs = min((long long)a.runs, all);
-    long long before = 0;
+    const Kv4Runs runs(a.runs, kv4_total(a) * heads8);
+    int before = 0;
     for (int i = lane; i < b; i += 32) before += kv4_weight(kv4_len(a, i));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    before = __reduce_add_sync(0xffffffffu, before);
     // runs that hold the first and the last unit of a head
     auto runs_of = [&](int tile8, int& r0, int& r1) {
-        const long long u0 = before * heads8 + (long long)(kvh * a.head_tiles + tile8) * weight + kKv4Head, u1 = u0 + units - 1;
-        r0 = (int)(((u0 + 1) * runs - 1) / all);
-        r1 = (int)(((u1 + 1) * runs - 1) / all);
+        const int u0 = before * heads8 + (kvh * a.head_tiles + tile8) * weight + kKv4Head;
+        r0 = runs.of(u0);
+        r1 = runs.of(u0 + units - 1);
     };
     auto part_of = [&](int r, int r0, int h) { return ((long long)r * 2 + (r == r0 ? 1 : 0)) * kKv4Heads + h % kKv4Heads; };
     int r0, r1;
