@@ -270,7 +270,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
                         const lpp_status st = launch_op(kernel, dim3(runs), kKv4Threads, smem, S(stream), a);
                         if (st != LPP_OK) return st;
                         const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;
-                        return launch_op(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + runs) * 4, S(stream), a);
+                        return launch_behind(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + runs) * 4, S(stream), a);
                     }));
 }
 
@@ -314,8 +314,8 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
     const int vec = row % 16 == 0 ? 16 : row % 8 == 0 ? 8 : 4;
     const long long per_head = ((long long)keep * (row / vec) + 255) / 256;
     const dim3 grid((unsigned)std::min<long long>(per_head, std::max<long long>(1, 8ll * sms / (long long)heads)), n_kv_heads, batch);
-    st = vec == 16 ? launch_op(kv4_move_kernel<uint4>, grid, 256, 0, S(stream), a)
-                   : vec == 8 ? launch_op(kv4_move_kernel<uint2>, grid, 256, 0, S(stream), a) : launch_op(kv4_move_kernel<uint32_t>, grid, 256, 0, S(stream), a);
+    st = vec == 16 ? launch_behind(kv4_move_kernel<uint4>, grid, 256, 0, S(stream), a)
+                   : vec == 8 ? launch_behind(kv4_move_kernel<uint2>, grid, 256, 0, S(stream), a) : launch_behind(kv4_move_kernel<uint32_t>, grid, 256, 0, S(stream), a);
     return launched("lpp_op_kv4_evict: the launch failed", st);
 }
 

@@ -363,6 +363,28 @@ __device__ __forceinline__ uint32_t kv4_high(uint32_t x, const Kv4Magic& c) {
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 
+// Barriers by address in shared memory (as pointers, their address is put together again at every use)
+__device__ __forceinline__ bool kv4_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+__device__ __forceinline__ bool kv4_wait(uint32_t bar, uint32_t parity) {  // bounded; the same answer for the whole warp
+    if (__all_sync(0xffffffffu, kv4_try_wait(bar, parity))) return true;
+    const long long t0 = clock64();
+    bool done = false;
+    while (!(done = kv4_try_wait(bar, parity)) && clock64() - t0 < kWaitCycles) {
+    }
+    return __all_sync(0xffffffffu, done);
+}
+__device__ __forceinline__ void kv4_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+
 struct Kv4Ahead {
     int b, len, head, at, put;  // the next unit to be requested, and its place in the ring
 };
@@ -437,6 +459,8 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         }
         ahead = x;
     };
+    uint32_t full_at = smem_u32(full), empty_at = smem_u32(empty), ring_at = smem_u32(smem) + warp * kKv4Tile * kRow;
+    asm volatile("" : "+r"(full_at), "+r"(empty_at), "+r"(ring_at));
     if (tid == 0) {
         ahead = {b, len, head, unit * kKv4Unit, 0};
         for (int i = 0; i < a.stages; ++i) request();
@@ -529,7 +553,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     auto tile = [&](auto whole, int at) {  // whole: every row lies below the length
         constexpr bool kWhole = decltype(whole)::value;
         const bool in0 = kWhole || at + g < p1, in1 = kWhole || at + g + 8 < p1;
-        const uint32_t sk = smem_u32(smem + stage * kStage) + warp * kKv4Tile * kRow, sv = sk + kStage / 2;
+        const uint32_t sk = ring_at + stage * kStage, sv = sk + kStage / 2;
         // ---- scores of rows g and g + 8
         float s[4];
         {
@@ -667,7 +691,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     const int unit_end = min(p1, (unit + mine) * kKv4Unit);
     for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
         const int at = unit_at + warp * kKv4Tile;
-        if (!__all_sync(0xffffffffu, mbar_try_wait(&full[stage], phase))) ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&full[stage], phase, nullptr));
+        ok = ok && kv4_wait(full_at + stage * 8, phase);
         if (!ok) {  // a copy that never came: the results of this run say so
             m[0] = m[1] = NAN;
             s_fail = 1;
@@ -680,11 +704,11 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         __syncwarp();
         // the unit before has been read by all warps but late ones: its place takes the next
         if (turn == warp && stage_before >= 0) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[stage_before], phase_before, nullptr));
+            ok = kv4_wait(empty_at + stage_before * 8, phase_before);
             if (lane == 0 && ok) request();
             __syncwarp();
         }
-        if (lane == 0) mbar_arrive(&empty[stage]);  // (after the request: who makes the next one sees how far it came)
+        if (lane == 0) kv4_arrive(empty_at + stage * 8);  // (after the request: who makes the next one sees how far it came)
         turn = (turn + 1) & (kKv4Warps - 1);
         stage_before = stage;
         phase_before = phase;

@@ -14,11 +14,11 @@ inline int blocks(long long n, int t) { return (int)std::max<long long>(1, (n + 
 
 // Launches an operator kernel.  It may start while the kernel before it in the stream ends (it waits for it in op_begin):
 // 18 operators of a layer one after the other take about a microsecond less each.  A stream that is being captured gets a plain
-// launch, because what comes before it in the graph need not be a kernel.  cluster: CTAs of a cluster along x.
+// launch, because what comes before it in the graph need not be a kernel; behind: it is one, this operator's own.  cluster: CTAs of a cluster along x.
 template <typename... KArgs, typename... Args>
-lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, Args... args) {
+lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, int cluster, bool behind, cudaStream_t s, Args... args) {
     cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(s, &capturing) != cudaSuccess) {
+    if (!behind && cudaStreamIsCapturing(s, &capturing) != cudaSuccess) {
         (void)cudaGetLastError();
         capturing = cudaStreamCaptureStatusActive;
     }
@@ -44,7 +44,11 @@ lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, s
 }
 template <typename... KArgs, typename... Args>
 lpp_status launch_op(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
-    return launch_op_cluster(kernel, grid, threads, smem, 1, s, args...);
+    return launch_op_cluster(kernel, grid, threads, smem, 1, false, s, args...);
+}
+template <typename... KArgs, typename... Args>
+lpp_status launch_behind(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {
+    return launch_op_cluster(kernel, grid, threads, smem, 1, true, s, args...);
 }
 
 }  // namespace
