@@ -23,7 +23,10 @@
 namespace lpp {
 
 constexpr int kPaRows = 128, kPaKeys = 128, kPaSub = 128 * 128;  // kPaSub: bytes of 128 rows x 64 columns
-constexpr int kPaSoftWarps = 8, kPaMmaWarp = 8, kPaLoadWarp = 9, kPaCheckWarp = 10, kPaThreads = 11 * 32;
+constexpr int kPaSoftWarps = 8, kPaMmaWarp = 8, kPaLoadWarp = 9, kPaCheckWarp = 10, kPaThreads = 12 * 32;
+// Registers: 384 threads start with 168 each; the two softmax warpgroups take what the third gives back (2 x 128 x 56 = 128 x 112)
+constexpr int kPaSoftRegs = 224, kPaOtherRegs = 56;
+static_assert(2 * 128 * kPaSoftRegs + 128 * kPaOtherRegs <= 384 * 168, "a split must not ask for more registers than the block was launched with");
 template <int HS>
 constexpr int kPaTileBytes = HS / 64 * kPaSub;
 template <int HS>
@@ -86,6 +89,60 @@ __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t* r) {
         "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Two FP32 values in one instruction
+__device__ __forceinline__ uint64_t f2_pack(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ float2 f2_unpack(uint64_t x) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^x of two values on the FMA pipe, relative error 2^-13.7 (BF16 probabilities) or 2^-18.5 (FP16): x = n + f with n the nearest integer (by
+// adding 1.5 2^23), a minimax polynomial for 2^f on [-1/2, 1/2] (Remez exchange for the relative error), n added to the exponent.  Below
+// 2^-126: 2^-126.
+template <typename T>
+__device__ __forceinline__ float2 pa_exp2_poly(uint64_t x2) {
+    float2 x = f2_unpack(x2);
+    x2 = f2_pack(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+    const uint64_t magic = f2_pack(12582912.f, 12582912.f), back = f2_pack(-12582912.f, -12582912.f), minus = f2_pack(-1.f, -1.f);
+    const uint64_t t = f2_add(x2, magic), f = f2_fma(f2_add(t, back), minus, x2);
+    uint64_t y;
+    if constexpr (std::is_same<T, __half>::value) {
+        y = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
+        y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
+        y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
+        y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
+    } else {
+        y = f2_fma(f2_pack(0.0551716685295105f, 0.0551716685295105f), f, f2_pack(0.2426111251115799f, 0.2426111251115799f));
+        y = f2_fma(y, f, f2_pack(0.6932609677314758f, 0.6932609677314758f));
+        y = f2_fma(y, f, f2_pack(0.9999280571937561f, 0.9999280571937561f));
+    }
+    const float2 n = f2_unpack(t), v = f2_unpack(y);
+    return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(v.y) + (__float_as_int(n.y) << 23)));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float pa_exp2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -119,6 +176,7 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
     constexpr int kPieces = HS / 64, kTile = kPaTileBytes<HS>;
     // FP16 probabilities stay clear of the subnormals: they are 2^(x - m + 6) at most 2^14
     constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
+    constexpr int kPoly = HS == 64 ? 6 : 4;  // of 16 exponentials, how many on the FMA pipe
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full[2], p_ready[2], o_full[2];
     __shared__ uint32_t tmem_slot;
@@ -164,6 +222,8 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
     // some row of the CTA sees only a part of key tile `it`
     auto partial = [&](int it) { return k0 + it * kPaKeys < last_start || k0 + it * kPaKeys + kPaKeys - 1 > t0; };
 
+    if (warp >= kPaSoftWarps) {
+    regs_down<kPaOtherRegs>();
     if (warp == kPaLoadWarp) {
         if (lane == 0) {
             bool ok = true;
@@ -256,7 +316,9 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_clean[b]);
         }
-    } else if (warp < kPaSoftWarps) {
+    }
+    } else {
+        regs_up<kPaSoftRegs>();
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const int r_cta = a.pair_heads ? row : x * kPaRows + row, token = t0 + r_cta, head = head0 + (a.pair_heads ? x : 0);
         const int i_row = min(token, t_end - 1), first = s_start[min(r_cta, t_end - 1 - t0)];
@@ -285,8 +347,9 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
 #pragma unroll
             for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
 #pragma unroll
-            for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
-            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.rate;
+            for (int c = 4; c < 128; ++c) mx[c & 3] = max_nan(mx[c & 3], __uint_as_float(s[c]));
+            const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.rate;
+            if (!(top < INFINITY)) l = NAN;  // a score that is not a number, or infinite
             const bool grows = top > m + kPaGrowth;
             if (__any_sync(0xffffffffu, grows)) {
                 const float next = grows ? top : m, f = grows ? pa_exp2(m - next) : 1.f;  // (from -infinity: 0)
@@ -307,20 +370,28 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
                 }
             }
             const float u = m == -INFINITY ? 0.f : m - kLift;
-            float sum[2] = {0.f, 0.f};
+            const uint64_t rate2 = f2_pack(a.rate, a.rate), u2 = f2_pack(-u, -u);
+            uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t p[32];
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    const float e0 = pa_exp2(fmaf(__uint_as_float(s[c * 64 + 2 * i]), a.rate, -u)), e1 = pa_exp2(fmaf(__uint_as_float(s[c * 64 + 2 * i + 1]), a.rate, -u));
-                    sum[0] += e0;
-                    sum[1] += e1;
-                    p[i] = pack2<T>(e0, e1);
+                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(s[c * 64 + 2 * i]), __uint_as_float(s[c * 64 + 2 * i + 1])), rate2, u2);
+                    float2 e;
+                    if ((i % 16) * kPoly % 16 >= 16 - kPoly) {
+                        e = pa_exp2_poly<T>(y);
+                    } else {
+                        e = f2_unpack(y);
+                        e = make_float2(pa_exp2(e.x), pa_exp2(e.y));
+                    }
+                    sum[i & 1] = f2_add(sum[i & 1], f2_pack(e.x, e.y));
+                    p[i] = pack2<T>(e.x, e.y);
                 }
                 tc_st32(ts + c * 32, p);
             }
-            l += sum[0] + sum[1];
+            const float2 total2 = f2_unpack(f2_add(sum[0], sum[1]));
+            l += total2.x + total2.y;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
