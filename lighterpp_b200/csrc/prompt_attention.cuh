@@ -23,7 +23,7 @@
 namespace lpp {
 
 constexpr int kPaRows = 128, kPaKeys = 128, kPaSub = 128 * 128;  // kPaSub: bytes of 128 rows x 64 columns
-constexpr int kPaSoftWarps = 8, kPaMmaWarp = 8, kPaLoadWarp = 9, kPaCheckWarp = 10, kPaThreads = 12 * 32;
+constexpr int kPaSoftWarps = 8, kPaMmaWarp = 8, kPaLoadWarp = 9, kPaCheckWarp = 10, kPaCheckWarps = 2, kPaThreads = 12 * 32;
 // Registers: 384 threads start with 168 each; the two softmax warpgroups take what the third gives back (2 x 128 x 56 = 128 x 112)
 constexpr int kPaSoftRegs = 224, kPaOtherRegs = 56;
 static_assert(2 * 128 * kPaSoftRegs + 128 * kPaOtherRegs <= 384 * 168, "a split must not ask for more registers than the block was launched with");
@@ -169,6 +169,7 @@ __device__ __forceinline__ int pa_start(const int* offsets, int n, int i) {
     }
     return max(0, min(offsets[lo], i));
 }
+constexpr int kPaOffsets = 1024;  // sequences whose offsets are searched in shared memory
 
 template <int HS, typename T>
 static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
@@ -176,11 +177,14 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
     constexpr int kPieces = HS / 64, kTile = kPaTileBytes<HS>;
     // FP16 probabilities stay clear of the subnormals: they are 2^(x - m + 6) at most 2^14
     constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
-    constexpr int kPoly = HS == 64 ? 6 : 4;  // of 16 exponentials, how many on the FMA pipe
+    constexpr int kPoly = HS == 64 ? 6 : 0;  // of 16 exponentials, how many on the FMA pipe
+    // Head sizes up to 64 leave room for probabilities beside the scores: the next scores are formed while these are exponentiated.
+    constexpr bool kApart = HS == 64;
+    constexpr uint32_t kO = 256, kOWide = HS, kP = kApart ? 384 : 0, kPWide = kApart ? 64 : 128;  // columns of the sums and the probabilities
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full[2], p_ready[2], o_full[2];
+    __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full[2], s_read[2], p_ready[2], o_done[2];
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_fail, s_odd, s_start[2 * kPaRows];
+    __shared__ int s_fail, s_odd, s_start[2 * kPaRows], s_off[kPaOffsets + 1];
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
     const uint32_t sq = base, sk = sq + 2 * kTile, sv = sk + 2 * kTile;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -188,7 +192,15 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
     const int work = blockIdx.x, tile = a.tiles - 1 - work / per_tile, unit = work - (work / per_tile) * per_tile;
     const int cta_rows = a.pair_heads ? kPaRows : 2 * kPaRows, t0 = tile * cta_rows;
     const int head0 = a.pair_heads ? 2 * unit : unit, kvh = head0 / a.gqa;
+    if (tid == 0) {
+        tma_prefetch_map(&q_map);
+        tma_prefetch_map(&k_map);
+        tma_prefetch_map(&v_map);
+    }
     pdl_wait();
+    const bool few = a.n_sequences <= kPaOffsets;
+    if (few)
+        for (int i = tid; i <= a.n_sequences; i += kPaThreads) s_off[i] = a.offsets[i];
     const int total = min(a.offsets[a.n_sequences], a.n_tokens);
     if (t0 >= total) return;
     const int t_end = min(total, t0 + cta_rows);
@@ -201,18 +213,20 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
-            mbar_init(&v_clean[i], 1);
+            mbar_init(&v_clean[i], kPaCheckWarps);
+            mbar_init(&s_read[i], 4);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_ready[i], 4);
-            mbar_init(&o_full[i], 1);
+            mbar_init(&o_done[i], 1);
         }
         mbar_fence_init();
     }
-    if (tid < cta_rows) s_start[tid] = pa_start(a.offsets, a.n_sequences, min(t0 + tid, t_end - 1));
     if (warp == kPaMmaWarp) {
         tc_alloc(&tmem_slot, 512);
         tc_relinquish();
     }
+    __syncthreads();
+    if (tid < cta_rows) s_start[tid] = pa_start(few ? s_off : a.offsets, a.n_sequences, min(t0 + tid, t_end - 1));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -267,9 +281,17 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
         }
         for (int it = 0; it < n_tiles && ok; ++it) {
             const int b = it & 1;
-            ok = wait(&v_full[b], (uint32_t)(it >> 1) & 1u);
-            ok = ok && wait(&v_clean[b], (uint32_t)(it >> 1) & 1u);
-            if (ok && it + 1 < n_tiles) ok = wait(&k_full[b ^ 1], (uint32_t)((it + 1) >> 1) & 1u);
+            const bool more = it + 1 < n_tiles;
+            if (more) ok = wait(&k_full[b ^ 1], (uint32_t)((it + 1) >> 1) & 1u);
+            if constexpr (kApart) {
+                for (int x = 0; x < 2 && ok && more; ++x) {  // these have been taken into registers: their place takes the next
+                    ok = wait(&s_read[x], (uint32_t)it & 1u);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(x, it + 1);
+                }
+            }
+            ok = ok && wait(&v_full[b], (uint32_t)(it >> 1) & 1u) && wait(&v_clean[b], (uint32_t)(it >> 1) & 1u);
             for (int x = 0; x < 2 && ok; ++x) {
                 ok = wait(&p_ready[x], (uint32_t)it & 1u);
                 if (!ok) break;
@@ -277,16 +299,17 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
                 if (elect_one()) {
 #pragma unroll
                     for (int ks = 0; ks < kPaKeys / 16; ++ks)
-                        tc_mma_f16_ts(tmem + 256 + x * 128, tmem + x * 128 + ks * 8, pa_desc_v(sv + b * kTile + ks * 2048), pa_idesc<T>(HS, true), it > 0 || ks > 0 ? 1u : 0u);
+                        tc_mma_f16_ts(tmem + kO + x * kOWide, tmem + kP + x * kPWide + ks * 8, pa_desc_v(sv + b * kTile + ks * 2048), pa_idesc<T>(HS, true),
+                                      it > 0 || ks > 0 ? 1u : 0u);
+                    if (kApart || !more) tc_commit(&o_done[x]);
                     if (x == 1) tc_commit(&v_empty[b]);
-                    if (it + 1 == n_tiles) tc_commit(&o_full[x]);
                 }
                 __syncwarp();
-                if (it + 1 < n_tiles) scores(x, it + 1);  // over the probabilities, which the product before it reads first
+                if (!kApart && more) scores(x, it + 1);  // over the probabilities, which the product before it reads first
             }
         }
         if (!ok) s_fail = 1;
-    } else if (warp == kPaCheckWarp) {
+    } else if (warp >= kPaCheckWarp) {
         constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u, kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
         for (int it = 0; it < n_tiles; ++it) {
             // (every tile passes through here: a wait for a phase is only unambiguous where every phase is visited)
@@ -295,21 +318,31 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
                 s_fail = 1;
                 break;
             }
-            for (int i = lane; i < (partial(it) ? kTile / 16 : 0); i += 32) {
-                const uint32_t at = sv + b * kTile + i * 16;
-                uint32_t w[4], odd = 0;
-                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+            constexpr int kAhead = 8;
+            for (int i0 = (warp - kPaCheckWarp) * 32 + lane; i0 < (partial(it) ? kTile / 16 : 0); i0 += kPaCheckWarps * 32 * kAhead) {
+                uint32_t w[kAhead][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) odd |= ((w[j] & kExp) + kOne) & 0x80008000u;  // an exponent of ones carries into the sign's place
-                if (odd) {
-                    s_odd = 1;
+                for (int k = 0; k < kAhead; ++k)
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+                                 : "r"(sv + b * kTile + (i0 + k * kPaCheckWarps * 32) * 16));
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t o = ((w[j] & kExp) + kOne) & 0x80008000u;
-                        if (o & 0x8000u) w[j] &= 0xffff0000u;
-                        if (o & 0x80000000u) w[j] &= 0x0000ffffu;
+                for (int k = 0; k < kAhead; ++k) {
+                    uint32_t odd = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) odd |= ((w[k][j] & kExp) + kOne) & 0x80008000u;  // an exponent of ones carries into the sign's place
+                    if (odd) {
+                        s_odd = 1;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t o = ((w[k][j] & kExp) + kOne) & 0x80008000u;
+                            if (o & 0x8000u) w[k][j] &= 0xffff0000u;
+                            if (o & 0x80000000u) w[k][j] &= 0x0000ffffu;
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sv + b * kTile + (i0 + k * kPaCheckWarps * 32) * 16), "r"(w[k][0]), "r"(w[k][1]), "r"(w[k][2]),
+                                     "r"(w[k][3])
+                                     : "memory");
                     }
-                    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
                 }
             }
             fence_async_smem();
@@ -324,7 +357,7 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
         const int i_row = min(token, t_end - 1), first = s_start[min(r_cta, t_end - 1 - t0)];
         // what all rows of the warp see in full: keys from the last row's sequence on, up to the first row
         const int w_first = __shfl_sync(0xffffffffu, first, 31), w_last = __shfl_sync(0xffffffffu, i_row, 0);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + x * 128, to = tmem + lanes + 256 + x * 128;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + x * 128, to = tmem + lanes + kO + x * kOWide, tp = tmem + lanes + kP + x * kPWide;
         float m = -INFINITY, l = 0.f;
         bool ok = true;
         for (int it = 0; it < n_tiles && ok; ++it) {
@@ -337,11 +370,20 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             tc_wait_ld();
 #pragma unroll
             for (int c = 0; c < 8; ++c) pin16(s + c * 16);
+            if constexpr (kApart) {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_read[x]);
+            }
             const int key = k0 + it * kPaKeys;
             if (key < w_first || key + kPaKeys - 1 > w_last) {
                 const int lo = first - key, hi = i_row - key;
 #pragma unroll
-                for (int c = 0; c < 128; ++c) s[c] = c >= lo && c <= hi ? s[c] : 0xff800000u;
+                for (int c = 0; c < 128; c += 32) {  // a bit a key
+                    const uint32_t from = lo <= c ? ~0u : lo < c + 32 ? ~0u << (lo - c) : 0u, to_ = hi >= c + 31 ? ~0u : hi >= c ? ~0u >> (31 - (hi - c)) : 0u, seen = from & to_;
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) s[c + i] = seen & (1u << i) ? s[c + i] : 0xff800000u;
+                }
             }
             float mx[4];
 #pragma unroll
@@ -351,7 +393,16 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.rate;
             if (!(top < INFINITY)) l = NAN;  // a score that is not a number, or infinite
             const bool grows = top > m + kPaGrowth;
+            bool summed = !kApart || it == 0;  // the sums, and the probabilities' place, are free: the product of the tile before has run
+            auto wait_summed = [&]() {
+                if (!summed) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (uint32_t)(it - 1) & 1u, nullptr));
+                    tc_fence_after();
+                    summed = true;
+                }
+            };
             if (__any_sync(0xffffffffu, grows)) {
+                wait_summed();
                 const float next = grows ? top : m, f = grows ? pa_exp2(m - next) : 1.f;  // (from -infinity: 0)
                 m = next;
                 l *= f;
@@ -388,7 +439,8 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
                     sum[i & 1] = f2_add(sum[i & 1], f2_pack(e.x, e.y));
                     p[i] = pack2<T>(e.x, e.y);
                 }
-                tc_st32(ts + c * 32, p);
+                if (c == 0) wait_summed();
+                tc_st32(tp + c * 32, p);
             }
             const float2 total2 = f2_unpack(f2_add(sum[0], sum[1]));
             l += total2.x + total2.y;
@@ -397,7 +449,7 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[x]);
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&o_full[x], 0, nullptr));
+        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], kApart ? (uint32_t)(n_tiles - 1) & 1u : 0u, nullptr));
         if (!ok) s_fail = 1;
         tc_fence_after();
         const bool mine = token < t_end;
@@ -420,7 +472,7 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
                         *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
                     }
         }
-        if (ok && mine && *reinterpret_cast<volatile int*>(&s_odd)) {  // (set before the products that o_full waited for)
+        if (ok && mine && *reinterpret_cast<volatile int*>(&s_odd)) {  // (set before the last product)
             for (int it = 0; it < n_tiles; ++it) {
                 if (!partial(it)) continue;
                 const int j1 = min(k0 + it * kPaKeys + kPaKeys - 1, i_row);

@@ -19,6 +19,8 @@ __device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const CUtensorMap
                  : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
+
 // Shared-memory matrix descriptor of a K-major operand tile with the 128-byte swizzle: start address / 16 in bits
 // 0-13, leading byte offset (unused for swizzled K-major, set to 1) in bits 16-29, stride between 8-row groups
 // (1024 bytes) / 16 in bits 32-45, descriptor version 1 in bits 46-47, layout type 2 (128-byte swizzle) in bits 61-63.
