@@ -160,21 +160,23 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
     a.heads = n_heads;
     a.gqa = n_heads / n_kv_heads;
     a.head_size = head_size;
-    a.pair_heads = a.gqa % 2 == 0;
-    const int cta_rows = a.pair_heads ? kPaRows : 2 * kPaRows, per_tile = a.pair_heads ? n_heads / 2 : n_heads;
-    a.tiles = (n_tokens + cta_rows - 1) / cta_rows;
-    a.rate = scale * 1.4426950408889634f;
-    if ((long long)a.tiles * per_tile > 0x7fffffffll) return refuse("prompt attention: too many tokens", LPP_ERR_TOO_LARGE);
-    auto go = [&](auto kernel, int smem) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+    auto go = [&](auto shape, auto* t) {
+        using T = std::remove_pointer_t<decltype(t)>;
+        constexpr int HS = shape.value;
+        using Shape = PaShape<HS>;
+        a.pair_heads = Shape::kTiles == 2 && a.gqa % 2 == 0;
+        const int cta_rows = a.pair_heads ? kPaRows : Shape::kTiles * kPaRows, per_tile = a.pair_heads ? n_heads / 2 : n_heads;
+        a.tiles = (n_tokens + cta_rows - 1) / cta_rows;
+        a.rate = scale * 1.4426950408889634f;
+        if ((long long)a.tiles * per_tile > 0x7fffffffll) return LPP_ERR_TOO_LARGE;
+        if (cudaFuncSetAttribute(prompt_attention_kernel<HS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess) {
             (void)cudaGetLastError();
             return LPP_ERR_CUDA;
         }
-        return launch_op(kernel, dim3(a.tiles * per_tile), kPaThreads, smem, S(stream), q_map, k_map, v_map, a);
+        return launch_op(prompt_attention_kernel<HS, T>, dim3(a.tiles * per_tile), Shape::kThreads, Shape::kSmem, S(stream), q_map, k_map, v_map, a);
     };
-    return launched("lpp_op_prompt_attention: the launch failed",
-                    head_size <= 64 ? (dtype == LPP_F16 ? go(prompt_attention_kernel<64, __half>, kPaSmem<64>) : go(prompt_attention_kernel<64, __nv_bfloat16>, kPaSmem<64>))
-                                    : (dtype == LPP_F16 ? go(prompt_attention_kernel<128, __half>, kPaSmem<128>) : go(prompt_attention_kernel<128, __nv_bfloat16>, kPaSmem<128>)));
+    auto by_type = [&](auto shape) { return dtype == LPP_F16 ? go(shape, (__half*)nullptr) : go(shape, (__nv_bfloat16*)nullptr); };
+    return launched("lpp_op_prompt_attention: too many tokens, or the launch failed", head_size <= 64 ? by_type(Int<64>()) : by_type(Int<128>()));
 }
 
 int64_t lpp_op_kv4_row_bytes(int head_size) { return head_size <= 0 || head_size > 256 ? -1 : kv4_row_bytes(kv4_held_groups(head_size)); }

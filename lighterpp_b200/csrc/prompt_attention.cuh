@@ -1,20 +1,21 @@
 // Causal attention of whole prompts, packed one behind the other, with grouped query heads (the reference runs a prompt token by token
 // through src/model.cpp:178-199): out_i = sum_j softmax_j(scale q_i . k_j) v_j over the tokens j <= i of i's own sequence.
 //
-// A CTA takes two tiles of 128 query rows that read the same keys and values: the same 128 tokens of two heads that share a
-// key/value head (or 256 tokens of one head where heads do not pair up).  Per tile of 128 keys and row tile one tcgen05.mma chain
-// forms the scores S = Q . K^T in tensor memory; a warpgroup, one thread a row, takes the row into registers, forms the
-// probabilities and writes them back over the scores as the 16-bit operand of the second chain, O += P . V, whose sums stay in tensor
-// memory.  The two row tiles take turns: while one's rows are exponentiated the tensor cores work for the other.
-//     tensor memory columns: S/P of tile 0 | S/P of tile 1 | O of tile 0 | O of tile 1, 128 each
-// Sums O are rescaled only when a row's maximum has grown by more than 2^8 since it was last set: they are complete whenever the
-// scores of the next key tile are (the tensor cores work in order), so the row's own thread does it.
+// Tiles of 128 query rows of a head against tiles of 128 keys.  One tcgen05.mma chain forms the scores S = Q . K^T in tensor memory; four
+// warps, one thread a row, take them into registers, form the probabilities and write them to tensor memory as the 16-bit operand of
+// the second chain, O += P . V, whose sums stay there.  While rows are exponentiated the tensor cores work on something else:
+// * head sizes up to 64: a CTA has one row tile and half of an SM's tensor memory (S 128 columns, P 64, O 64).  The next scores are
+//   formed while the present ones, already in registers, are exponentiated, and a second CTA on the SM fills what is left.
+// * head sizes up to 128: a CTA has two row tiles that read the same keys and values (two heads that share them, or 256 tokens), and
+//   all of the tensor memory: S 128 columns and O 128 for either.  P takes the place of S, and the row tiles take turns.
+// Sums O are rescaled only when a row's maximum has grown by more than 2^8 since it was last set, by the row's own thread, when the
+// product of the tile before is complete.
 //
 // Sequences do not have to begin at tiles: row tiles cover the packed tokens whatever the borders, a row sees the keys from its
 // sequence's start to itself, and a tile runs over the keys from its first row's sequence on.  Many short prompts share a tile.
 //
 // Keys of tokens that a row does not see are masked after the product; their values meet probabilities of 0, which hides everything but
-// NaN and infinity.  So a warp looks through the value tiles that some row sees only in part, zeroes what is not finite, and the rows
+// NaN and infinity.  So two warps look through the value tiles that some row sees only in part, zero what is not finite, and the rows
 // that do see it get it added to their results at the end.
 #pragma once
 #include "common.cuh"
@@ -23,22 +24,30 @@
 namespace lpp {
 
 constexpr int kPaRows = 128, kPaKeys = 128, kPaSub = 128 * 128;  // kPaSub: bytes of 128 rows x 64 columns
-constexpr int kPaSoftWarps = 8, kPaMmaWarp = 8, kPaLoadWarp = 9, kPaCheckWarp = 10, kPaCheckWarps = 2, kPaThreads = 12 * 32;
-// Registers: 384 threads start with 168 each; the two softmax warpgroups take what the third gives back (2 x 128 x 56 = 128 x 112)
-constexpr int kPaSoftRegs = 224, kPaOtherRegs = 56;
-static_assert(2 * 128 * kPaSoftRegs + 128 * kPaOtherRegs <= 384 * 168, "a split must not ask for more registers than the block was launched with");
+constexpr float kPaGrowth = 8.f;     // of a row's maximum (base 2) before its sums are rescaled
+constexpr int kPaOffsets = 1024;     // sequences whose offsets are searched in shared memory
+constexpr int kPaCheckWarps = 2;
 template <int HS>
-constexpr int kPaTileBytes = HS / 64 * kPaSub;
-template <int HS>
-constexpr int kPaSmem = 1024 /*alignment*/ + 6 * kPaTileBytes<HS>;  // 2 x Q, 2 x K, 2 x V
-constexpr float kPaGrowth = 8.f;  // of a row's maximum (base 2) before its sums are rescaled
+struct PaShape {
+    static constexpr int kTiles = HS == 64 ? 1 : 2, kCtas = HS == 64 ? 2 : 1;  // row tiles of a CTA, CTAs of an SM
+    static constexpr int kSoftWarps = 4 * kTiles, kMmaWarp = kSoftWarps, kLoadWarp = kSoftWarps + 1, kCheckWarp = kSoftWarps + 2, kThreads = (kSoftWarps + 4) * 32;
+    // Registers: the threads start with kRegs each; the softmax warps take what the other four give back
+    static constexpr int kRegs = HS == 64 ? 128 : 168, kSoftRegs = HS == 64 ? 200 : 224, kOtherRegs = 56;
+    static_assert(kSoftWarps * 32 * kSoftRegs + 128 * kOtherRegs <= kThreads * kRegs && kThreads * kRegs * kCtas <= 65536,
+                  "a split must not ask for more registers than the block was launched with");
+    static constexpr int kTile = HS / 64 * kPaSub;                            // bytes of 128 rows
+    static constexpr int kSmem = 1024 /*alignment*/ + (kTiles + 4) * kTile;  // Q, 2 x K, 2 x V
+    static constexpr bool kApart = HS == 64;                                  // probabilities beside the scores, not over them
+    static constexpr uint32_t kColumns = HS == 64 ? 256 : 512, kP = kApart ? 128 : 0, kO = HS == 64 ? 192 : 256;  // tensor memory; S at 0; 128 columns further for row tile 1
+};
 
 struct PromptAttnArgs {
     void* out;
     const void* v;        // for rows that see a value that is not finite
     const int* offsets;   // [sequences + 1]
     long long out_stride, v_stride;
-    int n_sequences, n_tokens, heads, gqa, head_size, pair_heads, tiles;
+    int n_sequences, n_tokens, heads, gqa, head_size, tiles;
+    int pair_heads;       // two row tiles: 128 tokens of two heads; else 256 tokens of one
     float rate;           // scale * log2(e)
 };
 
@@ -115,29 +124,6 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
-// 2^x of two values on the FMA pipe, relative error 2^-13.7 (BF16 probabilities) or 2^-18.5 (FP16): x = n + f with n the nearest integer (by
-// adding 1.5 2^23), a minimax polynomial for 2^f on [-1/2, 1/2] (Remez exchange for the relative error), n added to the exponent.  Below
-// 2^-126: 2^-126.
-template <typename T>
-__device__ __forceinline__ float2 pa_exp2_poly(uint64_t x2) {
-    float2 x = f2_unpack(x2);
-    x2 = f2_pack(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
-    const uint64_t magic = f2_pack(12582912.f, 12582912.f), back = f2_pack(-12582912.f, -12582912.f), minus = f2_pack(-1.f, -1.f);
-    const uint64_t t = f2_add(x2, magic), f = f2_fma(f2_add(t, back), minus, x2);
-    uint64_t y;
-    if constexpr (std::is_same<T, __half>::value) {
-        y = f2_fma(f2_pack(0.009570102207362652f, 0.009570102207362652f), f, f2_pack(0.05591785907745361f, 0.05591785907745361f));
-        y = f2_fma(y, f, f2_pack(0.240247443318367f, 0.240247443318367f));
-        y = f2_fma(y, f, f2_pack(0.6931217908859253f, 0.6931217908859253f));
-        y = f2_fma(y, f, f2_pack(0.9999992847442627f, 0.9999992847442627f));
-    } else {
-        y = f2_fma(f2_pack(0.0551716685295105f, 0.0551716685295105f), f, f2_pack(0.2426111251115799f, 0.2426111251115799f));
-        y = f2_fma(y, f, f2_pack(0.6932609677314758f, 0.6932609677314758f));
-        y = f2_fma(y, f, f2_pack(0.9999280571937561f, 0.9999280571937561f));
-    }
-    const float2 n = f2_unpack(t), v = f2_unpack(y);
-    return make_float2(__int_as_float(__float_as_int(v.x) + (__float_as_int(n.x) << 23)), __int_as_float(__float_as_int(v.y) + (__float_as_int(n.y) << 23)));
-}
 __device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
@@ -169,42 +155,32 @@ __device__ __forceinline__ int pa_start(const int* offsets, int n, int i) {
     }
     return max(0, min(offsets[lo], i));
 }
-constexpr int kPaOffsets = 1024;  // sequences whose offsets are searched in shared memory
-
 template <int HS, typename T>
-static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map, const __grid_constant__ CUtensorMap k_map,
-                                                                                const __grid_constant__ CUtensorMap v_map, const PromptAttnArgs a) {
-    constexpr int kPieces = HS / 64, kTile = kPaTileBytes<HS>;
+static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCtas) prompt_attention_kernel(const __grid_constant__ CUtensorMap q_map,
+                                                                                                            const __grid_constant__ CUtensorMap k_map,
+                                                                                                            const __grid_constant__ CUtensorMap v_map, const PromptAttnArgs a) {
+    using Shape = PaShape<HS>;
+    constexpr int kPieces = HS / 64, kTile = Shape::kTile, kTiles = Shape::kTiles;
+    constexpr bool kApart = Shape::kApart;
     // FP16 probabilities stay clear of the subnormals: they are 2^(x - m + 6) at most 2^14
     constexpr float kLift = std::is_same<T, __half>::value ? 6.f : 0.f;
-    constexpr int kPoly = HS == 64 ? 6 : 0;  // of 16 exponentials, how many on the FMA pipe
-    // Head sizes up to 64 leave room for probabilities beside the scores: the next scores are formed while these are exponentiated.
-    constexpr bool kApart = HS == 64;
-    constexpr uint32_t kO = 256, kOWide = HS, kP = kApart ? 384 : 0, kPWide = kApart ? 64 : 128;  // columns of the sums and the probabilities
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full[2], s_read[2], p_ready[2], o_done[2];
+    __shared__ uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_clean[2], s_full[kTiles], s_read[kTiles], p_ready[kTiles], o_done[kTiles];
     __shared__ uint32_t tmem_slot;
-    __shared__ int s_fail, s_odd, s_start[2 * kPaRows], s_off[kPaOffsets + 1];
+    __shared__ int s_fail, s_odd, s_start[kTiles * kPaRows], s_off[kPaOffsets + 1];
     const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
-    const uint32_t sq = base, sk = sq + 2 * kTile, sv = sk + 2 * kTile;
+    const uint32_t sq = base, sk = sq + kTiles * kTile, sv = sk + 2 * kTile;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
-    const int per_tile = a.pair_heads ? a.heads / 2 : a.heads;
-    const int work = blockIdx.x, tile = a.tiles - 1 - work / per_tile, unit = work - (work / per_tile) * per_tile;
-    const int cta_rows = a.pair_heads ? kPaRows : 2 * kPaRows, t0 = tile * cta_rows;
-    const int head0 = a.pair_heads ? 2 * unit : unit, kvh = head0 / a.gqa;
+    const bool pair = kTiles == 2 && a.pair_heads;
+    // The last row tiles come first: of one sequence they are the longest.  (Several sequences' tiles sorted by length, so that long ones share
+    // SMs: ten packed prompts of up to 1500 tokens 49 us against 47.)
+    const int per_tile = pair ? a.heads / 2 : a.heads, rank = (int)blockIdx.x / per_tile, unit = (int)blockIdx.x - rank * per_tile;
+    const int cta_rows = pair ? kPaRows : kTiles * kPaRows, t0 = (a.tiles - 1 - rank) * cta_rows;
+    const int head0 = pair ? 2 * unit : unit, kvh = head0 / a.gqa;
     if (tid == 0) {
         tma_prefetch_map(&q_map);
         tma_prefetch_map(&k_map);
         tma_prefetch_map(&v_map);
-    }
-    pdl_wait();
-    const bool few = a.n_sequences <= kPaOffsets;
-    if (few)
-        for (int i = tid; i <= a.n_sequences; i += kPaThreads) s_off[i] = a.offsets[i];
-    const int total = min(a.offsets[a.n_sequences], a.n_tokens);
-    if (t0 >= total) return;
-    const int t_end = min(total, t0 + cta_rows);
-    if (tid == 0) {
         s_fail = 0;
         s_odd = 0;
         mbar_init(&q_full, 1);
@@ -214,15 +190,24 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             mbar_init(&v_full[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&v_clean[i], kPaCheckWarps);
-            mbar_init(&s_read[i], 4);
+        }
+        for (int i = 0; i < kTiles; ++i) {
             mbar_init(&s_full[i], 1);
+            mbar_init(&s_read[i], 4);
             mbar_init(&p_ready[i], 4);
             mbar_init(&o_done[i], 1);
         }
         mbar_fence_init();
     }
-    if (warp == kPaMmaWarp) {
-        tc_alloc(&tmem_slot, 512);
+    pdl_wait();
+    const bool few = a.n_sequences <= kPaOffsets;
+    if (few)
+        for (int i = tid; i <= a.n_sequences; i += Shape::kThreads) s_off[i] = a.offsets[i];
+    const int total = min(a.offsets[a.n_sequences], a.n_tokens);
+    if (t0 >= total) return;
+    const int t_end = min(total, t0 + cta_rows);
+    if (warp == Shape::kMmaWarp) {
+        tc_alloc(&tmem_slot, Shape::kColumns);
         tc_relinquish();
     }
     __syncthreads();
@@ -235,154 +220,159 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
     const int k0 = s_start[0], n_tiles = (t_end - 1 - k0) / kPaKeys + 1, last_start = s_start[t_end - 1 - t0];
     // some row of the CTA sees only a part of key tile `it`
     auto partial = [&](int it) { return k0 + it * kPaKeys < last_start || k0 + it * kPaKeys + kPaKeys - 1 > t0; };
+    auto wait = [](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, (uint32_t)phase & 1u, nullptr)) != 0; };
 
-    if (warp >= kPaSoftWarps) {
-    regs_down<kPaOtherRegs>();
-    if (warp == kPaLoadWarp) {
-        if (lane == 0) {
-            bool ok = true;
-            mbar_arrive_expect_tx(&q_full, 2 * kTile);
-            for (int x = 0; x < 2; ++x)
-                for (int p = 0; p < kPieces; ++p)
-                    tma_load_3d(sq + x * kTile + p * kPaSub, &q_map, p * 64, a.pair_heads ? head0 + x : head0, t0 + (a.pair_heads ? 0 : x * kPaRows), smem_u32(&q_full));
-            for (int it = 0; it < n_tiles && ok; ++it) {
-                const int b = it & 1;
-                const uint32_t par = (uint32_t)((it >> 1) - 1) & 1u;
-                ok = it < 2 || mbar_wait_bounded(&k_empty[b], par, nullptr);
-                if (!ok) break;
-                mbar_arrive_expect_tx(&k_full[b], kTile);
-                for (int p = 0; p < kPieces; ++p) tma_load_3d(sk + b * kTile + p * kPaSub, &k_map, p * 64, kvh, k0 + it * kPaKeys, smem_u32(&k_full[b]));
-                ok = it < 2 || mbar_wait_bounded(&v_empty[b], par, nullptr);
-                if (!ok) break;
-                mbar_arrive_expect_tx(&v_full[b], kTile);
-                for (int p = 0; p < kPieces; ++p) tma_load_3d(sv + b * kTile + p * kPaSub, &v_map, p * 64, kvh, k0 + it * kPaKeys, smem_u32(&v_full[b]));
-            }
-            if (!ok) s_fail = 1;
-        }
-    } else if (warp == kPaMmaWarp) {
-        auto scores = [&](int x, int it) {
-            if (elect_one()) {
-#pragma unroll
-                for (int ks = 0; ks < HS / 16; ++ks) {
-                    const uint32_t off = (uint32_t)((ks >> 2) * kPaSub + (ks & 3) * 32);
-                    tc_mma_f16(tmem + x * 128, umma_desc(sq + x * kTile + off), umma_desc(sk + (it & 1) * kTile + off), pa_idesc<T>(kPaKeys, false), ks > 0 ? 1u : 0u);
-                }
-                tc_commit(&s_full[x]);
-                if (x == 1) tc_commit(&k_empty[it & 1]);
-            }
-            __syncwarp();
-        };
-        auto wait = [](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, nullptr)) != 0; };
-        bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
-        if (ok) {
-            tc_fence_after();
-            scores(0, 0);
-            scores(1, 0);
-        }
-        for (int it = 0; it < n_tiles && ok; ++it) {
-            const int b = it & 1;
-            const bool more = it + 1 < n_tiles;
-            if (more) ok = wait(&k_full[b ^ 1], (uint32_t)((it + 1) >> 1) & 1u);
-            if constexpr (kApart) {
-                for (int x = 0; x < 2 && ok && more; ++x) {  // these have been taken into registers: their place takes the next
-                    ok = wait(&s_read[x], (uint32_t)it & 1u);
+    if (warp >= Shape::kSoftWarps) {
+        regs_down<Shape::kOtherRegs>();
+        if (warp == Shape::kLoadWarp) {
+            // ---------------- queries, keys and values
+            if (lane == 0) {
+                auto load = [&](uint32_t to, const CUtensorMap* map, int head, int token, uint64_t* bar) {
+                    for (int p = 0; p < kPieces; ++p) tma_load_3d(to + p * kPaSub, map, p * 64, head, token, smem_u32(bar));
+                };
+                mbar_arrive_expect_tx(&q_full, kTiles * kTile);
+                for (int x = 0; x < kTiles; ++x) load(sq + x * kTile, &q_map, head0 + (pair ? x : 0), t0 + (pair ? 0 : x * kPaRows), &q_full);
+                bool ok = true;
+                for (int it = 0; it < n_tiles && ok; ++it) {
+                    const int b = it & 1;
+                    ok = it < 2 || mbar_wait_bounded(&k_empty[b], (uint32_t)((it >> 1) - 1) & 1u, nullptr);
                     if (!ok) break;
-                    tc_fence_after();
-                    scores(x, it + 1);
+                    mbar_arrive_expect_tx(&k_full[b], kTile);
+                    load(sk + b * kTile, &k_map, kvh, k0 + it * kPaKeys, &k_full[b]);
+                    ok = it < 2 || mbar_wait_bounded(&v_empty[b], (uint32_t)((it >> 1) - 1) & 1u, nullptr);
+                    if (!ok) break;
+                    mbar_arrive_expect_tx(&v_full[b], kTile);
+                    load(sv + b * kTile, &v_map, kvh, k0 + it * kPaKeys, &v_full[b]);
                 }
+                if (!ok) s_fail = 1;
             }
-            ok = ok && wait(&v_full[b], (uint32_t)(it >> 1) & 1u) && wait(&v_clean[b], (uint32_t)(it >> 1) & 1u);
-            for (int x = 0; x < 2 && ok; ++x) {
-                ok = wait(&p_ready[x], (uint32_t)it & 1u);
-                if (!ok) break;
-                tc_fence_after();
+        } else if (warp == Shape::kMmaWarp) {
+            // ---------------- products
+            auto scores = [&](int x, int it) {
                 if (elect_one()) {
 #pragma unroll
-                    for (int ks = 0; ks < kPaKeys / 16; ++ks)
-                        tc_mma_f16_ts(tmem + kO + x * kOWide, tmem + kP + x * kPWide + ks * 8, pa_desc_v(sv + b * kTile + ks * 2048), pa_idesc<T>(HS, true),
-                                      it > 0 || ks > 0 ? 1u : 0u);
-                    if (kApart || !more) tc_commit(&o_done[x]);
-                    if (x == 1) tc_commit(&v_empty[b]);
+                    for (int ks = 0; ks < HS / 16; ++ks) {
+                        const uint32_t off = (uint32_t)((ks >> 2) * kPaSub + (ks & 3) * 32);
+                        tc_mma_f16(tmem + x * 128, umma_desc(sq + x * kTile + off), umma_desc(sk + (it & 1) * kTile + off), pa_idesc<T>(kPaKeys, false), ks > 0 ? 1u : 0u);
+                    }
+                    tc_commit(&s_full[x]);
+                    if (x == kTiles - 1) tc_commit(&k_empty[it & 1]);
                 }
                 __syncwarp();
-                if (!kApart && more) scores(x, it + 1);  // over the probabilities, which the product before it reads first
+            };
+            bool ok = wait(&q_full, 0) && wait(&k_full[0], 0);
+            if (ok) {
+                tc_fence_after();
+                for (int x = 0; x < kTiles; ++x) scores(x, 0);
             }
-        }
-        if (!ok) s_fail = 1;
-    } else if (warp >= kPaCheckWarp) {
-        constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u, kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
-        for (int it = 0; it < n_tiles; ++it) {
-            // (every tile passes through here: a wait for a phase is only unambiguous where every phase is visited)
-            const int b = it & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&v_full[b], (uint32_t)(it >> 1) & 1u, nullptr))) {
-                s_fail = 1;
-                break;
-            }
-            constexpr int kAhead = 8;
-            for (int i0 = (warp - kPaCheckWarp) * 32 + lane; i0 < (partial(it) ? kTile / 16 : 0); i0 += kPaCheckWarps * 32 * kAhead) {
-                uint32_t w[kAhead][4];
+            for (int it = 0; it < n_tiles && ok; ++it) {
+                const int b = it & 1;
+                const bool more = it + 1 < n_tiles;
+                if (more) ok = wait(&k_full[b ^ 1], (it + 1) >> 1);
+                if (kApart && more && ok) {  // the scores have been taken into registers: their place takes the next
+                    ok = wait(&s_read[0], it);
+                    if (!ok) break;
+                    tc_fence_after();
+                    scores(0, it + 1);
+                }
+                ok = ok && wait(&v_full[b], it >> 1) && wait(&v_clean[b], it >> 1);
+                for (int x = 0; x < kTiles && ok; ++x) {
+                    ok = wait(&p_ready[x], it);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kAhead; ++k)
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
-                                 : "r"(sv + b * kTile + (i0 + k * kPaCheckWarps * 32) * 16));
-#pragma unroll
-                for (int k = 0; k < kAhead; ++k) {
-                    uint32_t odd = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) odd |= ((w[k][j] & kExp) + kOne) & 0x80008000u;  // an exponent of ones carries into the sign's place
-                    if (odd) {
-                        s_odd = 1;
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t o = ((w[k][j] & kExp) + kOne) & 0x80008000u;
-                            if (o & 0x8000u) w[k][j] &= 0xffff0000u;
-                            if (o & 0x80000000u) w[k][j] &= 0x0000ffffu;
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sv + b * kTile + (i0 + k * kPaCheckWarps * 32) * 16), "r"(w[k][0]), "r"(w[k][1]), "r"(w[k][2]),
-                                     "r"(w[k][3])
-                                     : "memory");
+                        for (int ks = 0; ks < kPaKeys / 16; ++ks)
+                            tc_mma_f16_ts(tmem + Shape::kO + x * 128, tmem + Shape::kP + x * 128 + ks * 8, pa_desc_v(sv + b * kTile + ks * 2048), pa_idesc<T>(HS, true),
+                                          it > 0 || ks > 0 ? 1u : 0u);
+                        if (kApart || !more) tc_commit(&o_done[x]);
+                        if (x == kTiles - 1) tc_commit(&v_empty[b]);
                     }
+                    __syncwarp();
+                    if (!kApart && more) scores(x, it + 1);  // over the probabilities, which the product before it reads first
                 }
             }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_clean[b]);
+            if (!ok) s_fail = 1;
+        } else {
+            // ---------------- values that are not finite
+            constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u, kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
+            constexpr int kAhead = 8, kStep = kPaCheckWarps * 32;
+            static_assert(kTile / 16 % (kAhead * kStep) == 0, "a tile is a whole number of rounds");
+            for (int it = 0; it < n_tiles; ++it) {
+                // (every tile passes through here: a wait for a phase is only unambiguous where every phase is visited)
+                const int b = it & 1;
+                if (!wait(&v_full[b], it >> 1)) {
+                    s_fail = 1;
+                    break;
+                }
+                for (int i0 = (warp - Shape::kCheckWarp) * 32 + lane; i0 < (partial(it) ? kTile / 16 : 0); i0 += kAhead * kStep) {
+                    uint32_t w[kAhead][4];
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[k][0]), "=r"(w[k][1]), "=r"(w[k][2]), "=r"(w[k][3])
+                                     : "r"(sv + b * kTile + (i0 + k * kStep) * 16));
+#pragma unroll
+                    for (int k = 0; k < kAhead; ++k) {
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) odd |= ((w[k][j] & kExp) + kOne) & 0x80008000u;  // an exponent of ones carries into the sign's place
+                        if (odd) {
+                            s_odd = 1;
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const uint32_t o = ((w[k][j] & kExp) + kOne) & 0x80008000u;
+                                if (o & 0x8000u) w[k][j] &= 0xffff0000u;
+                                if (o & 0x80000000u) w[k][j] &= 0x0000ffffu;
+                            }
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(sv + b * kTile + (i0 + k * kStep) * 16), "r"(w[k][0]), "r"(w[k][1]), "r"(w[k][2]), "r"(w[k][3])
+                                         : "memory");
+                        }
+                    }
+                }
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_clean[b]);
+            }
         }
-    }
     } else {
-        regs_up<kPaSoftRegs>();
-        const int x = warp >> 2, row = (warp & 3) * 32 + lane;
-        const int r_cta = a.pair_heads ? row : x * kPaRows + row, token = t0 + r_cta, head = head0 + (a.pair_heads ? x : 0);
+        // ---------------- probabilities and results: a thread a row
+        regs_up<Shape::kSoftRegs>();
+        const int x = warp >> 2, row = (warp & 3) * 32 + lane, r_cta = pair ? row : x * kPaRows + row;
+        const int token = t0 + r_cta, head = head0 + (pair ? x : 0);
         const int i_row = min(token, t_end - 1), first = s_start[min(r_cta, t_end - 1 - t0)];
-        // what all rows of the warp see in full: keys from the last row's sequence on, up to the first row
+        // what all rows of the warp see: keys from the last row's sequence on, up to the first row
         const int w_first = __shfl_sync(0xffffffffu, first, 31), w_last = __shfl_sync(0xffffffffu, i_row, 0);
-        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, ts = tmem + lanes + x * 128, to = tmem + lanes + kO + x * kOWide, tp = tmem + lanes + kP + x * kPWide;
-        float m = -INFINITY, l = 0.f;
+        const uint32_t tm = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * 128;
+        const uint64_t rate2 = f2_pack(a.rate, a.rate);
+        float m = -INFINITY, l = 0.f;  // reference of the exponentials (base 2), sum of the probabilities
         bool ok = true;
         for (int it = 0; it < n_tiles && ok; ++it) {
-            ok = __all_sync(0xffffffffu, mbar_wait_bounded(&s_full[x], (uint32_t)it & 1u, nullptr));
+            ok = wait(&s_full[x], it);
             if (!ok) break;
             tc_fence_after();
             uint32_t s[128];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) tc_ld32_async(ts + c * 32, s + c * 32);
+            for (int c = 0; c < 128; c += 32) tc_ld32_async(tm + c, s + c);
             tc_wait_ld();
 #pragma unroll
-            for (int c = 0; c < 8; ++c) pin16(s + c * 16);
+            for (int c = 0; c < 128; c += 16) pin16(s + c);
             if constexpr (kApart) {
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_read[x]);
             }
             const int key = k0 + it * kPaKeys;
+            uint32_t blank = 0;  // bit c: no row of the warp sees any of the keys 32 c .. 32 c + 31
             if (key < w_first || key + kPaKeys - 1 > w_last) {
                 const int lo = first - key, hi = i_row - key;
 #pragma unroll
-                for (int c = 0; c < 128; c += 32) {  // a bit a key
-                    const uint32_t from = lo <= c ? ~0u : lo < c + 32 ? ~0u << (lo - c) : 0u, to_ = hi >= c + 31 ? ~0u : hi >= c ? ~0u >> (31 - (hi - c)) : 0u, seen = from & to_;
+                for (int c = 0; c < 4; ++c) {
+                    const int lo_c = lo - 32 * c, hi_c = hi - 32 * c;
+                    const uint32_t seen = (lo_c <= 0 ? ~0u : lo_c < 32 ? ~0u << lo_c : 0u) & (hi_c >= 31 ? ~0u : hi_c >= 0 ? ~0u >> (31 - hi_c) : 0u);
+                    if (kTiles == 1 && !__any_sync(0xffffffffu, seen != 0u)) blank |= 1u << c;
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) s[c + i] = seen & (1u << i) ? s[c + i] : 0xff800000u;
+                    for (int i = 0; i < 32; ++i) s[c * 32 + i] = seen & (1u << i) ? s[c * 32 + i] : 0xff800000u;
                 }
             }
             float mx[4];
@@ -392,85 +382,88 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
             for (int c = 4; c < 128; ++c) mx[c & 3] = max_nan(mx[c & 3], __uint_as_float(s[c]));
             const float top = max_nan(max_nan(mx[0], mx[1]), max_nan(mx[2], mx[3])) * a.rate;
             if (!(top < INFINITY)) l = NAN;  // a score that is not a number, or infinite
-            const bool grows = top > m + kPaGrowth;
-            bool summed = !kApart || it == 0;  // the sums, and the probabilities' place, are free: the product of the tile before has run
+            bool summed = !kApart || it == 0;  // the product of the tile before has run: sums and the probabilities' place are free
             auto wait_summed = [&]() {
                 if (!summed) {
-                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], (uint32_t)(it - 1) & 1u, nullptr));
+                    ok = wait(&o_done[x], it - 1);
                     tc_fence_after();
                     summed = true;
                 }
             };
+            const bool grows = top > m + kPaGrowth;
             if (__any_sync(0xffffffffu, grows)) {
-                wait_summed();
                 const float next = grows ? top : m, f = grows ? pa_exp2(m - next) : 1.f;  // (from -infinity: 0)
                 m = next;
                 l *= f;
                 if (it > 0) {
+                    wait_summed();
 #pragma unroll
-                    for (int c = 0; c < HS / 32; ++c) {
+                    for (int c = 0; c < HS; c += 32) {
                         uint32_t o[32];
-                        tc_ld32_async(to + c * 32, o);
+                        tc_ld32_async(tm + Shape::kO + c, o);
                         tc_wait_ld();
                         pin16(o);
                         pin16(o + 16);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        tc_st32(to + c * 32, o);
+                        tc_st32(tm + Shape::kO + c, o);
                     }
                 }
             }
             const float u = m == -INFINITY ? 0.f : m - kLift;
-            const uint64_t rate2 = f2_pack(a.rate, a.rate), u2 = f2_pack(-u, -u);
+            const uint64_t u2 = f2_pack(-u, -u);
             uint64_t sum[2] = {0ull, 0ull};
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 uint32_t p[32];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(s[c * 64 + 2 * i]), __uint_as_float(s[c * 64 + 2 * i + 1])), rate2, u2);
-                    float2 e;
-                    if ((i % 16) * kPoly % 16 >= 16 - kPoly) {
-                        e = pa_exp2_poly<T>(y);
-                    } else {
-                        e = f2_unpack(y);
-                        e = make_float2(pa_exp2(e.x), pa_exp2(e.y));
+                for (int h = 0; h < 2; ++h) {
+                    if (kTiles == 1 && (blank & (1u << (2 * c + h)))) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) p[h * 16 + i] = 0u;
+                        continue;
                     }
-                    sum[i & 1] = f2_add(sum[i & 1], f2_pack(e.x, e.y));
-                    p[i] = pack2<T>(e.x, e.y);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int at = c * 64 + h * 32 + 2 * i;
+                        const uint64_t y = f2_fma(f2_pack(__uint_as_float(s[at]), __uint_as_float(s[at + 1])), rate2, u2);
+                        const float2 z = f2_unpack(y);
+                        const float e0 = pa_exp2(z.x), e1 = pa_exp2(z.y);
+                        sum[i & 1] = f2_add(sum[i & 1], f2_pack(e0, e1));
+                        p[h * 16 + i] = pack2<T>(e0, e1);
+                    }
                 }
                 if (c == 0) wait_summed();
-                tc_st32(tp + c * 32, p);
+                tc_st32(tm + Shape::kP + c * 32, p);
             }
-            const float2 total2 = f2_unpack(f2_add(sum[0], sum[1]));
-            l += total2.x + total2.y;
+            const float2 both = f2_unpack(f2_add(sum[0], sum[1]));
+            l += both.x + both.y;
             tc_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_ready[x]);
         }
-        ok = ok && __all_sync(0xffffffffu, mbar_wait_bounded(&o_done[x], kApart ? (uint32_t)(n_tiles - 1) & 1u : 0u, nullptr));
+        ok = ok && wait(&o_done[x], kApart ? n_tiles - 1 : 0);
         if (!ok) s_fail = 1;
         tc_fence_after();
         const bool mine = token < t_end;
         T* dst = reinterpret_cast<T*>(a.out) + (long long)token * a.out_stride + (long long)head * a.head_size;
         const float inv = ok ? __fdiv_rn(1.f, l) : NAN;
 #pragma unroll
-        for (int c = 0; c < HS / 32; ++c) {
+        for (int c = 0; c < HS; c += 32) {
             uint32_t o[32];
-            tc_ld32_async(to + c * 32, o);
+            tc_ld32_async(tm + Shape::kO + c, o);
             tc_wait_ld();
             pin16(o);
             pin16(o + 16);
-            if (mine)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    if (c * 32 + i * 8 < a.head_size) {
-                        uint32_t w[4];
+            for (int i = 0; i < 32; i += 8)
+                if (mine && c + i < a.head_size) {
+                    uint32_t w[4];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) w[j] = pack2<T>(__uint_as_float(o[i * 8 + 2 * j]) * inv, __uint_as_float(o[i * 8 + 2 * j + 1]) * inv);
-                        *reinterpret_cast<uint4*>(dst + c * 32 + i * 8) = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    for (int j = 0; j < 4; ++j) w[j] = pack2<T>(__uint_as_float(o[i + 2 * j]) * inv, __uint_as_float(o[i + 2 * j + 1]) * inv);
+                    *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
         }
         if (ok && mine && *reinterpret_cast<volatile int*>(&s_odd)) {  // (set before the last product)
             for (int it = 0; it < n_tiles; ++it) {
@@ -496,7 +489,7 @@ static __global__ void __launch_bounds__(kPaThreads, 1) prompt_attention_kernel(
         while (clock64() - c0 < (1 << 17)) __nanosleep(1000);
     }
     __syncthreads();
-    if (warp == kPaMmaWarp) tc_dealloc(tmem, 512);
+    if (warp == Shape::kMmaWarp) tc_dealloc(tmem, Shape::kColumns);
 }
 
 }  // namespace lpp
