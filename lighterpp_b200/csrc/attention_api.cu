@@ -311,13 +311,15 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
     a.keep = keep;
     a.recent = recent;
     a.row_bytes = row;
-    lpp_status st = launch_op(kv4_select_kernel, dim3(n_kv_heads, batch), kKv4EvictThreads, 0, S(stream), a);
-    if (st != LPP_OK) return launched("lpp_op_kv4_evict: the launch failed", st);
-    const int vec = row % 16 == 0 ? 16 : row % 8 == 0 ? 8 : 4;
-    const long long per_head = ((long long)keep * (row / vec) + 255) / 256;
-    const dim3 grid((unsigned)std::min<long long>(per_head, std::max<long long>(1, 8ll * sms / (long long)heads)), n_kv_heads, batch);
-    st = vec == 16 ? launch_behind(kv4_move_kernel<uint4>, grid, 256, 0, S(stream), a)
-                   : vec == 8 ? launch_behind(kv4_move_kernel<uint2>, grid, 256, 0, S(stream), a) : launch_behind(kv4_move_kernel<uint32_t>, grid, 256, 0, S(stream), a);
+    // CTAs of a head: up to eight (a portable cluster), while they all run at once and have some hundred rows each
+    a.cluster = 1;
+    while (a.cluster < kKv4EvictCluster && 2ll * a.cluster * (long long)heads <= sms && capacity >= 1024ll * a.cluster) a.cluster *= 2;
+    const dim3 grid(a.cluster, n_kv_heads, batch);
+    auto go = [&](auto* t) {
+        using V = std::remove_pointer_t<decltype(t)>;
+        return launch_op_cluster(kv4_evict_kernel<V>, grid, kKv4EvictThreads, 0, a.cluster, false, S(stream), a);
+    };
+    const lpp_status st = row % 16 == 0 ? go((uint4*)nullptr) : row % 8 == 0 ? go((uint2*)nullptr) : go((uint32_t*)nullptr);
     return launched("lpp_op_kv4_evict: the launch failed", st);
 }
 

@@ -888,9 +888,13 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // ------------------------------------------------------------------ eviction
 //
 // Keeps the `recent` last rows of every head and, of the rows before them, those with the largest sums (the lowest position first among
-// equals; a NaN counts as -infinity), in their order.  One CTA per head finds the smallest sum that stays, digit by digit, and writes
-// the list of kept rows; a second kernel moves them.
-constexpr int kKv4EvictThreads = 1024;
+// equals; a NaN counts as -infinity), in their order.  A cluster of CTAs takes a head, every CTA a run of its rows: the smallest sum that
+// stays is found digit by digit (histograms of 8 bits of the sums' order, every CTA adding up all of the cluster's through distributed
+// shared memory), then every CTA knows where its kept rows begin in the new cache, lists them and moves them.
+// Bound by the rows' bytes where they are many, by the six meetings of the cluster where they are few.  (Digits of 11 bits added up by
+// remote atomics in one CTA: three passes of 3 - 8 us each instead of four of under 1 us.)
+constexpr int kKv4EvictThreads = 1024, kKv4EvictCluster = 8;
+constexpr int kKv4EvictKeep = 4;  // rows of a thread whose ranks stay in registers
 
 struct Kv4EvictArgs {
     const unsigned char *k, *v;
@@ -900,7 +904,7 @@ struct Kv4EvictArgs {
     int *kept, *lens_out;
     const int* lens;
     long long capacity, capacity_out;
-    int kv_heads, keep, recent, row_bytes;
+    int kv_heads, keep, recent, row_bytes, cluster;
 };
 
 // Order of the sums as unsigned integers
@@ -908,100 +912,171 @@ __device__ __forceinline__ uint32_t kv4_rank(float x) {
     const uint32_t u = x != x ? 0xff800000u : __float_as_uint(x + 0.f);  // (-0 becomes 0)
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
-
-static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_select_kernel(const Kv4EvictArgs a) {
-    __shared__ uint32_t hist[2048], warp_sums[32], s_digit, s_left;
-    op_begin();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.x, b = blockIdx.y;
-    const int len = (int)max(0ll, min((long long)a.lens[b], a.capacity)), stay = min(len, a.keep), old = max(0, len - a.recent);
-    const long long head = (long long)b * a.kv_heads + kvh;
-    const float* sums = a.sums + head * a.capacity;
-    int* kept = a.kept + head * a.keep;
-    if (kvh == 0 && tid == 0) a.lens_out[b] = stay;
-    const uint32_t choose = (uint32_t)max(0, stay - (len - old));  // of the `old` first rows
-    // the choose-th largest rank: digits of 11, 11 and 10 bits
-    uint32_t prefix = 0, mask = 0, left = choose;
-    if (choose > 0 && choose < (uint32_t)old) {
-        for (int pass = 0; pass < 3; ++pass) {
-            const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
-            const uint32_t digits = pass == 2 ? 1023u : 2047u;
-            for (int i = tid; i < 2048; i += kKv4EvictThreads) hist[i] = 0;
-            __syncthreads();
-            for (int i = tid; i < old; i += kKv4EvictThreads) {
-                const uint32_t r = kv4_rank(sums[i]);
-                if ((r & mask) == prefix) atomicAdd(&hist[(r >> shift) & digits], 1u);
-            }
-            __syncthreads();
-            // digits from the top, two a thread
-            const uint32_t c0 = hist[2047 - 2 * tid], c1 = hist[2046 - 2 * tid];
-            uint32_t x = c0 + c1;
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-                if (lane >= d) x += y;
-            }
-            if (lane == 31) warp_sums[warp] = x;
-            __syncthreads();
-            for (int w = 0; w < warp; ++w) x += warp_sums[w];
-            const uint32_t before = x - c0 - c1;
-            if (before < left && left <= x) {
-                const bool first = left <= before + c0;
-                s_digit = (uint32_t)(first ? 2047 - 2 * tid : 2046 - 2 * tid);
-                s_left = left - before - (first ? 0u : c0);
-            }
-            __syncthreads();
-            prefix |= s_digit << shift;
-            mask |= digits << shift;
-            left = s_left;
-        }
-    }
-    // rows with a larger rank stay, of those that equal it the first `left`
-    const bool all = choose >= (uint32_t)old;
-    uint32_t n = 0, equal = 0;  // rows kept and equals seen so far
-    for (int i0 = 0; i0 < old; i0 += kKv4EvictThreads) {
-        const int i = i0 + tid;
-        const uint32_t r = i < old ? kv4_rank(sums[i]) : 0u;
-        const bool same = i < old && choose > 0 && !all && r == prefix, more = i < old && choose > 0 && (all || r > prefix);
-        uint32_t x = (same ? 1u << 16 : 0u) + (more ? 1u : 0u);
-        const uint32_t own = x;
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-            if (lane >= d) x += y;
-        }
-        __syncthreads();
-        if (lane == 31) warp_sums[warp] = x;
-        __syncthreads();
-        uint32_t total = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) x += warp_sums[w];
-            total += warp_sums[w];
-        }
-        x -= own;
-        const uint32_t eq = equal + (x >> 16);  // equals before this row
-        const uint32_t at = n + (x & 0xffffu) + (all ? 0u : min(eq, left) - min(equal, left));
-        if (more || (same && eq < left)) kept[at] = i;
-        n += (total & 0xffffu) + (all ? 0u : min(equal + (total >> 16), left) - min(equal, left));
-        equal += total >> 16;
-    }
-    for (int i = tid; i < len - old && i < stay; i += kKv4EvictThreads) kept[stay - (len - old) + i] = old + i;
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t cluster_map(uint32_t smem_addr, uint32_t cta) {  // the same place in another CTA of the cluster
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_addr), "r"(cta));
+    return r;
+}
+__device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
+    uint32_t r;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(r) : "r"(a) : "memory");
+    return r;
 }
 
 // V: bytes a thread moves at once (16, 8 or 4, by the row's size)
 template <typename V>
-static __global__ void __launch_bounds__(256) kv4_move_kernel(const Kv4EvictArgs a) {
-    op_begin();
-    const int kvh = blockIdx.y, b = blockIdx.z, units = a.row_bytes / (int)sizeof(V);
+static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(const Kv4EvictArgs a) {
+    __shared__ uint32_t hist[4][256], parts[kKv4EvictThreads / 256][256];  // hist: a pass each
+    __shared__ uint32_t counts[kKv4EvictCluster][2], warp_sums[32], s_digit, s_left;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x % a.cluster, kvh = blockIdx.y, b = blockIdx.z;
+    const int len = (int)max(0ll, min((long long)a.lens[b], a.capacity)), stay = min(len, a.keep), old = max(0, len - a.recent);
     const long long head = (long long)b * a.kv_heads + kvh;
-    const int stay = (int)max(0ll, min(min((long long)a.lens[b], a.capacity), (long long)a.keep));
-    const int* kept = a.kept + head * a.keep;
-    const V *k = reinterpret_cast<const V*>(a.k + head * a.capacity * a.row_bytes), *v = reinterpret_cast<const V*>(a.v + head * a.capacity * a.row_bytes);
-    V *ko = reinterpret_cast<V*>(a.k_out + head * a.capacity_out * a.row_bytes), *vo = reinterpret_cast<V*>(a.v_out + head * a.capacity_out * a.row_bytes);
-    const long long step = (long long)gridDim.x * blockDim.x, total = (long long)stay * units;
-    for (long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += step) {
-        const int row = (int)(i / units), unit = (int)(i - (long long)row * units), from = kept[row];
-        ko[i] = k[(long long)from * units + unit];
-        vo[i] = v[(long long)from * units + unit];
-        if (unit == 0) a.sums_out[head * a.capacity_out + row] = a.sums[head * a.capacity + from];
+    const float* sums = a.sums + head * a.capacity;
+    int* kept = a.kept + head * a.keep;
+    if (cta == 0 && kvh == 0 && tid == 0) a.lens_out[b] = stay;
+    const int each = ((len + a.cluster - 1) / a.cluster + 31) & ~31, row0 = min(len, cta * each), row1 = min(len, row0 + each);
+    uint32_t rank[kKv4EvictKeep];
+#pragma unroll
+    for (int j = 0; j < kKv4EvictKeep; ++j) {
+        const int i = row0 + tid + j * kKv4EvictThreads;
+        rank[j] = i < min(row1, old) ? kv4_rank(sums[i]) : 0u;
     }
+    hist[tid >> 8][tid & 255] = 0;
+    __syncthreads();
+    // the choose-th largest rank of the `old` first rows
+    const uint32_t choose = (uint32_t)max(0, stay - (len - old));
+    const bool every = choose >= (uint32_t)old, none = choose == 0;
+    uint32_t prefix = 0, mask = 0, left = choose;
+    if (!every && !none) {  // (the same for the whole cluster)
+        const int end = min(row1, old);
+#pragma unroll 1
+        for (int pass = 0; pass < 4; ++pass) {
+            const int shift = 24 - 8 * pass;
+#pragma unroll
+            for (int j = 0; j < kKv4EvictKeep; ++j)
+                if (row0 + tid + j * kKv4EvictThreads < end && (rank[j] & mask) == prefix) atomicAdd(&hist[pass][rank[j] >> shift & 255u], 1u);
+            for (int i = row0 + tid + kKv4EvictKeep * kKv4EvictThreads; i < end; i += kKv4EvictThreads) {
+                const uint32_t r = kv4_rank(sums[i]);
+                if ((r & mask) == prefix) atomicAdd(&hist[pass][r >> shift & 255u], 1u);
+            }
+            cluster_barrier();  // every CTA has started, and counted
+            const int digit = 255 - (tid & 255);  // from the top
+            uint32_t x = 0;
+            for (int c = tid >> 8; c < a.cluster; c += kKv4EvictThreads / 256) x += kv4_cluster_load(cluster_map(smem_u32(&hist[pass][digit]), c));
+            parts[tid >> 8][tid & 255] = x;
+            __syncthreads();
+            uint32_t own = 0;
+            if (tid < 256) {
+                own = parts[0][tid] + parts[1][tid] + parts[2][tid] + parts[3][tid];
+                x = own;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
+                    if (lane >= d) x += y;
+                }
+                if (lane == 31) warp_sums[warp] = x;
+            }
+            __syncthreads();
+            if (tid < 256) {
+                x += __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0u);
+                if (x - own < left && left <= x) {
+                    s_digit = (uint32_t)digit;
+                    s_left = left - (x - own);
+                }
+            }
+            __syncthreads();
+            prefix |= s_digit << shift;
+            mask |= 255u << shift;
+            left = s_left;
+        }
+    } else {
+        cluster_barrier();  // every CTA has started
+    }
+    // rows with a larger rank stay, and the recent ones; of those that equal it the first `left`
+    auto judge = [&](int i, uint32_t r, bool& more, bool& same) {
+        const bool is_old = i < old;
+        more = i < row1 && (!is_old || every || (!none && r > prefix));
+        same = i < row1 && is_old && !every && !none && r == prefix;
+    };
+    auto rank_of = [&](int i) { return i < min(row1, old) ? kv4_rank(sums[i]) : 0u; };
+    uint32_t n_more = 0, n_same = 0;
+    auto count = [&](int i, uint32_t r) {
+        bool more, same;
+        judge(i, r, more, same);
+        n_more += __popc(__ballot_sync(0xffffffffu, more));
+        n_same += __popc(__ballot_sync(0xffffffffu, same));
+    };
+#pragma unroll
+    for (int j = 0; j < kKv4EvictKeep; ++j) count(row0 + tid + j * kKv4EvictThreads, rank[j]);
+    for (int i0 = row0 + kKv4EvictKeep * kKv4EvictThreads; i0 < row1; i0 += kKv4EvictThreads) count(i0 + tid, rank_of(i0 + tid));
+    if (lane == 0) parts[0][warp] = n_more, parts[0][32 + warp] = n_same;
+    __syncthreads();
+    if (warp == 0) {
+        n_more = __reduce_add_sync(0xffffffffu, parts[0][lane]);
+        n_same = __reduce_add_sync(0xffffffffu, parts[0][32 + lane]);
+        if (lane < a.cluster) {  // to every CTA of the cluster
+            const uint32_t to = cluster_map(smem_u32(&counts[cta][0]), lane);
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(n_more) : "memory");
+            asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4), "r"(n_same) : "memory");
+        }
+    }
+    cluster_barrier();  // (also the last time that another CTA's shared memory is touched)
+    uint32_t at = 0, equal = 0;
+    for (int c = 0; c < cta; ++c) at += counts[c][0], equal += counts[c][1];
+    at += min(equal, left);
+    const uint32_t begin = at;
+    auto place = [&](int i, uint32_t r) {
+        bool more, same;
+        judge(i, r, more, same);
+        const uint32_t bm = __ballot_sync(0xffffffffu, more), bs = __ballot_sync(0xffffffffu, same), below = (1u << lane) - 1u;
+        __syncthreads();
+        if (lane == 0) warp_sums[warp] = (uint32_t)__popc(bm) | (uint32_t)__popc(bs) << 16;
+        __syncthreads();
+        const uint32_t w = warp_sums[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u), total = __reduce_add_sync(0xffffffffu, w);
+        const uint32_t eq = equal + (before >> 16) + __popc(bs & below);  // equals before this row
+        const uint32_t to = at + (before & 0xffffu) + __popc(bm & below) + min(eq, left) - min(equal, left);
+        if (more || (same && eq < left)) kept[to] = i;
+        at += (total & 0xffffu) + min(equal + (total >> 16), left) - min(equal, left);
+        equal += total >> 16;
+    };
+#pragma unroll
+    for (int j = 0; j < kKv4EvictKeep; ++j)
+        if (row0 + j * kKv4EvictThreads < row1) place(row0 + tid + j * kKv4EvictThreads, rank[j]);  // (the same for the whole CTA)
+    for (int i0 = row0 + kKv4EvictKeep * kKv4EvictThreads; i0 < row1; i0 += kKv4EvictThreads) place(i0 + tid, rank_of(i0 + tid));
+    __syncthreads();
+    // ---- the rows
+    const int units = a.row_bytes / (int)sizeof(V), rows = (int)(at - begin);
+    const V *k = reinterpret_cast<const V*>(a.k + head * a.capacity * a.row_bytes), *v = reinterpret_cast<const V*>(a.v + head * a.capacity * a.row_bytes);
+    V *ko = reinterpret_cast<V*>(a.k_out + (head * a.capacity_out + begin) * a.row_bytes), *vo = reinterpret_cast<V*>(a.v_out + (head * a.capacity_out + begin) * a.row_bytes);
+    const int* list = kept + begin;
+    constexpr int kAhead = 4;
+    for (int i0 = tid; i0 < rows * units; i0 += kAhead * kKv4EvictThreads) {
+        V x[kAhead], y[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + j * kKv4EvictThreads, row = i / units;
+            if (i < rows * units) {
+                const long long from = (long long)list[row] * units + (i - row * units);
+                x[j] = k[from];
+                y[j] = v[from];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            const int i = i0 + j * kKv4EvictThreads;
+            if (i < rows * units) {
+                ko[i] = x[j];
+                vo[i] = y[j];
+            }
+        }
+    }
+    for (int i = tid; i < rows; i += kKv4EvictThreads) a.sums_out[head * a.capacity_out + begin + i] = sums[list[i]];
 }
 
 }  // namespace lpp
