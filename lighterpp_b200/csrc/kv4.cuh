@@ -893,8 +893,9 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // shared memory), then every CTA knows where its kept rows begin in the new cache, lists them and moves them.
 // Bound by the rows' bytes where they are many, by the six meetings of the cluster where they are few.  (Digits of 11 bits added up by
 // remote atomics in one CTA: three passes of 3 - 8 us each instead of four of under 1 us.)
-constexpr int kKv4EvictThreads = 1024, kKv4EvictCluster = 8;
-constexpr int kKv4EvictKeep = 4;  // rows of a thread whose ranks stay in registers
+// 512 threads: two CTAs fit an SM (of 1024, sixteen clusters of eight did not fit the GPU at once, and the last ran alone).
+constexpr int kKv4EvictThreads = 512, kKv4EvictCluster = 8;
+constexpr int kKv4EvictKeep = 8;  // rows of a thread whose ranks stay in registers
 
 struct Kv4EvictArgs {
     const unsigned char *k, *v;
@@ -929,9 +930,9 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
 
 // V: bytes a thread moves at once (16, 8 or 4, by the row's size)
 template <typename V>
-static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(const Kv4EvictArgs a) {
-    __shared__ uint32_t hist[4][256], parts[kKv4EvictThreads / 256][256];  // hist: a pass each
-    __shared__ uint32_t counts[kKv4EvictCluster][2], warp_sums[32], s_digit, s_left;
+static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_evict_kernel(const Kv4EvictArgs a) {
+    __shared__ uint32_t hist[4][256], parts[2][256];  // hist: a pass each
+    __shared__ uint32_t counts[kKv4EvictCluster][2], warp_sums[32], s_digit, s_left, s_all;
     pdl_wait();
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, cta = blockIdx.x % a.cluster, kvh = blockIdx.y, b = blockIdx.z;
@@ -947,7 +948,8 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
         const int i = row0 + tid + j * kKv4EvictThreads;
         rank[j] = i < min(row1, old) ? kv4_rank(sums[i]) : 0u;
     }
-    hist[tid >> 8][tid & 255] = 0;
+    hist[tid >> 8][tid & 255] = hist[2 + (tid >> 8)][tid & 255] = 0;
+    if (tid < 32) warp_sums[tid] = 0;
     __syncthreads();
     // the choose-th largest rank of the `old` first rows
     const uint32_t choose = (uint32_t)max(0, stay - (len - old));
@@ -967,18 +969,24 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
             }
             cluster_barrier();  // every CTA has started, and counted
             const int digit = 255 - (tid & 255);  // from the top
-            uint32_t x = 0;
-            for (int c = tid >> 8; c < a.cluster; c += kKv4EvictThreads / 256) x += kv4_cluster_load(cluster_map(smem_u32(&hist[pass][digit]), c));
+            uint32_t y[kKv4EvictCluster / 2], x = 0;
+#pragma unroll
+            for (int j = 0; j < kKv4EvictCluster / 2; ++j) {
+                const int c = (tid >> 8) + 2 * j;
+                y[j] = c < a.cluster ? kv4_cluster_load(cluster_map(smem_u32(&hist[pass][digit]), c)) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < kKv4EvictCluster / 2; ++j) x += y[j];
             parts[tid >> 8][tid & 255] = x;
             __syncthreads();
             uint32_t own = 0;
             if (tid < 256) {
-                own = parts[0][tid] + parts[1][tid] + parts[2][tid] + parts[3][tid];
+                own = parts[0][tid] + parts[1][tid];
                 x = own;
 #pragma unroll
                 for (int d = 1; d < 32; d <<= 1) {
-                    const uint32_t y = __shfl_up_sync(0xffffffffu, x, d);
-                    if (lane >= d) x += y;
+                    const uint32_t z = __shfl_up_sync(0xffffffffu, x, d);
+                    if (lane >= d) x += z;
                 }
                 if (lane == 31) warp_sums[warp] = x;
             }
@@ -988,12 +996,14 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
                 if (x - own < left && left <= x) {
                     s_digit = (uint32_t)digit;
                     s_left = left - (x - own);
+                    s_all = s_left == own ? 1u : 0u;
                 }
             }
             __syncthreads();
             prefix |= s_digit << shift;
             mask |= 255u << shift;
             left = s_left;
+            if (s_all) break;  // all of these stay: further digits tell nothing apart
         }
     } else {
         cluster_barrier();  // every CTA has started
@@ -1001,8 +1011,8 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
     // rows with a larger rank stay, and the recent ones; of those that equal it the first `left`
     auto judge = [&](int i, uint32_t r, bool& more, bool& same) {
         const bool is_old = i < old;
-        more = i < row1 && (!is_old || every || (!none && r > prefix));
-        same = i < row1 && is_old && !every && !none && r == prefix;
+        more = i < row1 && (!is_old || every || (!none && (r & mask) > prefix));
+        same = i < row1 && is_old && !every && !none && (r & mask) == prefix;
     };
     auto rank_of = [&](int i) { return i < min(row1, old) ? kv4_rank(sums[i]) : 0u; };
     uint32_t n_more = 0, n_same = 0;
@@ -1015,11 +1025,12 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
 #pragma unroll
     for (int j = 0; j < kKv4EvictKeep; ++j) count(row0 + tid + j * kKv4EvictThreads, rank[j]);
     for (int i0 = row0 + kKv4EvictKeep * kKv4EvictThreads; i0 < row1; i0 += kKv4EvictThreads) count(i0 + tid, rank_of(i0 + tid));
+    constexpr int kWarps = kKv4EvictThreads / 32;
     if (lane == 0) parts[0][warp] = n_more, parts[0][32 + warp] = n_same;
     __syncthreads();
     if (warp == 0) {
-        n_more = __reduce_add_sync(0xffffffffu, parts[0][lane]);
-        n_same = __reduce_add_sync(0xffffffffu, parts[0][32 + lane]);
+        n_more = __reduce_add_sync(0xffffffffu, lane < kWarps ? parts[0][lane] : 0u);
+        n_same = __reduce_add_sync(0xffffffffu, lane < kWarps ? parts[0][32 + lane] : 0u);
         if (lane < a.cluster) {  // to every CTA of the cluster
             const uint32_t to = cluster_map(smem_u32(&counts[cta][0]), lane);
             asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to), "r"(n_more) : "memory");
@@ -1038,7 +1049,7 @@ static __global__ void __launch_bounds__(kKv4EvictThreads) kv4_evict_kernel(cons
         __syncthreads();
         if (lane == 0) warp_sums[warp] = (uint32_t)__popc(bm) | (uint32_t)__popc(bs) << 16;
         __syncthreads();
-        const uint32_t w = warp_sums[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u), total = __reduce_add_sync(0xffffffffu, w);
+        const uint32_t w = lane < kWarps ? warp_sums[lane] : 0u, before = __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u), total = __reduce_add_sync(0xffffffffu, w);
         const uint32_t eq = equal + (before >> 16) + __popc(bs & below);  // equals before this row
         const uint32_t to = at + (before & 0xffffu) + __popc(bm & below) + min(eq, left) - min(equal, left);
         if (more || (same && eq < left)) kept[to] = i;
