@@ -314,12 +314,17 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
     // CTAs of a head: up to eight (a portable cluster), while they all run at once and have some hundred rows each
     a.cluster = 1;
     while (a.cluster < kKv4EvictCluster && 2ll * a.cluster * (long long)heads <= sms && capacity >= 1024ll * a.cluster) a.cluster *= 2;
-    const dim3 grid(a.cluster, n_kv_heads, batch);
-    auto go = [&](auto* t) {
-        using V = std::remove_pointer_t<decltype(t)>;
-        return launch_op_cluster(kv4_evict_kernel<V>, grid, kKv4EvictThreads, 0, a.cluster, false, S(stream), a);
-    };
-    const lpp_status st = row % 16 == 0 ? go((uint4*)nullptr) : row % 8 == 0 ? go((uint2*)nullptr) : go((uint32_t*)nullptr);
+    lpp_status st = launch_op_cluster(kv4_select_kernel, dim3(a.cluster, n_kv_heads, batch), kKv4EvictThreads, 0, a.cluster, false, S(stream), a);
+    if (st != LPP_OK) return launched("lpp_op_kv4_evict: the launch failed", st);
+    const dim3 grid(blocks(std::min<int64_t>(keep, capacity), kKv4MoveRows), n_kv_heads, batch);
+    auto move = [&](auto kernel) { return launch_behind(kernel, grid, kKv4MoveRows, 0, S(stream), a); };
+    switch (row / 20) {  // groups of a row
+        case 1: st = move(kv4_move_kernel<uint32_t, 5>); break;
+        case 2: st = move(kv4_move_kernel<uint2, 5>); break;
+        case 3: st = move(kv4_move_kernel<uint32_t, 15>); break;
+        case 4: st = move(kv4_move_kernel<uint4, 5>); break;
+        default: st = move(kv4_move_kernel<uint4, 10>);
+    }
     return launched("lpp_op_kv4_evict: the launch failed", st);
 }
 

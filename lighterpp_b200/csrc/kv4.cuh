@@ -890,9 +890,10 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // Keeps the `recent` last rows of every head and, of the rows before them, those with the largest sums (the lowest position first among
 // equals; a NaN counts as -infinity), in their order.  A cluster of CTAs takes a head, every CTA a run of its rows: the smallest sum that
 // stays is found digit by digit (histograms of 8 bits of the sums' order, every CTA adding up all of the cluster's through distributed
-// shared memory), then every CTA knows where its kept rows begin in the new cache, lists them and moves them.
-// Bound by the rows' bytes where they are many, by the six meetings of the cluster where they are few.  (Digits of 11 bits added up by
-// remote atomics in one CTA: three passes of 3 - 8 us each instead of four of under 1 us.)
+// shared memory), then every CTA knows where its kept rows begin in the new cache and lists them.  A second kernel, of many small CTAs,
+// moves them: bound by the rows' bytes where they are many, by the meetings of the cluster where they are few.  (Digits of 11 bits added
+// up by remote atomics in one CTA: passes of 3 - 8 us each instead of 1.4.  Rows moved by the cluster that lists them, two sequences of
+// 32768 and 20011 positions to 12000: 30 us, its SMs being too few for the bandwidth; now NN.)
 // 512 threads: two CTAs fit an SM (of 1024, sixteen clusters of eight did not fit the GPU at once, and the last ran alone).
 constexpr int kKv4EvictThreads = 512, kKv4EvictCluster = 8;
 constexpr int kKv4EvictKeep = 8;  // rows of a thread whose ranks stay in registers
@@ -928,9 +929,7 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
     return r;
 }
 
-// V: bytes a thread moves at once (16, 8 or 4, by the row's size)
-template <typename V>
-static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_evict_kernel(const Kv4EvictArgs a) {
+static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_select_kernel(const Kv4EvictArgs a) {
     __shared__ uint32_t hist[4][256], parts[2][256];  // hist: a pass each
     __shared__ uint32_t counts[kKv4EvictCluster][2], warp_sums[32], s_digit, s_left, s_all;
     pdl_wait();
@@ -1041,7 +1040,6 @@ static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_evict_kernel(c
     uint32_t at = 0, equal = 0;
     for (int c = 0; c < cta; ++c) at += counts[c][0], equal += counts[c][1];
     at += min(equal, left);
-    const uint32_t begin = at;
     auto place = [&](int i, uint32_t r) {
         bool more, same;
         judge(i, r, more, same);
@@ -1060,34 +1058,45 @@ static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_evict_kernel(c
     for (int j = 0; j < kKv4EvictKeep; ++j)
         if (row0 + j * kKv4EvictThreads < row1) place(row0 + tid + j * kKv4EvictThreads, rank[j]);  // (the same for the whole CTA)
     for (int i0 = row0 + kKv4EvictKeep * kKv4EvictThreads; i0 < row1; i0 += kKv4EvictThreads) place(i0 + tid, rank_of(i0 + tid));
-    __syncthreads();
-    // ---- the rows
-    const int units = a.row_bytes / (int)sizeof(V), rows = (int)(at - begin);
-    const V *k = reinterpret_cast<const V*>(a.k + head * a.capacity * a.row_bytes), *v = reinterpret_cast<const V*>(a.v + head * a.capacity * a.row_bytes);
-    V *ko = reinterpret_cast<V*>(a.k_out + (head * a.capacity_out + begin) * a.row_bytes), *vo = reinterpret_cast<V*>(a.v_out + (head * a.capacity_out + begin) * a.row_bytes);
-    const int* list = kept + begin;
-    constexpr int kAhead = 4;
-    for (int i0 = tid; i0 < rows * units; i0 += kAhead * kKv4EvictThreads) {
+}
+
+// V: bytes a thread moves at once (16, 8 or 4, by the row's size), UNITS of them a row.  A CTA takes 256 rows, a thread UNITS pieces of the
+// keys and of the values, all on their way at once.  Grid (blocks of rows, kv_heads, batch).
+constexpr int kKv4MoveRows = 256;
+template <typename V, int UNITS>
+static __global__ void __launch_bounds__(kKv4MoveRows) kv4_move_kernel(const Kv4EvictArgs a) {
+    pdl_launch_dependents();
+    const int tid = threadIdx.x, kvh = blockIdx.y, b = blockIdx.z, row0 = blockIdx.x * kKv4MoveRows;
+    const long long head = (long long)b * a.kv_heads + kvh;
+    const int rows = (int)max(0ll, min(min((long long)a.lens[b], a.capacity), (long long)a.keep)) - row0;
+    const int* kept = a.kept + head * a.keep + row0;
+    const V *k = reinterpret_cast<const V*>(a.k) + head * a.capacity * UNITS, *v = reinterpret_cast<const V*>(a.v) + head * a.capacity * UNITS;
+    V *ko = reinterpret_cast<V*>(a.k_out) + (head * a.capacity_out + row0) * UNITS, *vo = reinterpret_cast<V*>(a.v_out) + (head * a.capacity_out + row0) * UNITS;
+    constexpr int kAhead = UNITS > 5 ? 5 : UNITS;
+    pdl_wait();
+    if (tid < rows) a.sums_out[head * a.capacity_out + row0 + tid] = a.sums[head * a.capacity + kept[tid]];
+#pragma unroll
+    for (int j0 = 0; j0 < UNITS; j0 += kAhead) {
+        long long from[kAhead];
         V x[kAhead], y[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
-            const int i = i0 + j * kKv4EvictThreads, row = i / units;
-            if (i < rows * units) {
-                const long long from = (long long)list[row] * units + (i - row * units);
-                x[j] = k[from];
-                y[j] = v[from];
-            }
+            const int i = tid + (j0 + j) * kKv4MoveRows, row = i / UNITS;
+            from[j] = row < rows ? (long long)kept[row] * UNITS + (i - row * UNITS) : -1;
         }
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
-            const int i = i0 + j * kKv4EvictThreads;
-            if (i < rows * units) {
-                ko[i] = x[j];
-                vo[i] = y[j];
+        for (int j = 0; j < kAhead; ++j)
+            if (from[j] >= 0) {
+                x[j] = k[from[j]];
+                y[j] = v[from[j]];
             }
-        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            if (from[j] >= 0) {
+                ko[tid + (j0 + j) * kKv4MoveRows] = x[j];
+                vo[tid + (j0 + j) * kKv4MoveRows] = y[j];
+            }
     }
-    for (int i = tid; i < rows; i += kKv4EvictThreads) a.sums_out[head * a.capacity_out + begin + i] = sums[list[i]];
 }
 
 }  // namespace lpp
