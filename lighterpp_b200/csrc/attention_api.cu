@@ -78,18 +78,19 @@ lpp_status rows_op(const char* name, const void* k, const void* v, const int64_t
                    int head_size, int64_t k_stride, int64_t v_stride, int dtype, Launch launch) {
     if (const char* f = cache_fault(kc, vc, batch, kv_heads, capacity, head_size)) return refuse(f);
     if (!is_dtype(dtype)) return refuse("4-bit cache: rows are F32, F16 or BF16");
-    if (n < 0 || (long long)n * kv_heads > 0x7fffffffll) return refuse("4-bit cache: too many rows");
+    if (n < 0 || (long long)n * kv_heads > (1 << 27)) return refuse("4-bit cache: too many rows");
     if (n == 0) return LPP_OK;
     if (!k || !v || !slots) return refuse("4-bit cache: null pointer");
     const int element = dtype == LPP_F32 ? 4 : 2;
     if (((uintptr_t)k | (uintptr_t)v) & (element - 1) || (uintptr_t)slots & 7) return refuse("4-bit cache: a pointer is not aligned to its type");
     const int64_t dense = (int64_t)kv_heads * head_size;
     if (k_stride < dense || v_stride < dense) return refuse("4-bit cache: a token's rows overlap the next one's");
-    // eight values at once where every row starts on a 16-byte boundary
+    // 16 bytes at once where every row starts on such a boundary
     const bool wide = head_size % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) && k_stride * element % 16 == 0 && v_stride * element % 16 == 0;
-    Kv4Cache c = {(unsigned char*)kc, (unsigned char*)vc, capacity, (long long)batch * capacity, kv_heads};
+    auto by = [](uint32_t d) { return Kv4Div{d, d > 1 ? (uint32_t)((1ull << 32) / d) : 0u}; };
+    Kv4Cache c = {(unsigned char*)kc, (unsigned char*)vc, capacity, (long long)batch * capacity, kv_heads, by((uint32_t)kv_heads), by((uint32_t)capacity)};
     const int groups = kv4_held_groups(head_size), rows = n * kv_heads;
-    const long long ctas = ((long long)rows * 4 * groups + kKv4RowThreads - 1) / kKv4RowThreads;
+    const long long ctas = ((long long)rows * 2 * groups + kKv4RowThreads - 1) / kKv4RowThreads;
     return launched(name, launch(c, groups, dim3((unsigned)ctas, 2), rows, wide));
 }
 

@@ -17,31 +17,49 @@ constexpr int kKv4Group = 32;
 __host__ __device__ constexpr int kv4_groups(int head_size) { return (head_size + kKv4Group - 1) / kKv4Group; }
 __host__ __device__ constexpr int kv4_row_bytes(int groups) { return groups * (kKv4Group / 2 + 4); }
 
+// n / d for 32-bit numbers by the reciprocal floor(2^32 / d), which gives the quotient or one less
+struct Kv4Div {
+    uint32_t d, inv;
+    __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+        const uint32_t q = d == 1 ? n : __umulhi(n, inv);
+        return q + (n - q * d >= d ? 1u : 0u);
+    }
+};
 // The caches of one layer: [batch][kv_heads][capacity] rows.
 struct Kv4Cache {
     unsigned char *k, *v;
     long long capacity, slots;  // slots: batch * capacity
     int kv_heads;
+    Kv4Div by_heads, by_capacity;  // (the second where there are fewer than 2^32 slots)
+    __device__ __forceinline__ long long row(long long slot, int head) const {
+        const long long b = slots >> 32 ? slot / capacity : (long long)by_capacity((uint32_t)slot);
+        return (b * kv_heads + head) * capacity + (slot - b * capacity);
+    }
 };
 
 // ------------------------------------------------------------------ writing and reading rows
 //
-// Four threads a group, eight dimensions (one 32-bit word of codes) each; bound by the bytes of the values.
+// Two threads a group, sixteen dimensions (two 32-bit words of codes) each.  Bound by the instructions on the way in (about 20 an element; eight
+// elements a thread, conversions by the conversion unit and 64-bit divisions: 34 us where this takes NN), by the bytes of the values on
+// the way out.
 
-constexpr int kKv4RowThreads = 256;
+constexpr int kKv4RowThreads = 256, kKv4Each = 16;  // kKv4Each: dimensions of a thread
 
-// Eight consecutive values; `n` of them exist.
+// Sixteen consecutive values; `n` of them exist.
 template <typename T>
-__device__ __forceinline__ void kv4_load8(const T* p, int n, bool wide, float (&x)[8]) {
-    if (wide && n >= 8) {
+__device__ __forceinline__ void kv4_load(const T* p, int n, bool wide, float (&x)[kKv4Each]) {
+    if (wide && n >= kKv4Each) {
         if constexpr (sizeof(T) == 4) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
-            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
-        } else {
-            const uint4 a = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+            float4 a[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < 4; ++i) a[i] = reinterpret_cast<const float4*>(p)[i];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[4 * i] = a[i].x, x[4 * i + 1] = a[i].y, x[4 * i + 2] = a[i].z, x[4 * i + 3] = a[i].w;
+        } else {
+            const uint4 a = reinterpret_cast<const uint4*>(p)[0], b = reinterpret_cast<const uint4*>(p)[1];
+            const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
                 const float2 f = unpack2<T>(w[i]);
                 x[2 * i] = f.x;
                 x[2 * i + 1] = f.y;
@@ -49,7 +67,7 @@ __device__ __forceinline__ void kv4_load8(const T* p, int n, bool wide, float (&
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
+        for (int i = 0; i < kKv4Each; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
     }
 }
 
@@ -60,97 +78,117 @@ __device__ __forceinline__ float exact_sub(float a, float b, float& e) {
     return d;
 }
 
-// The code of x - 8: round((x - zero) / scale) to even, in [-8, 7].  `inv` is about 1 / scale; next to a border between two codes the
-// exact remainder decides, so that the code is that of the exact quotient.
-__device__ __forceinline__ int kv4_code(float x, float zero, float scale, float inv) {
-    const float t = fminf(fmaxf((x - zero) * inv, -8.f), 7.f);
-    float r = rintf(t);
-    if (fabsf(t - r) > 0.4999f) {  // (the quotient's error is below 8 * 2^-21)
-        float e;
-        const float d = exact_sub(x, zero, e), border = floorf(t) + 0.5f;  // border * scale: 5 + 11 bits, exact
-        const float rest = __fadd_rn(__fsub_rn(d, border * scale), e);      // the subtraction is exact so near the border
-        r = rest > 0.f ? border + 0.5f : rest < 0.f ? border - 0.5f : rintf(border);
-    }
-    return (int)fminf(fmaxf(r, -8.f), 7.f);
+// Next to a border between two codes the exact remainder decides, so that the code is that of the exact quotient (x - zero) / scale.
+// t: about the quotient + 8, from 0 to 15.
+static __device__ __noinline__ float kv4_border(float x, float zero, float scale, float t) {
+    float e;
+    const float d = exact_sub(x, zero, e), border = floorf(t) + 0.5f;                    // (border - 8) * scale: 5 + 11 bits, exact
+    const float rest = __fadd_rn(__fsub_rn(d, (border - 8.f) * scale), e);               // the subtraction is exact so near the border
+    return rest > 0.f ? border + 0.5f : rest < 0.f ? border - 0.5f : rintf(border);
 }
 
 template <typename T, int NG>
-static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(Kv4Cache c, const T* k, const T* v, const long long* slots, int n_rows,
+static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(const Kv4Cache c, const T* k, const T* v, const long long* slots, int n_rows,
                                                                           int head_size, long long k_stride, long long v_stride, bool wide) {
     op_begin();
-    constexpr int kLanes = 4 * NG;  // threads of a row
-    const long long i = (long long)blockIdx.x * kKv4RowThreads + threadIdx.x;
-    const long long row = i / kLanes;
-    if ((i - (threadIdx.x & 31)) / kLanes >= n_rows) return;  // (whole warps: the shuffles below need all lanes)
-    const int lane = (int)(i - row * kLanes), d0 = lane * 8;
-    const int token = (int)min(row, (long long)n_rows - 1) / c.kv_heads, head = (int)min(row, (long long)n_rows - 1) - token * c.kv_heads;
+    constexpr int kLanes = 2 * NG;  // threads of a row
+    const uint32_t i = blockIdx.x * kKv4RowThreads + threadIdx.x, row = i / kLanes, lane = i - row * kLanes;
+    if ((i - (threadIdx.x & 31)) / kLanes >= (uint32_t)n_rows) return;  // (whole warps: the shuffles below need all lanes)
+    const uint32_t known = min(row, (uint32_t)n_rows - 1), token = c.by_heads(known), head = known - token * c.kv_heads;
     const long long slot = slots[token];
-    const bool valid = row < n_rows && slot >= 0 && slot < c.slots;
-    float x[8];
-    const int n = head_size - d0;
+    const int d0 = lane * kKv4Each, n = head_size - d0;
+    float x[kKv4Each];
     const T* src = blockIdx.y ? v + token * v_stride : k + token * k_stride;
-    kv4_load8(src + (long long)head * head_size + d0, n, wide, x);
-    float lo = INFINITY, hi = -INFINITY;
+    kv4_load(src + (long long)head * head_size + d0, n, wide, x);
+    float lo, hi;
+    auto ends = [&]() {  // NaN where there is one
+        lo = INFINITY;
+        hi = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
-        if (j < n) {
-            lo = fminf(lo, x[j]);
-            hi = fmaxf(hi, x[j]);
-        }
-    }
+        for (int j = 0; j < kKv4Each; ++j)
+            if (j < n) {
+                asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(x[j]));
+                asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(x[j]));
+            }
+    };
+    ends();
+    if (!(lo >= -65504.f && hi <= 65504.f)) {  // (also where the thread has no dimension, which changes nothing)
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+        for (int j = 0; j < kKv4Each; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
+        ends();
     }
+    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
+    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
     if (lo > hi) lo = hi = 0.f;  // no dimension of the head lies in this group
-    // (hi - lo) / 15 as the exact difference's quotient rounded once to FP32, then to FP16
+    // (hi - lo) / 15: the exact difference's quotient rounded once to FP32, then to FP16
     float e;
-    const float d = exact_sub(hi, lo, e), q = __fdiv_rn(d, 15.f), rest = __fadd_rn(__fmaf_rn(-15.f, q, d), e);
-    const __half scale_h = __float2half_rn(__fadd_rn(q, rest * (1.f / 15.f)));
+    const float d = exact_sub(hi, lo, e), q = d * (1.f / 15.f), rest = __fadd_rn(__fmaf_rn(-15.f, q, d), e);
+    const __half scale_h = __float2half_rn(__fmaf_rn(rest, 1.f / 15.f, q));
     const float scale = __half2float(scale_h);
     const __half zero_h = __float2half_rn(__fmaf_rn(8.f, scale, lo));
-    const float zero = __half2float(zero_h), inv = __fdiv_rn(1.f, scale);
-    uint32_t word = 0;
+    const float zero = __half2float(zero_h);
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+    if (scale == 0.f) inv = 0.f;  // every code 8
+    // codes: quotient + 8 between 0 and 15, rounded by adding 1.5 2^23 (its error is below 16 2^-22; a quotient within 2^-13 of a border is
+    // looked at again)
+    uint32_t word[2] = {0u, 0u};
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int code = j < n && scale > 0.f ? kv4_code(x[j], zero, scale, inv) : 0;
-        word |= (uint32_t)(code + 8) << (4 * j);
+    for (int j = 0; j < kKv4Each; ++j) {
+        float t = fminf(fmaxf(__fadd_rn(__fmul_rn(__fsub_rn(x[j], zero), inv), 8.f), 0.f), 15.f);
+        if (j >= n) t = 8.f;
+        float y = __fadd_rn(t, 12582912.f);
+        if (fabsf(__fsub_rn(t, __fsub_rn(y, 12582912.f))) > 0.49987f) y = __fadd_rn(kv4_border(x[j], zero, scale, t), 12582912.f);
+        word[j / 8] |= (__float_as_uint(y) & 15u) << (4 * (j % 8));
     }
-    if (!valid) return;
-    const long long b = slot / c.capacity, p = slot - b * c.capacity;
-    unsigned char* dst = (blockIdx.y ? c.v : c.k) + ((b * c.kv_heads + head) * c.capacity + p) * kv4_row_bytes(NG);
-    *reinterpret_cast<uint32_t*>(dst + lane * 4) = word;
-    if ((lane & 3) == 0)
-        *reinterpret_cast<uint32_t*>(dst + NG * 16 + lane) = (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(zero_h) << 16;
+    if (row >= (uint32_t)n_rows || slot < 0 || slot >= c.slots) return;
+    unsigned char* dst = (blockIdx.y ? c.v : c.k) + c.row(slot, head) * kv4_row_bytes(NG);
+    if constexpr (NG % 2 == 0) {
+        *reinterpret_cast<uint2*>(dst + lane * 8) = make_uint2(word[0], word[1]);
+    } else {
+        reinterpret_cast<uint32_t*>(dst + lane * 8)[0] = word[0];
+        reinterpret_cast<uint32_t*>(dst + lane * 8)[1] = word[1];
+    }
+    if ((lane & 1) == 0)
+        *reinterpret_cast<uint32_t*>(dst + NG * 16 + lane * 2) = (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(zero_h) << 16;
 }
 
 template <typename T, int NG>
-static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(Kv4Cache c, T* k, T* v, const long long* slots, int n_rows, int head_size,
+static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(const Kv4Cache c, T* k, T* v, const long long* slots, int n_rows, int head_size,
                                                                          long long k_stride, long long v_stride, bool wide) {
     op_begin();
-    constexpr int kLanes = 4 * NG;
-    const long long i = (long long)blockIdx.x * kKv4RowThreads + threadIdx.x;
-    const long long row = i / kLanes;
-    if (row >= n_rows) return;
-    const int lane = (int)(i - row * kLanes), d0 = lane * 8, n = head_size - d0;
-    const int token = (int)row / c.kv_heads, head = (int)row - token * c.kv_heads;
+    constexpr int kLanes = 2 * NG;
+    const uint32_t i = blockIdx.x * kKv4RowThreads + threadIdx.x, row = i / kLanes, lane = i - row * kLanes;
+    if (row >= (uint32_t)n_rows) return;
+    const uint32_t token = c.by_heads(row), head = row - token * c.kv_heads;
+    const int d0 = lane * kKv4Each, n = head_size - d0;
     const long long slot = slots[token];
     if (n <= 0 || slot < 0 || slot >= c.slots) return;
-    const long long b = slot / c.capacity, p = slot - b * c.capacity;
-    const unsigned char* src = (blockIdx.y ? c.v : c.k) + ((b * c.kv_heads + head) * c.capacity + p) * kv4_row_bytes(NG);
-    const uint32_t word = *reinterpret_cast<const uint32_t*>(src + lane * 4);
-    const float2 sz = half2_bits_to_float2(*reinterpret_cast<const uint32_t*>(src + NG * 16 + (lane & ~3)));
-    T* dst = (blockIdx.y ? v + token * v_stride : k + token * k_stride) + (long long)head * head_size + d0;
-    __align__(16) T y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = from_float<T>(__fadd_rn(sz.y, sz.x * (float)((int)(word >> (4 * j) & 15) - 8)));  // (the product is exact)
-    if (wide && n >= 8) {
-#pragma unroll
-        for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
+    const unsigned char* src = (blockIdx.y ? c.v : c.k) + c.row(slot, head) * kv4_row_bytes(NG);
+    uint32_t word[2];
+    if constexpr (NG % 2 == 0) {
+        const uint2 w = *reinterpret_cast<const uint2*>(src + lane * 8);
+        word[0] = w.x;
+        word[1] = w.y;
     } else {
-        for (int j = 0; j < n && j < 8; ++j) dst[j] = y[j];
+        word[0] = reinterpret_cast<const uint32_t*>(src + lane * 8)[0];
+        word[1] = reinterpret_cast<const uint32_t*>(src + lane * 8)[1];
+    }
+    const float2 sz = half2_bits_to_float2(*reinterpret_cast<const uint32_t*>(src + NG * 16 + (lane & ~1u) * 2));
+    T* dst = (blockIdx.y ? v + token * v_stride : k + token * k_stride) + (long long)head * head_size + d0;
+    __align__(16) T y[kKv4Each];
+#pragma unroll
+    for (int j = 0; j < kKv4Each; ++j) {  // 2^23 + code as a bit pattern; the product is exact
+        const float code = __fsub_rn(__uint_as_float(0x4b000000u | (word[j / 8] >> (4 * (j % 8)) & 15u)), 8388616.f);
+        y[j] = from_float<T>(__fmaf_rn(sz.x, code, sz.y));
+    }
+    if (wide && n >= kKv4Each) {
+#pragma unroll
+        for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < kKv4Each; ++j)
+            if (j < n) dst[j] = y[j];
     }
 }
 
