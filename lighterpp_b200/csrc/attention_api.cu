@@ -85,8 +85,8 @@ lpp_status rows_op(const char* name, const void* k, const void* v, const int64_t
     if (((uintptr_t)k | (uintptr_t)v) & (element - 1) || (uintptr_t)slots & 7) return refuse("4-bit cache: a pointer is not aligned to its type");
     const int64_t dense = (int64_t)kv_heads * head_size;
     if (k_stride < dense || v_stride < dense) return refuse("4-bit cache: a token's rows overlap the next one's");
-    // 16 bytes at once where every row starts on such a boundary
-    const bool wide = head_size % 8 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) && k_stride * element % 16 == 0 && v_stride * element % 16 == 0;
+    // 16 bytes at once where every thread's dimensions start on such a boundary
+    const bool wide = head_size % 16 == 0 && !(((uintptr_t)k | (uintptr_t)v) & 15) && k_stride * element % 16 == 0 && v_stride * element % 16 == 0;
     auto by = [](uint32_t d) { return Kv4Div{d, d > 1 ? (uint32_t)((1ull << 32) / d) : 0u}; };
     Kv4Cache c = {(unsigned char*)kc, (unsigned char*)vc, capacity, (long long)batch * capacity, kv_heads, by((uint32_t)kv_heads), by((uint32_t)capacity)};
     const int groups = kv4_held_groups(head_size), rows = n * kv_heads;
@@ -189,8 +189,8 @@ lpp_status lpp_op_kv4_write(void* d_k_cache, void* d_v_cache, const void* d_k, c
                        return with_groups(groups, [&](auto ng) {
                            return with_type(dtype, [&](auto* t) {
                                using T = std::remove_pointer_t<decltype(t)>;
-                               return launch_op(kv4_write_kernel<T, ng.value>, grid, kKv4RowThreads, 0, S(stream), c, (const T*)d_k, (const T*)d_v, (const long long*)d_slots,
-                                                rows, head_size, (long long)k_stride, (long long)v_stride, wide);
+                               return launch_op(wide ? kv4_write_kernel<T, ng.value, true> : kv4_write_kernel<T, ng.value, false>, grid, kKv4RowThreads, 0, S(stream), c, (const T*)d_k, (const T*)d_v, (const long long*)d_slots,
+                                                rows, head_size, (long long)k_stride, (long long)v_stride);
                            });
                        });
                    });
@@ -203,8 +203,8 @@ lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const vo
                        return with_groups(groups, [&](auto ng) {
                            return with_type(dtype, [&](auto* t) {
                                using T = std::remove_pointer_t<decltype(t)>;
-                               return launch_op(kv4_read_kernel<T, ng.value>, grid, kKv4RowThreads, 0, S(stream), c, (T*)d_k, (T*)d_v, (const long long*)d_slots, rows, head_size,
-                                                (long long)k_stride, (long long)v_stride, wide);
+                               return launch_op(wide ? kv4_read_kernel<T, ng.value, true> : kv4_read_kernel<T, ng.value, false>, grid, kKv4RowThreads, 0, S(stream), c, (T*)d_k, (T*)d_v, (const long long*)d_slots, rows, head_size,
+                                                (long long)k_stride, (long long)v_stride);
                            });
                        });
                    });

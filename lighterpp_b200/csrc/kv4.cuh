@@ -40,15 +40,15 @@ struct Kv4Cache {
 // ------------------------------------------------------------------ writing and reading rows
 //
 // Two threads a group, sixteen dimensions (two 32-bit words of codes) each.  Bound by the instructions on the way in (about 20 an element; eight
-// elements a thread, conversions by the conversion unit and 64-bit divisions: 34 us where this takes NN), by the bytes of the values on
+// elements a thread, conversions by the conversion unit and 64-bit divisions: 34 us for 8001 tokens of 8 heads of 128 where this takes 16), by the bytes of the values on
 // the way out.
 
 constexpr int kKv4RowThreads = 256, kKv4Each = 16;  // kKv4Each: dimensions of a thread
 
-// Sixteen consecutive values; `n` of them exist.
-template <typename T>
-__device__ __forceinline__ void kv4_load(const T* p, int n, bool wide, float (&x)[kKv4Each]) {
-    if (wide && n >= kKv4Each) {
+// Sixteen consecutive values; `n` of them exist, the others are the first one again.  WIDE: all or none exist, on a 16-byte boundary.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void kv4_load(const T* p, int n, float (&x)[kKv4Each]) {
+    if constexpr (WIDE) {
         if constexpr (sizeof(T) == 4) {
             float4 a[4];
 #pragma unroll
@@ -67,7 +67,7 @@ __device__ __forceinline__ void kv4_load(const T* p, int n, bool wide, float (&x
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < kKv4Each; ++i) x[i] = i < n ? to_float(p[i]) : 0.f;
+        for (int i = 0; i < kKv4Each; ++i) x[i] = i < n ? to_float(p[i]) : i > 0 ? x[0] : 0.f;
     }
 }
 
@@ -78,18 +78,18 @@ __device__ __forceinline__ float exact_sub(float a, float b, float& e) {
     return d;
 }
 
-// Next to a border between two codes the exact remainder decides, so that the code is that of the exact quotient (x - zero) / scale.
-// t: about the quotient + 8, from 0 to 15.
-static __device__ __noinline__ float kv4_border(float x, float zero, float scale, float t) {
+// The code of x where about `t` = (x - zero) / scale + 8, from 0 to 15, comes out next to a border between two codes: the exact remainder
+// decides, so that the code is that of the exact quotient.
+__device__ __forceinline__ uint32_t kv4_border(float x, float zero, float scale, float t) {
     float e;
-    const float d = exact_sub(x, zero, e), border = floorf(t) + 0.5f;                    // (border - 8) * scale: 5 + 11 bits, exact
-    const float rest = __fadd_rn(__fsub_rn(d, (border - 8.f) * scale), e);               // the subtraction is exact so near the border
-    return rest > 0.f ? border + 0.5f : rest < 0.f ? border - 0.5f : rintf(border);
+    const float d = exact_sub(x, zero, e), border = floorf(t) + 0.5f;       // (border - 8) * scale: 5 + 11 bits, exact
+    const float rest = __fadd_rn(__fsub_rn(d, (border - 8.f) * scale), e);  // the subtraction is exact so near the border
+    return (uint32_t)(rest > 0.f ? border + 0.5f : rest < 0.f ? border - 0.5f : rintf(border));
 }
 
-template <typename T, int NG>
-static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(const Kv4Cache c, const T* k, const T* v, const long long* slots, int n_rows,
-                                                                          int head_size, long long k_stride, long long v_stride, bool wide) {
+template <typename T, int NG, bool WIDE>
+static __global__ void __launch_bounds__(kKv4RowThreads, 5) kv4_write_kernel(const Kv4Cache c, const T* k, const T* v, const long long* slots, int n_rows,
+                                                                          int head_size, long long k_stride, long long v_stride) {
     op_begin();
     constexpr int kLanes = 2 * NG;  // threads of a row
     const uint32_t i = blockIdx.x * kKv4RowThreads + threadIdx.x, row = i / kLanes, lane = i - row * kLanes;
@@ -99,27 +99,29 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(const 
     const int d0 = lane * kKv4Each, n = head_size - d0;
     float x[kKv4Each];
     const T* src = blockIdx.y ? v + token * v_stride : k + token * k_stride;
-    kv4_load(src + (long long)head * head_size + d0, n, wide, x);
+    kv4_load<T, WIDE>(src + (long long)head * head_size + (n > 0 ? d0 : 0), n, x);  // (where there is none: the first, which does not count)
     float lo, hi;
     auto ends = [&]() {  // NaN where there is one
-        lo = INFINITY;
-        hi = -INFINITY;
+        lo = hi = x[0];
 #pragma unroll
-        for (int j = 0; j < kKv4Each; ++j)
-            if (j < n) {
-                asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(x[j]));
-                asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(x[j]));
-            }
+        for (int j = 1; j < kKv4Each; ++j) {
+            asm("min.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(x[j]));
+            asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(x[j]));
+        }
     };
     ends();
-    if (!(lo >= -65504.f && hi <= 65504.f)) {  // (also where the thread has no dimension, which changes nothing)
+    if (!(lo >= -65504.f && hi <= 65504.f)) {
 #pragma unroll
         for (int j = 0; j < kKv4Each; ++j) x[j] = x[j] == x[j] ? fminf(fmaxf(x[j], -65504.f), 65504.f) : 0.f;
         ends();
     }
+    if (n <= 0) {  // no dimension of the head lies here
+        lo = INFINITY;
+        hi = -INFINITY;
+    }
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, 1));
     hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
-    if (lo > hi) lo = hi = 0.f;  // no dimension of the head lies in this group
+    if (lo > hi) lo = hi = 0.f;  // nor in the whole group
     // (hi - lo) / 15: the exact difference's quotient rounded once to FP32, then to FP16
     float e;
     const float d = exact_sub(hi, lo, e), q = d * (1.f / 15.f), rest = __fadd_rn(__fmaf_rn(-15.f, q, d), e);
@@ -129,17 +131,37 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(const 
     const float zero = __half2float(zero_h);
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
-    if (scale == 0.f) inv = 0.f;  // every code 8
-    // codes: quotient + 8 between 0 and 15, rounded by adding 1.5 2^23 (its error is below 16 2^-22; a quotient within 2^-13 of a border is
-    // looked at again)
+    inv = scale == 0.f ? 0.f : inv * (1.f / 15.f);  // (0: every code 8)
+    // Codes: a fifteenth of (quotient + 8), cut to 0 .. 1, times fifteen and rounded by adding 1.5 2^23.  The quotient is off by less than
+    // 2^-17; where one came within 2^-13 of a border the thread looks at its values again.
     uint32_t word[2] = {0u, 0u};
+    float worst = 0.f;
 #pragma unroll
     for (int j = 0; j < kKv4Each; ++j) {
-        float t = fminf(fmaxf(__fadd_rn(__fmul_rn(__fsub_rn(x[j], zero), inv), 8.f), 0.f), 15.f);
-        if (j >= n) t = 8.f;
-        float y = __fadd_rn(t, 12582912.f);
-        if (fabsf(__fsub_rn(t, __fsub_rn(y, 12582912.f))) > 0.49987f) y = __fadd_rn(kv4_border(x[j], zero, scale, t), 12582912.f);
-        word[j / 8] |= (__float_as_uint(y) & 15u) << (4 * (j % 8));
+        float t;
+        asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(t) : "f"(__fsub_rn(x[j], zero)), "f"(inv), "f"(8.f / 15.f));
+        const float y = __fmaf_rn(t, 15.f, 12582912.f);
+        worst = fmaxf(worst, fabsf(__fmaf_rn(t, 15.f, -__fsub_rn(y, 12582912.f))));
+        word[j / 8] += __float_as_uint(y) << (4 * (j % 8));
+    }
+#pragma unroll
+    for (int w = 0; w < 2; ++w) word[w] -= 0x3f400000u;  // what 1.5 2^23 put there eight times, 4 bits apart
+    if (worst > 0.49987f) {
+        float from = zero;
+        asm volatile("" : "+f"(from));  // (quotients are made again here, not kept from above)
+#pragma unroll
+        for (int j = 0; j < kKv4Each; ++j) {
+            const float u = fminf(fmaxf(__fmaf_rn(__fsub_rn(x[j], from), inv * 15.f, 8.f), 0.f), 15.f);
+            if (fabsf(u - rintf(u)) > 0.4998f) word[j / 8] = (word[j / 8] & ~(15u << (4 * (j % 8)))) | min(kv4_border(x[j], zero, scale, u), 15u) << (4 * (j % 8));
+        }
+    }
+    if (n < (WIDE ? 1 : kKv4Each)) {  // dimensions that the head does not have: code 8
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int have = n - 8 * w;
+            const uint32_t there = have >= 8 ? ~0u : have <= 0 ? 0u : (1u << (4 * have)) - 1u;
+            word[w] = (word[w] & there) | (0x88888888u & ~there);
+        }
     }
     if (row >= (uint32_t)n_rows || slot < 0 || slot >= c.slots) return;
     unsigned char* dst = (blockIdx.y ? c.v : c.k) + c.row(slot, head) * kv4_row_bytes(NG);
@@ -153,9 +175,9 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_write_kernel(const 
         *reinterpret_cast<uint32_t*>(dst + NG * 16 + lane * 2) = (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(zero_h) << 16;
 }
 
-template <typename T, int NG>
+template <typename T, int NG, bool WIDE>
 static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(const Kv4Cache c, T* k, T* v, const long long* slots, int n_rows, int head_size,
-                                                                         long long k_stride, long long v_stride, bool wide) {
+                                                                         long long k_stride, long long v_stride) {
     op_begin();
     constexpr int kLanes = 2 * NG;
     const uint32_t i = blockIdx.x * kKv4RowThreads + threadIdx.x, row = i / kLanes, lane = i - row * kLanes;
@@ -182,7 +204,7 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(const K
         const float code = __fsub_rn(__uint_as_float(0x4b000000u | (word[j / 8] >> (4 * (j % 8)) & 15u)), 8388616.f);
         y[j] = from_float<T>(__fmaf_rn(sz.x, code, sz.y));
     }
-    if (wide && n >= kKv4Each) {
+    if constexpr (WIDE) {
 #pragma unroll
         for (int j = 0; j < (int)sizeof(T); ++j) reinterpret_cast<uint4*>(dst)[j] = reinterpret_cast<const uint4*>(y)[j];
     } else {
