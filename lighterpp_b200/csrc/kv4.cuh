@@ -233,7 +233,8 @@ static __global__ void __launch_bounds__(kKv4RowThreads) kv4_read_kernel(const K
 // FP16 range: probabilities are 2^(x - M) with M far enough below the largest x + log2(scale) seen when M was set that they keep their
 // bits, and M moves only when a product would leave the range.  So a tile needs no maximum over lanes, only a vote.
 //
-// FP32 queries and FP32 results go in as two FP16 operands each (hi + lo), the sums of either added up.
+// SPLIT: FP32 queries and FP32 results go in as two FP16 operands each (hi + lo), the sums of either added up, and the keys' codes are
+// n - 8 too, with (0, Q_g): sums of n and 8 Q_g that cancel would cost two bits of the scores.
 constexpr int kKv4Warps = 8, kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tile = 16;     // positions of a warp's tile
 constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
@@ -452,6 +453,7 @@ struct Kv4Ahead {
 template <int NG, bool SPLIT>
 static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_kernel(const Kv4AttnArgs a) {
     constexpr int kRow = kv4_row_bytes(NG), kStage = kKv4StageBytes<NG>, kParts = SPLIT ? 2 : 1, kPitch = kKv4Pitch<NG>;
+    constexpr float kUnit = SPLIT ? 1.f : 0x1p24f;  // of the keys' codes as operands
     extern __shared__ __align__(128) unsigned char smem[];
     __shared__ float s_m[kKv4Warps][kKv4Heads], s_l[kKv4Warps][kKv4Heads];
     __shared__ uint64_t full[kKv4MaxStages], empty[kKv4MaxStages];
@@ -563,26 +565,27 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
         for (int i = 0; i < NG; ++i) {
             float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16
-                const float f = (j & 1) ? 1.f / 16.f : 1.f;
+            for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16 (SPLIT: none)
+                const bool sixteenth = !SPLIT && (j & 1);
+                const float f = sixteenth ? 1.f / 16.f : 1.f;
                 const float u = x[i][j] * f0 * f1, w = x[i][j + 4] * f0 * f1;
                 const __half2 hi = __floats2half2_rn(u * f, w * f);
                 const float2 hf = __half22float2(hi);
                 qf[0][i][j] = *reinterpret_cast<const uint32_t*>(&hi);
-                sum += (hf.x + hf.y) * ((j & 1) ? 16.f : 1.f);
+                sum += (hf.x + hf.y) * (sixteenth ? 16.f : 1.f);
                 if constexpr (SPLIT) {
                     const __half2 lo = __floats2half2_rn(u * f - hf.x, w * f - hf.y);
                     const float2 lf = __half22float2(lo);
                     qf[1][i][j] = *reinterpret_cast<const uint32_t*>(&lo);
-                    sum += (lf.x + lf.y) * ((j & 1) ? 16.f : 1.f);
+                    sum += lf.x + lf.y;
                 }
             }
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
             sums[i] = sum;
         }
-        // 2^24 / 2^e, back from the operands' factors
-        const float back = __int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * 0x1p24f * a.rate;
+        // back from the operands' factors: 2^24 / 2^e
+        const float back = __int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * kUnit * a.rate;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int from = (2 * t + j) * 4;
@@ -595,7 +598,8 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
 #pragma unroll
         for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
             const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
-            const __half2 both = __halves2half2(__hmul(hi, __float2half_rn(-8.f)), hi), rest = __halves2half2(__hmul(lo, __float2half_rn(-8.f)), lo);
+            const __half times = __float2half_rn(SPLIT ? 0.f : -8.f);
+            const __half2 both = __halves2half2(__hmul(hi, times), hi), rest = __halves2half2(__hmul(lo, times), lo);
             zf[0][i] = *reinterpret_cast<const uint32_t*>(&both);
             zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = *reinterpret_cast<const uint32_t*>(&rest);
         }
@@ -622,7 +626,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
             kv4_params<NG>(r0, p0);
             kv4_params<NG>(r1, p1w);
-            // rows of (scale, zero) pairs as they lie there times (-8 Q, Q)
+            // rows of (scale, zero) pairs as they lie there times (-8 Q, Q), or (0, Q)
             float zacc[4], acc[NG][4];
             if constexpr (NG > 4) {
                 const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
@@ -634,22 +638,23 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             }
             // (the groups' chains of products side by side)
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
-                kv4_mma(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[0][gr][0], qf[0][gr][1]);
-            if constexpr (SPLIT) {
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr)
-                    kv4_mma_add(acc[gr], w[gr][0] & 0x000f000fu, w[gr][1] & 0x000f000fu, w[gr][0] & 0x00f000f0u, w[gr][1] & 0x00f000f0u, qf[1][gr][0], qf[1][gr][1]);
-            }
-#pragma unroll
-            for (int part = 0; part < kParts; ++part)
+            for (int half = 0; half < 2; ++half)
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr) {
-                    const uint32_t v0 = w[gr][0] >> 8, v1 = w[gr][1] >> 8;
-                    kv4_mma_add(acc[gr], v0 & 0x000f000fu, v1 & 0x000f000fu, v0 & 0x00f000f0u, v1 & 0x00f000f0u, qf[part][gr][2], qf[part][gr][3]);
+                    const uint32_t x0 = w[gr][0] >> (8 * half), x1 = w[gr][1] >> (8 * half);
+                    uint32_t a0, a1, a2, a3;
+                    if constexpr (SPLIT)
+                        a0 = kv4_low(x0, magic), a1 = kv4_low(x1, magic), a2 = kv4_high(x0, magic), a3 = kv4_high(x1, magic);
+                    else
+                        a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+                    if (half == 0)
+                        kv4_mma(acc[gr], a0, a1, a2, a3, qf[0][gr][0], qf[0][gr][1]);
+                    else
+                        kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[0][gr][2], qf[0][gr][3]);
+                    if constexpr (SPLIT) kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[1][gr][2 * half], qf[1][gr][2 * half + 1]);
                 }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = zacc[j] * 0x1p-24f;
+            for (int j = 0; j < 4; ++j) s[j] = zacc[j] * (1.f / kUnit);
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 const float s0 = half2_bits_to_float2(p0[gr]).x, s1 = half2_bits_to_float2(p1w[gr]).x;
@@ -953,7 +958,7 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // shared memory), then every CTA knows where its kept rows begin in the new cache and lists them.  A second kernel, of many small CTAs,
 // moves them: bound by the rows' bytes where they are many, by the meetings of the cluster where they are few.  (Digits of 11 bits added
 // up by remote atomics in one CTA: passes of 3 - 8 us each instead of 1.4.  Rows moved by the cluster that lists them, two sequences of
-// 32768 and 20011 positions to 12000: 30 us, its SMs being too few for the bandwidth; now NN.)
+// 32768 and 20011 positions to 12000: 30 us, its SMs being too few for the bandwidth; now 26.)
 // 512 threads: two CTAs fit an SM (of 1024, sixteen clusters of eight did not fit the GPU at once, and the last ran alone).
 constexpr int kKv4EvictThreads = 512, kKv4EvictCluster = 8;
 constexpr int kKv4EvictKeep = 8;  // rows of a thread whose ranks stay in registers
