@@ -170,10 +170,7 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
         a.tiles = (n_tokens + cta_rows - 1) / cta_rows;
         a.rate = scale * 1.4426950408889634f;
         if ((long long)a.tiles * per_tile > 0x7fffffffll) return LPP_ERR_TOO_LARGE;
-        if (cudaFuncSetAttribute(prompt_attention_kernel<HS, T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem) != cudaSuccess) {
-            (void)cudaGetLastError();
-            return LPP_ERR_CUDA;
-        }
+        if (!allow_smem<prompt_attention_kernel<HS, T>>(Shape::kSmem)) return LPP_ERR_CUDA;
         return launch_op(prompt_attention_kernel<HS, T>, dim3(a.tiles * per_tile), Shape::kThreads, Shape::kSmem, S(stream), q_map, k_map, v_map, a);
     };
     auto by_type = [&](auto shape) { return dtype == LPP_F16 ? go(shape, (__half*)nullptr) : go(shape, (__nv_bfloat16*)nullptr); };
@@ -266,10 +263,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
                         a.stages = std::min(kKv4MaxStages, room / kKv4StageBytes<NG>);
                         const int smem = a.stages * kKv4StageBytes<NG> + sums;
                         auto kernel = dtype == LPP_F32 ? kv4_attn_kernel<NG, true> : kv4_attn_kernel<NG, false>;
-                        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
-                            (void)cudaGetLastError();
-                            return LPP_ERR_CUDA;
-                        }
+                        if (!(dtype == LPP_F32 ? allow_smem<kv4_attn_kernel<NG, true>>(smem) : allow_smem<kv4_attn_kernel<NG, false>>(smem))) return LPP_ERR_CUDA;
                         const lpp_status st = launch_op(kernel, dim3(runs), kKv4Threads, smem, S(stream), a);
                         if (st != LPP_OK) return st;
                         const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;

@@ -855,6 +855,7 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
     pdl_launch_dependents();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kvh = blockIdx.y, b = blockIdx.z, heads8 = a.kv_heads * a.head_tiles;
     const int len = kv4_len(a, b), units = kv4_units(len), weight = kv4_weight(len), row_block = (int)blockIdx.x - a.gqa;
+    if (row_block * kKv4FinishRows >= len && row_block >= 0) return;  // (others of the grid wait for the kernel before)
     const Kv4Runs runs(a.runs, kv4_total(a) * heads8);
     int before = 0;
     for (int i = lane; i < b; i += 32) before += kv4_weight(kv4_len(a, i));

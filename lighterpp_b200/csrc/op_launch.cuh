@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "../../include/lpp_b200.h"
 
@@ -41,6 +42,20 @@ lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, s
     cfg.attrs = attr;
     cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
     return chk();
+}
+// Lets a kernel have more than 48 KB of shared memory: once on every device (asked at every launch it is 0.4 us of the host's time).
+template <auto KERNEL>
+bool allow_smem(size_t bytes) {
+    static std::atomic<size_t> allowed[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return false;
+    }
+    allowed[dev].store(bytes, std::memory_order_relaxed);
+    return true;
 }
 template <typename... KArgs, typename... Args>
 lpp_status launch_op(void (*kernel)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t s, Args... args) {

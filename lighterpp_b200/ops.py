@@ -25,7 +25,15 @@ def _s() -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+_bound = None
+
+
 def _lib():
+    return _bound or _bind()
+
+
+def _bind():
+    global _bound
     lib = load_library()
     if not getattr(lib, "_ops_bound", False):
         vp, i, f, i64 = C.c_void_p, C.c_int, C.c_float, C.c_int64
@@ -55,6 +63,7 @@ def _lib():
         lib.lpp_op_kv4_attention.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, vp, f, i, i, i, i64, i, i64, i64, i, vp]
         lib.lpp_op_kv4_evict.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i64, i64, i, i, i, vp]
         lib._ops_bound = True
+    _bound = lib
     return lib
 
 
@@ -151,11 +160,12 @@ def _call(what, entry, device, *args):
         _check(st, what)
 
 
-def _device(what, first, *others):
-    device = first.get_device()
-    for t in others:
+def _device(what, *tensors):
+    """The one device of all ``tensors`` (None: left out)."""
+    device = tensors[0].get_device()
+    for t in tensors:
         if t is not None and t.get_device() != device:
-            raise ValueError(f"{what}: expected CUDA tensors on one device")
+            device = -1
     if device < 0:
         raise ValueError(f"{what}: expected CUDA tensors on one device")
     return device
@@ -168,11 +178,11 @@ def _want(what, t, dtype, *shape):
 
 def _heads(what, t, dtype, shape):
     """Elements from one token of ``t`` [tokens, heads, head_size] to the next."""
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and len(shape) == 3:
+        return shape[1] * shape[2]
     if t.dtype is not dtype or t.shape != shape or len(shape) != 3:
         raise ValueError(f"{what}: got {t.dtype} {tuple(t.shape)}, expected {dtype} [tokens, heads, head_size]" + (f" = {tuple(shape)}" if t.shape != shape else ""))
     tokens, heads, size = shape
-    if t.is_contiguous():
-        return heads * size
     if (size > 1 and t.stride(2) != 1) or (heads > 1 and t.stride(1) != size):
         raise ValueError(f"{what}: the heads of a token lie behind one another")
     return t.stride(0) if tokens > 1 else heads * size
