@@ -258,13 +258,23 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.rate = scale * 1.4426950408889634f;
     return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
                         constexpr int NG = ng.value;
+                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = (227 * 1024) / kKv4Ctas<NG> - 1024 * (NG + 2) - sums;
+                        auto go = [&](auto parts, auto clusters, int stages) {
+                            constexpr auto kernel = kv4_attn_kernel<NG, parts.value == 2, clusters.value == 1>;
+                            a.stages = std::min(stages, room / kKv4StageBytes<NG>);
+                            const int smem = a.stages * kKv4StageBytes<NG> + sums;
+                            if (!allow_smem<kernel>(smem)) return LPP_ERR_CUDA;
+                            return launch_op_cluster(kernel, dim3(clusters.value ? a.cluster * batch * n_kv_heads * a.head_tiles : runs), kKv4Threads, smem,
+                                                     clusters.value ? a.cluster : 1, false, S(stream), a);
+                        };
+                        // a cluster a head where the cache is short and the clusters run at once (with sums: where one has all query heads)
+                        const long long heads = (long long)batch * n_kv_heads * a.head_tiles, units = (capacity + kKv4Unit - 1) / kKv4Unit;
+                        a.cluster = 1;
+                        while (a.cluster < kKv4Cluster && a.cluster < units && 2 * a.cluster * heads <= (long long)sms * kKv4Ctas<NG>) a.cluster *= 2;
+                        if (units <= (long long)kKv4ClusterUnits * a.cluster && heads * a.cluster <= (long long)sms * kKv4Ctas<NG> && !(d_sums_out && a.head_tiles > 1))
+                            return dtype == LPP_F32 ? go(Int<2>(), Int<1>(), kKv4ClusterUnits) : go(Int<1>(), Int<1>(), kKv4ClusterUnits);
                         // as many units in flight as the shared memory holds beside the warps' sums
-                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = (227 * 1024) / kKv4Ctas<NG> - 2048 - sums;
-                        a.stages = std::min(kKv4MaxStages, room / kKv4StageBytes<NG>);
-                        const int smem = a.stages * kKv4StageBytes<NG> + sums;
-                        auto kernel = dtype == LPP_F32 ? kv4_attn_kernel<NG, true> : kv4_attn_kernel<NG, false>;
-                        if (!(dtype == LPP_F32 ? allow_smem<kv4_attn_kernel<NG, true>>(smem) : allow_smem<kv4_attn_kernel<NG, false>>(smem))) return LPP_ERR_CUDA;
-                        const lpp_status st = launch_op(kernel, dim3(runs), kKv4Threads, smem, S(stream), a);
+                        const lpp_status st = dtype == LPP_F32 ? go(Int<2>(), Int<0>(), kKv4MaxStages) : go(Int<1>(), Int<0>(), kKv4MaxStages);
                         if (st != LPP_OK) return st;
                         const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;
                         return launch_behind(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + runs) * 4, S(stream), a);

@@ -131,7 +131,10 @@ def check(T, q, k, v, lens, scale, name, with_sums=True, gap=0, call=None):
 @pytest.mark.parametrize("name", TYPES)
 @pytest.mark.parametrize("heads,kv,size,lens,cap", [
     (8, 2, 64, (1, 0, 17, 128), 128), (32, 8, 128, (129, 1000), 1024), (6, 6, 48, (200,), 200), (3, 1, 32, (15, 16, 31), 32), (9, 1, 64, (300, 5), 300),
-    (40, 2, 128, (257,), 260), (8, 8, 96, (127, 640, 64), 640), (4, 2, 33, (77,), 80), (2, 1, 256, (333, 2), 336), (12, 3, 160, (140,), 140), (1, 1, 1, (9,), 12)])
+    (40, 2, 128, (257,), 260), (8, 8, 96, (127, 640, 64), 640), (4, 2, 33, (77,), 80), (2, 1, 256, (333, 2), 336), (12, 3, 160, (140,), 140), (1, 1, 1, (9,), 12),
+    # caches that are not short: heads dealt out in runs
+    (8, 2, 64, (2500, 0, 17, 1), 2600), (32, 8, 128, (4000,), 4096), (6, 6, 48, (2300, 100), 2304), (9, 1, 64, (2500, 5), 2560), (40, 2, 128, (2570,), 2600),
+    (2, 1, 256, (2700,), 2720), (8, 4, 160, (2200, 2305), 2400), (1, 1, 1, (2100,), 2100), (16, 16, 96, (700, 1024, 3, 129), 2500)])
 def test_attention(T, name, heads, kv, size, lens, cap):
     q, k, v = setup(T, heads, kv, size, name, lens, cap, heads + size)
     check(T, q, k, v, lens, size ** -0.5, name, with_sums=True, gap=5 if size == 48 else 0)
@@ -148,9 +151,10 @@ def test_attention_without_sums(T, name):
 def test_attention_over_many_sequences(T, name):
     """More sequences than lanes of a warp; most of the runs hold several heads."""
     rng = np.random.default_rng(1)
-    lens = tuple(int(x) for x in rng.integers(0, 200, 75))
-    q, k, v = setup(T, 8, 2, 64, name, lens, 200, 6)
-    check(T, q, k, v, lens, 0.125, name)
+    for most in (200, 400):  # either side of what counts as short
+        lens = tuple(int(x) for x in rng.integers(0, most, 75))
+        q, k, v = setup(T, 8, 2, 64, name, lens, most, 6)
+        check(T, q, k, v, lens, 0.125, name)
 
 
 @pytest.mark.parametrize("name", TYPES)
