@@ -367,7 +367,8 @@ lpp_status lpp_op_sample_static(float* d_logits, int vocab_size, float temperatu
  * q and out are [token][n_heads][head_size], k and v [token][n_kv_heads][head_size], F16 or BF16, *_stride elements from one token to the
  * next (a multiple of 8, at least a token's elements), on 16-byte boundaries; head sizes are multiples of 8 up to 128.  The arrays hold n_tokens tokens:
  * results of those from d_offsets[n_sequences] on are left as they were, and their queries, keys and values are not looked at.  Scores and
- * sums are FP32, probabilities are rounded to the type. */
+ * sums are FP32, probabilities are rounded to the type.  What is not finite reaches the tokens that see it and no others.  The results
+ * overlap none of the inputs. */
 lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k, const void* d_v, const int* d_offsets, int n_sequences, int n_tokens,
                                    int n_heads, int n_kv_heads, int head_size, int64_t out_stride, int64_t q_stride, int64_t k_stride,
                                    int64_t v_stride, float scale, int dtype, void* stream);
@@ -399,7 +400,8 @@ lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const vo
  * d_sums_out (may be NULL) gets the running sums of attention weight that lpp_op_kv4_evict goes by, [batch][n_kv_heads][capacity]:
  * d_sums_in (NULL = zeros; may be the same array) plus, per position, the sum of the softmax over the query heads of the key/value
  * head.  Positions from the length on are left as they were.
- * scratch: lpp_op_kv4_attention_scratch_bytes(...) bytes on a 256-byte boundary, of any content; calls that may overlap need their own. */
+ * scratch: lpp_op_kv4_attention_scratch_bytes(...) bytes (0: none, it may be NULL) on a 256-byte boundary, of any content; calls that may
+ * overlap need their own. */
 int64_t lpp_op_kv4_attention_scratch_bytes(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int with_sums);
 lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_out, const void* d_q, const void* d_k_cache, const void* d_v_cache,
                                 const int* d_lens, const float* d_sums_in, float* d_sums_out, float scale, int batch, int n_heads, int n_kv_heads,

@@ -23,7 +23,7 @@ lpp_status refuse(const char* what, lpp_status s = LPP_ERR_INVALID_ARG) {
 }
 lpp_status launched(const char* what, lpp_status s) { return s == LPP_OK ? s : refuse(what, s); }
 
-int sm_count() {
+int sm_count() {  // of the current device; 0: none
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) {
         (void)cudaGetLastError();
@@ -94,23 +94,31 @@ lpp_status rows_op(const char* name, const void* k, const void* v, const int64_t
     return launched(name, launch(c, groups, dim3((unsigned)ctas, 2), rows, wide));
 }
 
-// ---- attention over the 4-bit cache: runs of work (one a CTA, as many CTAs as the SMs hold) and the scratch
-int attn_runs(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int sms) {
-    sms *= kv4_held_groups(head_size) > 4 ? kKv4Ctas<8> : kKv4Ctas<4>;
-    const int head_tiles = (n_heads / n_kv_heads + kKv4Heads - 1) / kKv4Heads;
-    return (int)std::min<long long>(sms, (long long)batch * n_kv_heads * head_tiles * ((capacity + kKv4Unit - 1) / kKv4Unit));
-}
-struct AttnLayout {
-    size_t whole, ml, part, scores, total;
+// ---- attention over the 4-bit cache: how the work is dealt out, and the scratch
+struct AttnPlan {
+    int cluster;  // CTAs of a head; 0: runs of all heads' units, as many as the SMs hold CTAs
+    int runs;
+    size_t whole, ml, part, scores, total;  // places in the scratch
 };
-AttnLayout attn_layout(int runs, int batch, int n_heads, int64_t capacity, int groups, bool sums) {
+AttnPlan attn_plan(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, bool sums, int sms) {
+    const int groups = kv4_held_groups(head_size), head_tiles = (n_heads / n_kv_heads + kKv4Heads - 1) / kKv4Heads;
+    const long long ctas = (long long)sms * (groups > 4 ? kKv4Ctas<8> : kKv4Ctas<4>), heads = (long long)batch * n_kv_heads * head_tiles;
+    const long long units = (capacity + kKv4Unit - 1) / kKv4Unit;
+    AttnPlan P = {};
     auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    AttnLayout L = {};
-    L.ml = up(sums ? (size_t)batch * n_heads * 8 : 0);
-    L.part = L.ml + up((size_t)runs * 2 * kKv4Heads * 8);
-    L.scores = L.part + up((size_t)runs * 2 * kKv4Heads * groups * 32 * 4);
-    L.total = L.scores + up(sums ? (size_t)batch * n_heads * capacity * 4 : 0);
-    return L;
+    // a cluster a head where the cache is short and the clusters run at once (with sums: where one has all query heads)
+    int cluster = 1;
+    while (cluster < kKv4Cluster && cluster < units && 2 * cluster * heads <= ctas) cluster *= 2;
+    if (units <= (long long)kKv4ClusterUnits * cluster && heads * cluster <= ctas && !(sums && head_tiles > 1)) {
+        P.cluster = cluster;
+    } else {
+        P.runs = (int)std::min(ctas, heads * units);
+        P.ml = up(sums ? (size_t)batch * n_heads * 8 : 0);
+        P.part = P.ml + up((size_t)P.runs * 2 * kKv4Heads * 8);
+        P.scores = P.part + up((size_t)P.runs * 2 * kKv4Heads * groups * 32 * 4);
+    }
+    P.total = P.scores + up(sums ? (size_t)batch * n_heads * capacity * 4 : 0);
+    return P;
 }
 const char* attn_fault(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size) {
     if (const char* f = size_fault(batch, n_kv_heads, capacity, head_size)) return f;
@@ -210,7 +218,7 @@ lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const vo
 int64_t lpp_op_kv4_attention_scratch_bytes(int batch, int n_heads, int n_kv_heads, int64_t capacity, int head_size, int with_sums) {
     const int sms = sm_count();
     if (sms <= 0 || attn_fault(batch, n_heads, n_kv_heads, capacity, head_size)) return -1;
-    return (int64_t)attn_layout(attn_runs(batch, n_heads, n_kv_heads, capacity, head_size, sms), batch, n_heads, capacity, kv4_held_groups(head_size), with_sums != 0).total;
+    return (int64_t)attn_plan(batch, n_heads, n_kv_heads, capacity, head_size, with_sums != 0, sms).total;
 }
 
 lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_out, const void* d_q, const void* d_k_cache, const void* d_v_cache, const int* d_lens,
@@ -218,7 +226,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
                                 int64_t out_stride, int64_t q_stride, int dtype, void* stream) {
     if (const char* f = cache_fault(d_k_cache, d_v_cache, batch, n_kv_heads, capacity, head_size)) return refuse(f);
     if (const char* f = attn_fault(batch, n_heads, n_kv_heads, capacity, head_size)) return refuse(f);
-    if (!scratch || ((uintptr_t)scratch & 255) || !d_out || !d_q || !d_lens) return refuse("4-bit attention: null pointer, or scratch not on a 256-byte boundary");
+    if (((uintptr_t)scratch & 255) || !d_out || !d_q || !d_lens) return refuse("4-bit attention: null pointer, or scratch not on a 256-byte boundary");
     if (!is_dtype(dtype)) return refuse("4-bit attention: queries are F32, F16 or BF16");
     const int element = dtype == LPP_F32 ? 4 : 2;
     if (((uintptr_t)d_out | (uintptr_t)d_q) & (element - 1) || ((uintptr_t)d_lens | (uintptr_t)d_sums_in | (uintptr_t)d_sums_out) & 3)
@@ -228,9 +236,9 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     if (d_sums_in && !d_sums_out) return refuse("4-bit attention: sums go in but not out");
     const int sms = sm_count();
     if (sms <= 0) return refuse("4-bit attention: no CUDA device", LPP_ERR_NO_DEVICE);
-    const int groups = kv4_held_groups(head_size), runs = attn_runs(batch, n_heads, n_kv_heads, capacity, head_size, sms);
-    const AttnLayout L = attn_layout(runs, batch, n_heads, capacity, groups, d_sums_out != nullptr);
-    if (scratch_bytes < (int64_t)L.total) return refuse("4-bit attention: scratch is smaller than lpp_op_kv4_attention_scratch_bytes() says");
+    const int groups = kv4_held_groups(head_size);
+    const AttnPlan P = attn_plan(batch, n_heads, n_kv_heads, capacity, head_size, d_sums_out != nullptr, sms);
+    if (scratch_bytes < (int64_t)P.total || (!scratch && P.total)) return refuse("4-bit attention: scratch is smaller than lpp_op_kv4_attention_scratch_bytes() says");
     char* w = (char*)scratch;
     Kv4AttnArgs a = {};
     a.k = (const unsigned char*)d_k_cache;
@@ -240,10 +248,10 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.lens = d_lens;
     a.sums_in = d_sums_in;
     a.sums_out = d_sums_out;
-    a.scores = d_sums_out ? (float*)(w + L.scores) : nullptr;
-    a.whole_ml = d_sums_out ? (float2*)(w + L.whole) : nullptr;
-    a.part_ml = (float2*)(w + L.ml);
-    a.part_o = (float*)(w + L.part);
+    a.scores = d_sums_out ? (float*)(w + P.scores) : nullptr;
+    a.whole_ml = d_sums_out ? (float2*)(w + P.whole) : nullptr;
+    a.part_ml = (float2*)(w + P.ml);
+    a.part_o = (float*)(w + P.part);
     a.capacity = capacity;
     a.q_stride = q_stride;
     a.out_stride = out_stride;
@@ -253,31 +261,28 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.gqa = n_heads / n_kv_heads;
     a.head_size = head_size;
     a.head_tiles = (a.gqa + kKv4Heads - 1) / kKv4Heads;
-    a.runs = runs;
+    a.runs = P.runs;
+    a.cluster = P.cluster;
     a.dtype = dtype;
     a.rate = scale * 1.4426950408889634f;
     return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
                         constexpr int NG = ng.value;
-                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = (227 * 1024) / kKv4Ctas<NG> - 1024 * (NG + 2) - sums;
-                        auto go = [&](auto parts, auto clusters, int stages) {
+                        constexpr int most = (227 * 1024) / kKv4Ctas<NG> - 1024 * (NG + 2);  // shared memory of a CTA beside its fixed arrays
+                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = most - sums;
+                        // as many units in flight as the shared memory holds beside the warps' sums; a short cache has no more
+                        auto go = [&](auto parts, auto clusters) {
                             constexpr auto kernel = kv4_attn_kernel<NG, parts.value == 2, clusters.value == 1>;
-                            a.stages = std::min(stages, room / kKv4StageBytes<NG>);
+                            a.stages = std::min(clusters.value ? kKv4ClusterUnits : kKv4MaxStages, room / kKv4StageBytes<NG>);
                             const int smem = a.stages * kKv4StageBytes<NG> + sums;
-                            if (!allow_smem<kernel>(smem)) return LPP_ERR_CUDA;
-                            return launch_op_cluster(kernel, dim3(clusters.value ? a.cluster * batch * n_kv_heads * a.head_tiles : runs), kKv4Threads, smem,
-                                                     clusters.value ? a.cluster : 1, false, S(stream), a);
+                            if (!allow_smem<kernel>(most)) return LPP_ERR_CUDA;
+                            return launch_op_cluster(kernel, dim3(clusters.value ? P.cluster * batch * n_kv_heads * a.head_tiles : P.runs), kKv4Threads, smem,
+                                                     clusters.value ? P.cluster : 1, false, S(stream), a);
                         };
-                        // a cluster a head where the cache is short and the clusters run at once (with sums: where one has all query heads)
-                        const long long heads = (long long)batch * n_kv_heads * a.head_tiles, units = (capacity + kKv4Unit - 1) / kKv4Unit;
-                        a.cluster = 1;
-                        while (a.cluster < kKv4Cluster && a.cluster < units && 2 * a.cluster * heads <= (long long)sms * kKv4Ctas<NG>) a.cluster *= 2;
-                        if (units <= (long long)kKv4ClusterUnits * a.cluster && heads * a.cluster <= (long long)sms * kKv4Ctas<NG> && !(d_sums_out && a.head_tiles > 1))
-                            return dtype == LPP_F32 ? go(Int<2>(), Int<1>(), kKv4ClusterUnits) : go(Int<1>(), Int<1>(), kKv4ClusterUnits);
-                        // as many units in flight as the shared memory holds beside the warps' sums
-                        const lpp_status st = dtype == LPP_F32 ? go(Int<2>(), Int<0>(), kKv4MaxStages) : go(Int<1>(), Int<0>(), kKv4MaxStages);
+                        if (P.cluster) return dtype == LPP_F32 ? go(Int<2>(), Int<1>()) : go(Int<1>(), Int<1>());
+                        const lpp_status st = dtype == LPP_F32 ? go(Int<2>(), Int<0>()) : go(Int<1>(), Int<0>());
                         if (st != LPP_OK) return st;
                         const long long rows = d_sums_out ? (capacity + kKv4FinishRows - 1) / kKv4FinishRows : 0;
-                        return launch_behind(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + runs) * 4, S(stream), a);
+                        return launch_behind(kv4_finish_kernel<NG>, dim3((unsigned)(a.gqa + rows), n_kv_heads, batch), kKv4FinishThreads, (size_t)(2 * a.gqa + P.runs) * 4, S(stream), a);
                     }));
 }
 

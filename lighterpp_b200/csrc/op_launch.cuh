@@ -43,18 +43,19 @@ lpp_status launch_op_cluster(void (*kernel)(KArgs...), dim3 grid, int threads, s
     cudaLaunchKernelEx(&cfg, kernel, ((KArgs)args)...);
     return chk();
 }
-// Lets a kernel have more than 48 KB of shared memory: once on every device (asked at every launch it is 0.4 us of the host's time).
+// Lets a kernel have `bytes` (the same at every call) of shared memory: once on every device, since asked at every launch it is 0.4 us of
+// the host's time.
 template <auto KERNEL>
-bool allow_smem(size_t bytes) {
-    static std::atomic<size_t> allowed[64];
+bool allow_smem(int bytes) {
+    static std::atomic<bool> allowed[64];
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-    if (allowed[dev].load(std::memory_order_relaxed) >= bytes) return true;
-    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) != cudaSuccess) {
+    if (allowed[dev].load(std::memory_order_relaxed)) return true;
+    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
         (void)cudaGetLastError();
         return false;
     }
-    allowed[dev].store(bytes, std::memory_order_relaxed);
+    allowed[dev].store(true, std::memory_order_relaxed);
     return true;
 }
 template <typename... KArgs, typename... Args>

@@ -284,8 +284,8 @@ def cuda_kv4_attention(d_out, d_q, d_k_cache, d_v_cache, d_lens, scale, d_sums_i
         _want(what, d_sums_out, torch.float32, batch, kv, capacity)
     room = _kv4_scratch_bytes(device, batch, heads, kv, capacity, size, d_sums_out is not None)
     # torch's allocator hands blocks on in stream order, so the scratch may be let go as soon as the work is queued
-    scratch = torch.empty(max(room, 1), dtype=torch.uint8, device=d_q.device)
-    _call(what, _lib().lpp_op_kv4_attention, device, scratch.data_ptr(), room, d_out.data_ptr(), d_q.data_ptr(), d_k_cache.data_ptr(), d_v_cache.data_ptr(), d_lens.data_ptr(),
+    scratch = torch.empty(room, dtype=torch.uint8, device=d_q.device) if room > 0 else None
+    _call(what, _lib().lpp_op_kv4_attention, device, _ptr(scratch), room, d_out.data_ptr(), d_q.data_ptr(), d_k_cache.data_ptr(), d_v_cache.data_ptr(), d_lens.data_ptr(),
           _ptr(d_sums_in), _ptr(d_sums_out), float(scale), batch, heads, kv, capacity, size, outs, qs, _type(what, d_q))
 
 

@@ -223,19 +223,20 @@ def test_the_same_call_gives_the_same_bits(T):
     assert all(T.equal(got[0][0], o) and T.equal(got[0][1], s) for o, s in got[1:])
 
 
+@pytest.mark.parametrize("cap", [640, 4000])
 @pytest.mark.parametrize("scratch_fill", [0, 255])
-def test_captured_replayed_and_on_another_stream(T, scratch_fill):
+def test_captured_replayed_and_on_another_stream(T, scratch_fill, cap):
     """One captured graph follows what lies in its inputs; scratch may hold anything."""
     from lighterpp_b200 import ops
     lib = ops._lib()
-    q, k, v = setup(T, 8, 2, 64, "f16", (640, 640), 640, 9, garbage=False)
-    kc, vc, dl = T.from_numpy(k).cuda(), T.from_numpy(v).cuda(), T.tensor([640, 0], dtype=T.int32, device="cuda")
-    out, sums = T.zeros_like(q), T.zeros((2, 2, 640), device="cuda")
-    n = lib.lpp_op_kv4_attention_scratch_bytes(2, 8, 2, 640, 64, 1)
+    q, k, v = setup(T, 8, 2, 64, "f16", (cap, cap), cap, 9, garbage=False)
+    kc, vc, dl = T.from_numpy(k).cuda(), T.from_numpy(v).cuda(), T.tensor([cap, 0], dtype=T.int32, device="cuda")
+    out, sums = T.zeros_like(q), T.zeros((2, 2, cap), device="cuda")
+    n = lib.lpp_op_kv4_attention_scratch_bytes(2, 8, 2, cap, 64, 1)
     scratch = T.full((n,), scratch_fill, dtype=T.uint8, device="cuda")
 
     def call():
-        st = lib.lpp_op_kv4_attention(ops._ptr(scratch), n, ops._ptr(out), ops._ptr(q), ops._ptr(kc), ops._ptr(vc), ops._ptr(dl), None, ops._ptr(sums), 0.125, 2, 8, 2, 640, 64,
+        st = lib.lpp_op_kv4_attention(ops._ptr(scratch), n, ops._ptr(out), ops._ptr(q), ops._ptr(kc), ops._ptr(vc), ops._ptr(dl), None, ops._ptr(sums), 0.125, 2, 8, 2, cap, 64,
                                       512, 512, 1, ops._s())
         assert st == 0
 
@@ -247,7 +248,7 @@ def test_captured_replayed_and_on_another_stream(T, scratch_fill):
     graph = T.cuda.CUDAGraph()
     with T.cuda.graph(graph):
         call()
-    for lens in ((3, 640), (640, 129), (0, 0)):
+    for lens in ((3, cap), (cap, 129), (0, 0)):
         dl.copy_(T.tensor(lens, dtype=T.int32))
         q.copy_(T.randn_like(q))
         out.fill_(9.0)
@@ -264,12 +265,17 @@ def test_captured_replayed_and_on_another_stream(T, scratch_fill):
 def test_scratch_that_is_too_small_is_refused(T):
     from lighterpp_b200 import ops
     lib = ops._lib()
-    n = lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 640, 64, 0)
-    assert 0 < n < lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 640, 64, 1)
     x = T.zeros(1 << 20, dtype=T.uint8, device="cuda")
     p = ops._ptr(x)
-    assert lib.lpp_op_kv4_attention(p, n - 1, p, p, p, p, p, None, None, 0.1, 1, 8, 2, 640, 64, 512, 512, 1, ops._s()) == 1
-    assert lib.lpp_op_kv4_attention(p, n, p, p, p, p, p, None, p, 0.1, 1, 8, 2, 640, 64, 512, 512, 1, ops._s()) == 1  # sums want more
+
+    def call(scratch, n, cap, sums):
+        return lib.lpp_op_kv4_attention(scratch, n, p, p, p, p, p, None, p if sums else None, 0.1, 1, 8, 2, cap, 64, 512, 512, 1, ops._s())
+
+    short, long = (lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, cap, 64, 0) for cap in (640, 6400))
+    assert short == 0 < long < lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 6400, 64, 1)
+    assert call(p, long - 1, 6400, False) == 1 and call(p, long, 6400, True) == 1 and call(None, long, 6400, False) == 1
+    n = lib.lpp_op_kv4_attention_scratch_bytes(1, 8, 2, 640, 64, 1)
+    assert n >= 640 * 8 * 4 and call(p, n - 1, 640, True) == 1 and call(None, n, 640, True) == 1
 
 
 def evict(T, size, kv, lens, cap, keep, recent, sums, cap_out=None, seed=0):
@@ -318,6 +324,39 @@ def test_evict_of_equal_and_odd_sums(T, kind):
         sums = rng.choice(np.float32([np.inf, -np.inf, np.nan, 1e-45, -1e-45, 3e38, -1.0, 0.0, -0.0]), (1, 2, cap))
     for keep, recent in ((1500, 0), (1500, 700), (3000, 1), (1, 1)):
         evict(T, 64, 2, (n,), cap, keep, recent, sums, seed=keep)
+
+
+def test_evict_captured_and_replayed(T):
+    """The second kernel starts behind the first in a graph too, with other lengths and sums at every replay."""
+    from lighterpp_b200 import ops
+    rng = np.random.default_rng(7)
+    cap, keep, recent, row = 3000, 700, 50, U.row_bytes(128)
+    k = rng.integers(0, 256, (1, 4, cap, row), dtype=np.uint8)
+    kc, sums, lens = T.from_numpy(k).cuda(), T.zeros((1, 4, cap), device="cuda"), T.zeros(1, dtype=T.int32, device="cuda")
+    vc = kc.flip(-1).contiguous()
+    ko, vo, so = T.zeros((1, 4, keep, row), dtype=T.uint8, device="cuda"), T.zeros((1, 4, keep, row), dtype=T.uint8, device="cuda"), T.zeros((1, 4, keep), device="cuda")
+    kept, lo = T.zeros((1, 4, keep), dtype=T.int32, device="cuda"), T.zeros(1, dtype=T.int32, device="cuda")
+
+    def call():
+        ops.cuda_kv4_evict(ko, vo, so, kept, lo, kc, vc, sums, lens, keep, recent)
+
+    side = T.cuda.Stream()
+    side.wait_stream(T.cuda.current_stream())
+    with T.cuda.stream(side):
+        call()
+    T.cuda.current_stream().wait_stream(side)
+    graph = T.cuda.CUDAGraph()
+    with T.cuda.graph(graph):
+        call()
+    for n in (3000, 701, 12, 2999):
+        w = rng.random((1, 4, cap)).astype(np.float32)
+        sums.copy_(T.from_numpy(w))
+        lens.fill_(n)
+        graph.replay()
+        for h in range(4):
+            rows = U.keep_rows(w[0, h], n, keep, recent)
+            assert int(lo) == len(rows) and list(kept[0, h, :len(rows)].cpu().numpy()) == rows
+            assert np.array_equal(ko[0, h, :len(rows)].cpu().numpy(), k[0, h, rows]) and np.array_equal(vo[0, h, :len(rows)].cpu().numpy(), k[0, h, rows][:, ::-1])
 
 
 def test_a_longer_cache_takes_everything(T):

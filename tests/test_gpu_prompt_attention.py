@@ -78,6 +78,19 @@ def test_prompts(T, name, lengths, heads, kv, size, behind):
     assert bool((out[n:] == 9.0).all())
 
 
+def test_more_prompts_than_shared_memory_holds_offsets(T):
+    from lighterpp_b200 import ops
+    rng = np.random.default_rng(0)
+    lengths = tuple(int(x) for x in rng.integers(0, 4, 1500)) + (300, 0, 5)
+    n = sum(lengths)
+    q, k, v = inputs(T, n + 3, 2, 1, 64, "f16", 2)
+    out = T.full_like(q, 9.0)
+    ops.cuda_prompt_attention(out, q, k, v, offsets(T, lengths), 0.125)
+    want, bound = reference(T, q[:n], k[:n], v[:n], lengths, 0.125)
+    close(T, out[:n], want, bound)
+    assert bool((out[n:] == 9.0).all())
+
+
 @pytest.mark.parametrize("name", ["f16", "bf16"])
 def test_views_of_wider_tensors(T, name):
     """Queries, keys and values as one projection leaves them, results between other columns."""

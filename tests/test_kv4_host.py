@@ -52,7 +52,7 @@ def attention(**kw):
                                                              "qs", "dtype")), None)
 
 
-@pytest.mark.parametrize("wrong", [dict(scratch=0), dict(scratch=P + 128), dict(out=0), dict(q=0), dict(kc=0), dict(vc=0), dict(lens=0), dict(lens=P + 2), dict(so=P + 1),
+@pytest.mark.parametrize("wrong", [dict(scratch=P + 128), dict(out=0), dict(q=0), dict(kc=0), dict(vc=0), dict(lens=0), dict(lens=P + 2), dict(so=P + 1),
                                    dict(si=P), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(heads=7), dict(heads=0), dict(kv=0),
                                    dict(batch=0), dict(cap=62), dict(size=300), dict(os=511), dict(qs=0), dict(dtype=7), dict(q=P + 1), dict(q=P + 2, dtype=0),
                                    dict(heads=4096, kv=2, size=1, os=4096, qs=4096)])
