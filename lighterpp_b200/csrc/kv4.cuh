@@ -133,7 +133,7 @@ static __global__ void __launch_bounds__(kKv4RowThreads, 5) kv4_write_kernel(con
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
     inv = scale == 0.f ? 0.f : inv * (1.f / 15.f);  // (0: every code 8)
     // Codes: a fifteenth of (quotient + 8), cut to 0 .. 1, times fifteen and rounded by adding 1.5 2^23.  The quotient is off by less than
-    // 2^-17; where one came within 2^-13 of a border the thread looks at its values again.
+    // 2^-17; where one came within twice that of a border the thread looks at its values again.
     uint32_t word[2] = {0u, 0u};
     float worst = 0.f;
 #pragma unroll
@@ -146,13 +146,13 @@ static __global__ void __launch_bounds__(kKv4RowThreads, 5) kv4_write_kernel(con
     }
 #pragma unroll
     for (int w = 0; w < 2; ++w) word[w] -= 0x3f400000u;  // what 1.5 2^23 put there eight times, 4 bits apart
-    if (worst > 0.49987f) {
+    if (worst > 0.499985f) {
         float from = zero;
         asm volatile("" : "+f"(from));  // (quotients are made again here, not kept from above)
 #pragma unroll
         for (int j = 0; j < kKv4Each; ++j) {
             const float u = fminf(fmaxf(__fmaf_rn(__fsub_rn(x[j], from), inv * 15.f, 8.f), 0.f), 15.f);
-            if (fabsf(u - rintf(u)) > 0.4998f) word[j / 8] = (word[j / 8] & ~(15u << (4 * (j % 8)))) | min(kv4_border(x[j], zero, scale, u), 15u) << (4 * (j % 8));
+            if (fabsf(u - rintf(u)) > 0.49996f) word[j / 8] = (word[j / 8] & ~(15u << (4 * (j % 8)))) | min(kv4_border(x[j], zero, scale, u), 15u) << (4 * (j % 8));
         }
     }
     if (n < (WIDE ? 1 : kKv4Each)) {  // dimensions that the head does not have: code 8
@@ -967,6 +967,21 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
         }
     }
     pdl_wait();
+    // rows of four scores are on their way while the references are put together
+    constexpr int kRows = kKv4FinishRows / kKv4FinishThreads;
+    const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
+    const bool four = a.gqa == 4;
+    auto own = [&](int j) { return row_block * kKv4FinishRows + tid + j * kKv4FinishThreads; };
+    float4 early[kRows];
+    float before_in[kRows] = {};
+    if (row_block >= 0 && four) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j)
+            if (own(j) < len) {
+                early[j] = *reinterpret_cast<const float4*>(a.scores + (row0 + own(j)) * 4);
+                if (a.sums_in) before_in[j] = a.sums_in[row0 + own(j)];
+            }
+    }
     // reference and sum of the head, or of all heads where their probabilities are wanted
     for (int h = row_block < 0 ? (int)blockIdx.x + warp : warp; h < (row_block < 0 ? (int)blockIdx.x + 1 : a.gqa); h += kKv4FinishThreads / 32) {
         runs_of(h / kKv4Heads, r0, r1);
@@ -1022,22 +1037,20 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
         }
         return;
     }
-    const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
-    const int end = (int)min((long long)len, (long long)(row_block + 1) * kKv4FinishRows);
-    for (int p = row_block * kKv4FinishRows + tid; p < end; p += kKv4FinishThreads) {
+    if (four) {
+#pragma unroll
+        for (int j = 0; j < kRows; ++j)
+            if (own(j) < len) {
+                const float sum = fmaf(exp2_fast(early[j].x - s_fin[0]), s_fin[1], fmaf(exp2_fast(early[j].y - s_fin[2]), s_fin[3], fmaf(exp2_fast(early[j].z - s_fin[4]), s_fin[5],
+                                       exp2_fast(early[j].w - s_fin[6]) * s_fin[7])));
+                a.sums_out[row0 + own(j)] = before_in[j] + sum;
+            }
+        return;
+    }
+    for (int p = own(0); p < min(len, (row_block + 1) * kKv4FinishRows); p += kKv4FinishThreads) {
         const float* x = a.scores + (row0 + p) * a.gqa;
         float sum = 0.f;
-        if (a.gqa % 4 == 0) {
-            for (int h = 0; h < a.gqa; h += 4) {
-                const float4 v = *reinterpret_cast<const float4*>(x + h);
-                sum = fmaf(exp2_fast(v.x - s_fin[2 * h]), s_fin[2 * h + 1], sum);
-                sum = fmaf(exp2_fast(v.y - s_fin[2 * h + 2]), s_fin[2 * h + 3], sum);
-                sum = fmaf(exp2_fast(v.z - s_fin[2 * h + 4]), s_fin[2 * h + 5], sum);
-                sum = fmaf(exp2_fast(v.w - s_fin[2 * h + 6]), s_fin[2 * h + 7], sum);
-            }
-        } else {
-            for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - s_fin[2 * h]), s_fin[2 * h + 1], sum);
-        }
+        for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - s_fin[2 * h]), s_fin[2 * h + 1], sum);
         a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
     }
 }
