@@ -2,7 +2,8 @@
 // it back, attends to it and makes it shorter.  Device pointers in and out, nothing synchronised or allocated; scratch comes from the
 // caller and may hold anything.
 #include <cuda_runtime.h>
-#include <stdio.h>
+#include <stdint.h>
+#include <string.h>
 
 #include "../../include/lpp_b200.h"
 #include "common.cuh"
@@ -336,6 +337,44 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
         default: st = move(kv4_move_kernel<uint4, 10>);
     }
     return launched("lpp_op_kv4_evict: the launch failed", st);
+}
+
+lpp_status lpp_op_call(int op, const void* words, int n_words, void* stream) {
+    static const int count[] = {16, 13, 13, 18, 16};
+    if (op < 0 || op > LPP_OP_KV4_EVICT || !words || n_words != count[op]) return refuse("lpp_op_call: no such operator, or another number of arguments");
+    int64_t w[18];
+    memcpy(w, words, (size_t)n_words * 8);
+    auto ptr = [&](int i) { return (void*)(uintptr_t)w[i]; };
+    bool fits = true;
+    auto num = [&](int i) {
+        fits = fits && w[i] >= INT32_MIN && w[i] <= INT32_MAX;
+        return (int)w[i];
+    };
+    auto real = [&](int i) {
+        double d;
+        memcpy(&d, &w[i], 8);
+        return (float)d;
+    };
+    // (the numbers are looked at before the call: arguments of one are evaluated in no order)
+    static const unsigned numbers[] = {0x83e0u, 0x12e0u, 0x12e0u, 0x25c00u, 0xe600u};
+    for (int i = 0; i < n_words; ++i)
+        if (numbers[op] >> i & 1u) num(i);
+    if (!fits) return refuse("lpp_op_call: a number does not fit 32 bits");
+    switch (op) {
+        case LPP_OP_PROMPT_ATTENTION:
+            return lpp_op_prompt_attention(ptr(0), ptr(1), ptr(2), ptr(3), (const int*)ptr(4), num(5), num(6), num(7), num(8), num(9), w[10], w[11], w[12], w[13], real(14), num(15),
+                                           stream);
+        case LPP_OP_KV4_WRITE:
+            return lpp_op_kv4_write(ptr(0), ptr(1), ptr(2), ptr(3), (const int64_t*)ptr(4), num(5), num(6), num(7), w[8], num(9), w[10], w[11], num(12), stream);
+        case LPP_OP_KV4_READ:
+            return lpp_op_kv4_read(ptr(0), ptr(1), ptr(2), ptr(3), (const int64_t*)ptr(4), num(5), num(6), num(7), w[8], num(9), w[10], w[11], num(12), stream);
+        case LPP_OP_KV4_ATTENTION:
+            return lpp_op_kv4_attention(ptr(0), w[1], ptr(2), ptr(3), ptr(4), ptr(5), (const int*)ptr(6), (const float*)ptr(7), (float*)ptr(8), real(9), num(10), num(11), num(12), w[13],
+                                        num(14), w[15], w[16], num(17), stream);
+        default:
+            return lpp_op_kv4_evict(ptr(0), ptr(1), (float*)ptr(2), (int*)ptr(3), (int*)ptr(4), ptr(5), ptr(6), (const float*)ptr(7), (const int*)ptr(8), num(9), num(10), w[11], w[12],
+                                    num(13), num(14), num(15), stream);
+    }
 }
 
 }  // extern "C"

@@ -44,7 +44,7 @@ EXPORTS = [
     "lpp_op_aggregation_multihead", "lpp_op_residual_add", "lpp_op_scatter_kv", "lpp_op_multihead_gemv",
     "lpp_op_rope_scatter", "lpp_op_sample", "lpp_op_sample_on",
     "lpp_op_sample_scratch_bytes", "lpp_op_sample_static",
-    "lpp_op_prompt_attention", "lpp_op_kv4_row_bytes", "lpp_op_kv4_write", "lpp_op_kv4_read", "lpp_op_kv4_attention_scratch_bytes", "lpp_op_kv4_attention", "lpp_op_kv4_evict",
+    "lpp_op_prompt_attention", "lpp_op_kv4_row_bytes", "lpp_op_kv4_write", "lpp_op_kv4_read", "lpp_op_kv4_attention_scratch_bytes", "lpp_op_kv4_attention", "lpp_op_kv4_evict", "lpp_op_call",
 ]
 
 

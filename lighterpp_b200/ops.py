@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import struct
 
 import torch
 
@@ -61,6 +62,7 @@ def _bind():
         lib.lpp_op_kv4_attention_scratch_bytes.argtypes = [i, i, i, i64, i, i]
         lib.lpp_op_kv4_attention_scratch_bytes.restype = i64
         lib.lpp_op_kv4_attention.argtypes = [vp, i64, vp, vp, vp, vp, vp, vp, vp, f, i, i, i, i64, i, i64, i64, i, vp]
+        lib.lpp_op_call.argtypes = [i, C.c_char_p, i, vp]
         lib.lpp_op_kv4_evict.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, i, i, i64, i64, i, i, i, vp]
         lib._ops_bound = True
     _bound = lib
@@ -142,33 +144,33 @@ def cuda_sample(d_logits, vocab_size, temperature, penalty, d_history, history_l
 # ---- operators beyond the reference's: sizes come from the tensors, work is queued on the current stream of their device.  One
 # sequence's (or token's) heads lie behind one another; from one to the next there may be a gap (a view of a wider tensor).
 #
-# A small call takes the GPU less time than the host, so the checks here look at every tensor once.  (With a device guard around every
-# call, sizes asked of the library each time and shapes compared as tuples a call took 22 - 26 us of host time.)
+# A small call takes the GPU less time than the host: checks look at every tensor once, and arguments travel as one block.  (With a device
+# guard around every call, sizes asked of the library each time, shapes compared as tuples and 18 arguments through ctypes a call took 22 -
+# 26 us of host time; now 7.5 - 11.5.)
 
 _DTYPES = {torch.float32: LPP_F32, torch.float16: LPP_F16, torch.bfloat16: LPP_BF16}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
+# (number of the operator, its arguments as 64-bit words: pointers, integers, a factor) as lpp_op_call takes them
+_PROMPT_ATTENTION, _KV4_WRITE, _KV4_READ, _KV4_ATTENTION, _KV4_EVICT = ((i, struct.Struct(f)) for i, f in enumerate(("=5Q9qdq", "=5Q8q", "=5Q8q", "=Qq7Qd8q", "=9Q7q")))
+
+
 def _call(what, entry, device, *args):
     """Queues the call on the current stream of ``device``."""
+    op, words = entry
+    lib = _bound or _bind()
     if torch.cuda.current_device() == device:
-        st = entry(*args, _raw_stream(device))
+        st = lib.lpp_op_call(op, words.pack(*args), words.size >> 3, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            st = entry(*args, _raw_stream(device))
+            st = lib.lpp_op_call(op, words.pack(*args), words.size >> 3, _raw_stream(device))
     if st:
         _check(st, what)
 
 
-def _device(what, *tensors):
-    """The one device of all ``tensors`` (None: left out)."""
-    device = tensors[0].get_device()
-    for t in tensors:
-        if t is not None and t.get_device() != device:
-            device = -1
-    if device < 0:
-        raise ValueError(f"{what}: expected CUDA tensors on one device")
-    return device
+def _no_device(what):
+    raise ValueError(f"{what}: expected CUDA tensors on one device")
 
 
 def _want(what, t, dtype, *shape):
@@ -196,7 +198,7 @@ def _type(what, t):
 
 
 def _ptr(t):
-    return t.data_ptr() if t is not None else None
+    return t.data_ptr() if t is not None else 0
 
 
 def _cache(what, k, v, head_size):
@@ -212,7 +214,9 @@ def cuda_prompt_attention(d_out, d_q, d_k, d_v, d_offsets, scale):
     """Causal attention of packed prompts: ``d_q``, ``d_out`` [tokens, heads, head_size], ``d_k``, ``d_v`` [tokens, kv heads, head_size] (F16
     or BF16); ``d_offsets`` (int32, prompts + 1) has the first token of each prompt and the end of the last.  Tokens behind are left as they were."""
     what = "cuda_prompt_attention"
-    device = _device(what, d_q, d_out, d_k, d_v, d_offsets)
+    device = d_q.get_device()
+    if not 0 <= device == d_out.get_device() == d_k.get_device() == d_v.get_device() == d_offsets.get_device():
+        _no_device(what)
     dtype, shape, kv_shape = d_q.dtype, d_q.shape, d_k.shape
     qs, outs = _heads(what, d_q, dtype, shape), _heads(what, d_out, dtype, shape)
     ks, vs = _heads(what, d_k, dtype, kv_shape), _heads(what, d_v, dtype, kv_shape)
@@ -221,7 +225,7 @@ def cuda_prompt_attention(d_out, d_q, d_k, d_v, d_offsets, scale):
         raise ValueError(f"{what}: as many keys as queries, of one head size, and offsets of prompts + 1")
     prompts = d_offsets.shape[0] - 1
     _want(what, d_offsets, torch.int32, prompts + 1)
-    _call(what, _lib().lpp_op_prompt_attention, device, d_out.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_offsets.data_ptr(), prompts, n, heads, kv_shape[1],
+    _call(what, _PROMPT_ATTENTION, device, d_out.data_ptr(), d_q.data_ptr(), d_k.data_ptr(), d_v.data_ptr(), d_offsets.data_ptr(), prompts, n, heads, kv_shape[1],
           size, outs, qs, ks, vs, float(scale), _type(what, d_q))
 
 
@@ -235,7 +239,9 @@ def kv4_row_bytes(head_size):
 
 
 def _kv4_rows(what, entry, first, second, k, v, caches, slots):
-    device = _device(what, k, v, slots, *caches)
+    device = k.get_device()
+    if not 0 <= device == v.get_device() == slots.get_device() == caches[0].get_device() == caches[1].get_device():
+        _no_device(what)
     shape = k.shape
     ks, vs = _heads(what, k, k.dtype, shape), _heads(what, v, k.dtype, shape)
     n, heads, size = shape
@@ -251,13 +257,13 @@ def cuda_kv4_write(d_k_cache, d_v_cache, d_k, d_v, d_slots):
     """Rows ``d_k``, ``d_v`` [tokens, kv heads, head_size] into the 4-bit cache at ``d_slots`` (int64; sequence * capacity + position,
     all different; a token whose slot is negative, or beyond the cache, is left out)."""
     caches, rows = (d_k_cache, d_v_cache), (d_k, d_v)
-    _kv4_rows("cuda_kv4_write", _lib().lpp_op_kv4_write, caches, rows, d_k, d_v, caches, d_slots)
+    _kv4_rows("cuda_kv4_write", _KV4_WRITE, caches, rows, d_k, d_v, caches, d_slots)
 
 
 def cuda_kv4_read(d_k, d_v, d_k_cache, d_v_cache, d_slots):
     """The values that the cache holds at ``d_slots``; a token whose slot is negative, or beyond the cache, is left as it was."""
     caches, rows = (d_k_cache, d_v_cache), (d_k, d_v)
-    _kv4_rows("cuda_kv4_read", _lib().lpp_op_kv4_read, rows, caches, d_k, d_v, caches, d_slots)
+    _kv4_rows("cuda_kv4_read", _KV4_READ, rows, caches, d_k, d_v, caches, d_slots)
 
 
 @functools.lru_cache(maxsize=None)
@@ -270,7 +276,9 @@ def cuda_kv4_attention(d_out, d_q, d_k_cache, d_v_cache, d_lens, scale, d_sums_i
     """Attention of one token per sequence, ``d_q`` [batch, heads, head_size], over the first ``d_lens`` (int32) positions of the 4-bit
     cache.  ``d_sums_out`` [batch, kv heads, capacity] (FP32) = ``d_sums_in`` (None: zeros) + the softmax summed over a key/value head's queries."""
     what = "cuda_kv4_attention"
-    device = _device(what, d_q, d_out, d_k_cache, d_v_cache, d_lens, d_sums_in, d_sums_out)
+    device = d_q.get_device()
+    if not 0 <= device == d_out.get_device() == d_k_cache.get_device() == d_v_cache.get_device() == d_lens.get_device():
+        _no_device(what)
     dtype, shape = d_q.dtype, d_q.shape
     qs, outs = _heads(what, d_q, dtype, shape), _heads(what, d_out, dtype, shape)
     n, heads, size = shape
@@ -278,14 +286,15 @@ def cuda_kv4_attention(d_out, d_q, d_k_cache, d_v_cache, d_lens, scale, d_sums_i
     _want(what, d_lens, torch.int32, n)
     if batch != n:
         raise ValueError(f"{what}: one query token per sequence of the cache")
-    if d_sums_in is not None:
-        _want(what, d_sums_in, torch.float32, batch, kv, capacity)
-    if d_sums_out is not None:
-        _want(what, d_sums_out, torch.float32, batch, kv, capacity)
+    for sums in (d_sums_in, d_sums_out):
+        if sums is not None:
+            if sums.get_device() != device:
+                _no_device(what)
+            _want(what, sums, torch.float32, batch, kv, capacity)
     room = _kv4_scratch_bytes(device, batch, heads, kv, capacity, size, d_sums_out is not None)
     # torch's allocator hands blocks on in stream order, so the scratch may be let go as soon as the work is queued
     scratch = torch.empty(room, dtype=torch.uint8, device=d_q.device) if room > 0 else None
-    _call(what, _lib().lpp_op_kv4_attention, device, _ptr(scratch), room, d_out.data_ptr(), d_q.data_ptr(), d_k_cache.data_ptr(), d_v_cache.data_ptr(), d_lens.data_ptr(),
+    _call(what, _KV4_ATTENTION, device, _ptr(scratch), room, d_out.data_ptr(), d_q.data_ptr(), d_k_cache.data_ptr(), d_v_cache.data_ptr(), d_lens.data_ptr(),
           _ptr(d_sums_in), _ptr(d_sums_out), float(scale), batch, heads, kv, capacity, size, outs, qs, _type(what, d_q))
 
 
@@ -296,7 +305,10 @@ def cuda_kv4_evict(d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_k_cache, 
     """Moves ``keep`` rows of every head into a shorter cache: the ``recent`` last ones and those with the largest ``d_sums``.  ``d_kept``
     [batch, kv heads, keep] (int32) gets their old positions, ``d_lens_out`` (int32) the new lengths."""
     what, keep, recent = "cuda_kv4_evict", int(keep), int(recent)
-    device = _device(what, d_k_cache, d_v_cache, d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_sums, d_lens)
+    device = d_k_cache.get_device()
+    if not 0 <= device == d_v_cache.get_device() == d_k_out.get_device() == d_v_out.get_device() == d_sums_out.get_device() == d_kept.get_device() \
+            == d_lens_out.get_device() == d_sums.get_device() == d_lens.get_device():
+        _no_device(what)
     if not _KV4_SIZES:
         _KV4_SIZES.update((kv4_row_bytes(s), s) for s in (32, 64, 96, 128, 256))
     size = _KV4_SIZES.get(d_k_cache.shape[-1], 0)  # (rows are moved whole)
@@ -311,5 +323,5 @@ def cuda_kv4_evict(d_k_out, d_v_out, d_sums_out, d_kept, d_lens_out, d_k_cache, 
     _want(what, d_kept, torch.int32, batch, kv, keep)
     _want(what, d_lens, torch.int32, batch)
     _want(what, d_lens_out, torch.int32, batch)
-    _call(what, _lib().lpp_op_kv4_evict, device, d_k_out.data_ptr(), d_v_out.data_ptr(), d_sums_out.data_ptr(), d_kept.data_ptr(), d_lens_out.data_ptr(), d_k_cache.data_ptr(),
+    _call(what, _KV4_EVICT, device, d_k_out.data_ptr(), d_v_out.data_ptr(), d_sums_out.data_ptr(), d_kept.data_ptr(), d_lens_out.data_ptr(), d_k_cache.data_ptr(),
           d_v_cache.data_ptr(), d_sums.data_ptr(), d_lens.data_ptr(), batch, kv, capacity, capacity_out, size, keep, recent)

@@ -80,6 +80,39 @@ def test_evict_refused(wrong):
     assert evict(**wrong) == 1
 
 
+def test_arguments_as_words_are_the_same_call():
+    """The block of words reaches the same refusals; a wrong number of words, or a number beyond 32 bits, is one."""
+    lib = ops._lib()
+
+    def words(entry, *args, n=None):
+        op, fmt = entry
+        return lib.lpp_op_call(op, fmt.pack(*args), fmt.size // 8 if n is None else n, None)
+
+    rows_ok = (P, 2 * P, 3 * P, 4 * P, 5 * P, 2, 2, 2, 64, 64, 128, 128, 1)
+    for i, bad in ((0, 0), (2, P + 1), (4, P + 4), (5, -1), (6, 0), (7, 0), (8, 66), (9, 257), (10, 127), (11, 0), (12, 3)):
+        args = list(rows_ok)
+        args[i] = bad
+        assert words(ops._KV4_WRITE, *args) == 1
+    assert words(ops._KV4_READ, P, 2 * P, 3 * P, 4 * P, 5 * P, 0, 2, 2, 64, 64, 128, 128, 1) == 0  # no rows
+    assert words(ops._KV4_READ, P, 2 * P, 3 * P, 4 * P, 5 * P, 1 << 32, 2, 2, 64, 64, 128, 128, 1) == 1
+    assert words(ops._KV4_WRITE, *rows_ok, n=12) == 1 and lib.lpp_op_call(5, b"", 0, None) == 1 and lib.lpp_op_call(-1, b"", 0, None) == 1
+    attn = [P, 1 << 40, 2 * P, 3 * P, 4 * P, 5 * P, 6 * P, 0, 0, 0.1, 2, 8, 2, 64, 64, 512, 512, 1]
+    for i, bad in ((0, P + 128), (2, 0), (6, P + 2), (7, P), (9, -1.0), (9, float("nan")), (11, 7), (13, 62), (14, 300), (15, 511), (17, 7), (17, 1 << 33)):
+        args = list(attn)
+        args[i] = bad
+        assert words(ops._KV4_ATTENTION, *args) == 1
+    ev = [P, 2 * P, 3 * P, 4 * P, 5 * P, 6 * P, 7 * P, 8 * P, 9 * P, 1, 2, 64, 32, 64, 20, 5]
+    for i, bad in ((0, 6 * P), (3, 0), (11, 66), (12, 18), (13, 0), (14, 33), (15, 21)):
+        args = list(ev)
+        args[i] = bad
+        assert words(ops._KV4_EVICT, *args) == 1
+    prompt = [P, 2 * P, 3 * P, 4 * P, 5 * P, 2, 10, 4, 2, 64, 256, 256, 128, 128, 0.1, 1]
+    for i, bad in ((0, 0), (5, -1), (7, 5), (9, 12), (10, 255), (13, 0), (14, 0.0), (15, 0)):
+        args = list(prompt)
+        args[i] = bad
+        assert words(ops._PROMPT_ATTENTION, *args) == 1
+
+
 def test_tensors_of_the_host_are_refused():
     import torch
     z = torch.zeros(1, 2, 64, 40, dtype=torch.uint8)
