@@ -39,9 +39,9 @@ struct Kv4Cache {
 
 // ------------------------------------------------------------------ writing and reading rows
 //
-// Two threads a group, sixteen dimensions (two 32-bit words of codes) each.  Bound by the instructions on the way in (about 20 an element; eight
-// elements a thread, conversions by the conversion unit and 64-bit divisions: 34 us for 8001 tokens of 8 heads of 128 where this takes 16), by the bytes of the values on
-// the way out.
+// Two threads a group, sixteen dimensions (two 32-bit words of codes) each.  Bound by the instructions on the way in (about 20 an element:
+// 8001 tokens of 8 heads of 128, keys and values, 16 us, 2.7 TB/s; with eight elements a thread, conversions by the conversion unit and
+// 64-bit divisions 34), by the bytes of the values and their latency on the way out (10 us, 4.2 TB/s).
 
 constexpr int kKv4RowThreads = 256, kKv4Each = 16;  // kKv4Each: dimensions of a thread
 
@@ -231,7 +231,6 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
     return r;
 }
 
-
 // ------------------------------------------------------------------ attention of one token per sequence
 //
 // out = sum_j p_j v_j, p = softmax(scale q . k_j) over the positions below the sequence's length.  Units of 128 positions of one
@@ -244,12 +243,17 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
 // n 2^-24, and the same bits four places up are 16 n 2^-24, so a mask makes two elements of an operand register (the query elements of
 // the second kind are divided by 16).  Sums are kept apart by group and multiplied with the group's scale in FP32:
 //     q . k = sum_g scale_g sum_d q_d n_d + (zero_g - 8 scale_g) Q_g,  Q_g = sum_d q_d;
-// the second part is one more product, of the (scale, zero) pairs as they lie in the row with (-8 Q_g, Q_g), Q_g as two FP16 operands.  For the values the scale goes to the probability before that is rounded to FP16, the codes
-// become n - 8 (rounding errors then are those of values around their middle), and sum_j p_j zero_jg is added in FP32.
+// the second part is one more product, of the (scale, zero) pairs as they lie in the row with (-8 Q_g, Q_g), Q_g as two FP16
+// operands.  For the values the scale goes to the probability before that is rounded to FP16, the codes become n - 8 (rounding errors then
+// are those of values around their middle), and sum_j p_j zero_jg is added in FP32.
 //
 // Reference of the exponentials: not the running maximum of the scores but a bound on the largest p * scale, which has to stay in the
 // FP16 range: probabilities are 2^(x - M) with M far enough below the largest x + log2(scale) seen when M was set that they keep their
 // bits, and M moves only when a product would leave the range.  So a tile needs no maximum over lanes, only a vote.
+//
+// Bound by the instructions around the products, about 400 a warp for 16 positions of 128 dimensions: 131071 positions of eight heads are
+// 24 us of issue slots, their 168 MB 26 us.  Four warps a scheduler fill 63 % of the slots: 43.5 us (3.9 TB/s); 32769 positions with sums
+// 23 us, of which starting and merging take 5 and the second kernel 4.
 //
 // SPLIT: FP32 queries and FP32 results go in as two FP16 operands each (hi + lo), the sums of either added up, and the keys' codes are
 // n - 8 too, with (0, Q_g): sums of n and 8 Q_g that cancel would cost two bits of the scores.
@@ -572,363 +576,363 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     magic.hide();
 
     while (CLUSTER || b < p_end.b || (b == p_end.b && (head < p_end.head || (head == p_end.head && unit < p_end.unit)))) {
-    const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
-    const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
-    const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
-    const int mine = (b == p_end.b && head == p_end.head ? p_end.unit : units) - unit, p1 = len;
-    // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^6 .. 2^7 (eight times
-    // their sums over a group stay in the FP16 range)
-    uint32_t qf[kParts][NG][4];
-    float rate[2];  // factor of the scores, heads 2 t and 2 t + 1
-    uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of (scale, zero), head g: (-8 Q, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
-    {
-        float x[NG][8], top = 0.f;
-        const bool some = g < n_heads;
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int d = i * 32 + t * 8 + j;
-                x[i][j] = some && d < a.head_size ? load_typed(a.q, (long long)b * a.q_stride + (long long)(h0 + g) * a.head_size + d, a.dtype) : 0.f;
-                top = fmaxf(top, fabsf(x[i][j]));
-            }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // exponents of 2 in two halves, either within the normal range
-        const int e = top > 0.f && top < INFINITY ? 6 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
-        const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
-        float sums[NG];
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16 (SPLIT: none)
-                const bool sixteenth = !SPLIT && (j & 1);
-                const float f = sixteenth ? 1.f / 16.f : 1.f;
-                const float u = x[i][j] * f0 * f1, w = x[i][j + 4] * f0 * f1;
-                const __half2 hi = __floats2half2_rn(u * f, w * f);
-                const float2 hf = __half22float2(hi);
-                qf[0][i][j] = *reinterpret_cast<const uint32_t*>(&hi);
-                sum += (hf.x + hf.y) * (sixteenth ? 16.f : 1.f);
-                if constexpr (SPLIT) {
-                    const __half2 lo = __floats2half2_rn(u * f - hf.x, w * f - hf.y);
-                    const float2 lf = __half22float2(lo);
-                    qf[1][i][j] = *reinterpret_cast<const uint32_t*>(&lo);
-                    sum += lf.x + lf.y;
-                }
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            sums[i] = sum;
-        }
-        // back from the operands' factors: 2^24 / 2^e
-        const float back = __int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * kUnit * a.rate;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int from = (2 * t + j) * 4;
-            rate[j] = __shfl_sync(0xffffffffu, back, from);
-        }
-        float own[NG > 4 ? 2 : 1] = {};
-#pragma unroll
-        for (int i = 0; i < NG; ++i)
-            if ((i & 3) == t) own[i >> 2] = sums[i];
-#pragma unroll
-        for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
-            const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
-            const __half times = __float2half_rn(SPLIT ? 0.f : -8.f);
-            const __half2 both = __halves2half2(__hmul(hi, times), hi), rest = __halves2half2(__hmul(lo, times), lo);
-            zf[0][i] = *reinterpret_cast<const uint32_t*>(&both);
-            zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = *reinterpret_cast<const uint32_t*>(&rest);
-        }
-    }
-
-    float o[2 * NG][4], z[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 2 * NG; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NG; ++i) z[i][0] = z[i][1] = 0.f;
-
-    float* scores = a.scores ? a.scores + (row0 + unit * kKv4Unit + warp * kKv4Tile + g) * a.gqa + tile8 * kKv4Heads + 2 * t : nullptr;
-    auto tile = [&](auto whole, int at) {  // whole: every row lies below the length
-        constexpr bool kWhole = decltype(whole)::value;
-        const bool in0 = kWhole || at + g < p1, in1 = kWhole || at + g + 8 < p1;
-        const uint32_t sk = ring_at + stage * kStage, sv = sk + kStage / 2;
-        // ---- scores of rows g and g + 8
-        float s[4];
+        const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
+        const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
+        const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
+        const int mine = (b == p_end.b && head == p_end.head ? p_end.unit : units) - unit, p1 = len;
+        // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^6 .. 2^7 (eight times
+        // their sums over a group stay in the FP16 range)
+        uint32_t qf[kParts][NG][4];
+        float rate[2];  // factor of the scores, heads 2 t and 2 t + 1
+        uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of (scale, zero), head g: (-8 Q, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
         {
-            uint32_t w[NG][2], p0[NG], p1w[NG];
-            kv4_codes<NG, false>(sk, lane, w);
-            const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
-            kv4_params<NG>(r0, p0);
-            kv4_params<NG>(r1, p1w);
-            // rows of (scale, zero) pairs as they lie there times (-8 Q, Q), or (0, Q)
-            float zacc[4], acc[NG][4];
-            if constexpr (NG > 4) {
-                const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
-                kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1]);
-                kv4_mma_add(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1]);
-            } else {
-                const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
-                kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1]);
-            }
-            // (the groups' chains of products side by side)
+            float x[NG][8], top = 0.f;
+            const bool some = g < n_heads;
 #pragma unroll
-            for (int half = 0; half < 2; ++half)
+            for (int i = 0; i < NG; ++i)
 #pragma unroll
-                for (int gr = 0; gr < NG; ++gr) {
-                    const uint32_t x0 = w[gr][0] >> (8 * half), x1 = w[gr][1] >> (8 * half);
-                    uint32_t a0, a1, a2, a3;
-                    if constexpr (SPLIT)
-                        a0 = kv4_low(x0, magic), a1 = kv4_low(x1, magic), a2 = kv4_high(x0, magic), a3 = kv4_high(x1, magic);
-                    else
-                        a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
-                    if (half == 0)
-                        kv4_mma(acc[gr], a0, a1, a2, a3, qf[0][gr][0], qf[0][gr][1]);
-                    else
-                        kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[0][gr][2], qf[0][gr][3]);
-                    if constexpr (SPLIT) kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[1][gr][2 * half], qf[1][gr][2 * half + 1]);
+                for (int j = 0; j < 8; ++j) {
+                    const int d = i * 32 + t * 8 + j;
+                    x[i][j] = some && d < a.head_size ? load_typed(a.q, (long long)b * a.q_stride + (long long)(h0 + g) * a.head_size + d, a.dtype) : 0.f;
+                    top = fmaxf(top, fabsf(x[i][j]));
                 }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            // exponents of 2 in two halves, either within the normal range
+            const int e = top > 0.f && top < INFINITY ? 6 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
+            const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
+            float sums[NG];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] = zacc[j] * (1.f / kUnit);
+            for (int i = 0; i < NG; ++i) {
+                float sum = 0.f;
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr) {
-                const float s0 = half2_bits_to_float2(p0[gr]).x, s1 = half2_bits_to_float2(p1w[gr]).x;
-                s[0] = fmaf(s0, acc[gr][0], s[0]);
-                s[1] = fmaf(s0, acc[gr][1], s[1]);
-                s[2] = fmaf(s1, acc[gr][2], s[2]);
-                s[3] = fmaf(s1, acc[gr][3], s[3]);
+                for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16 (SPLIT: none)
+                    const bool sixteenth = !SPLIT && (j & 1);
+                    const float f = sixteenth ? 1.f / 16.f : 1.f;
+                    const float u = x[i][j] * f0 * f1, w = x[i][j + 4] * f0 * f1;
+                    const __half2 hi = __floats2half2_rn(u * f, w * f);
+                    const float2 hf = __half22float2(hi);
+                    qf[0][i][j] = *reinterpret_cast<const uint32_t*>(&hi);
+                    sum += (hf.x + hf.y) * (sixteenth ? 16.f : 1.f);
+                    if constexpr (SPLIT) {
+                        const __half2 lo = __floats2half2_rn(u * f - hf.x, w * f - hf.y);
+                        const float2 lf = __half22float2(lo);
+                        qf[1][i][j] = *reinterpret_cast<const uint32_t*>(&lo);
+                        sum += lf.x + lf.y;
+                    }
+                }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+                sums[i] = sum;
             }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] *= rate[j & 1];
-        if constexpr (!kWhole) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (!(j < 2 ? in0 : in1)) s[j] = -INFINITY;
-        }
-        if (a.scores) {
-            if (2 * t + 1 < n_heads && a.gqa % 2 == 0) {
-                if (in0) *reinterpret_cast<float2*>(scores) = make_float2(s[0], s[1]);
-                if (in1) *reinterpret_cast<float2*>(scores + 8 * a.gqa) = make_float2(s[2], s[3]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) scores[(j >> 1) * 8 * a.gqa + (j & 1)] = s[j];
-            }
-            scores += (long long)kKv4Unit * a.gqa;
-        }
-        // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
-        uint32_t vp[2][NG], codes[NG][2];
-        kv4_codes<NG, true>(sv, lane, codes);
-        float top[2];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, vp[r]);
-            if (!(r ? in1 : in0)) {
-#pragma unroll
-                for (int gr = 0; gr < NG; ++gr) vp[r][gr] = 0u;
-            }
-            __half2 most = *reinterpret_cast<const __half2*>(&vp[r][0]);
-#pragma unroll
-            for (int gr = 1; gr < NG; ++gr) most = __hmax2(most, *reinterpret_cast<const __half2*>(&vp[r][gr]));
-            top[r] = fmaxf(__low2float(most), 0x1p-24f);
-        }
-        float p[4];  // (a row beyond the end: 0, or NaN while there is no reference, which the vote takes)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
-        if (__any_sync(0xffffffffu, !(fmaxf(p[0], p[1]) * top[0] <= kKv4Limit) || !(fmaxf(p[2], p[3]) * top[1] <= kKv4Limit))) {
-            // move the reference: the largest product becomes 2^8 .. 2^9
+            // back from the operands' factors: 2^24 / 2^e (finite: beyond, scores are alike, or so far apart that one position wins)
+            const float back = fminf(__int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * a.rate * kUnit, 3.402823466e38f);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                float x = fmaxf(s[j] + (float)(ilogbf(top[0]) - 8), s[j + 2] + (float)(ilogbf(top[1]) - 8));
+                const int from = (2 * t + j) * 4;
+                rate[j] = __shfl_sync(0xffffffffu, back, from);
+            }
+            float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
-                for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
-                const float next = fmaxf(m[j], x), f = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - next);
-                m[j] = next;
-                l[j] *= f;
+            for (int i = 0; i < NG; ++i)
+                if ((i & 3) == t) own[i >> 2] = sums[i];
 #pragma unroll
-                for (int k = 0; k < 2 * NG; ++k) {
-                    o[k][j] *= f;
-                    o[k][j + 2] *= f;
+            for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
+                const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
+                const __half times = __float2half_rn(SPLIT ? 0.f : -8.f);
+                const __half2 both = __halves2half2(__hmul(hi, times), hi), rest = __halves2half2(__hmul(lo, times), lo);
+                zf[0][i] = *reinterpret_cast<const uint32_t*>(&both);
+                zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = *reinterpret_cast<const uint32_t*>(&rest);
+            }
+        }
+
+        float o[2 * NG][4], z[NG][2], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[i][j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) z[i][0] = z[i][1] = 0.f;
+
+        float* scores = a.scores ? a.scores + (row0 + unit * kKv4Unit + warp * kKv4Tile + g) * a.gqa + tile8 * kKv4Heads + 2 * t : nullptr;
+        auto tile = [&](auto whole, int at) {  // whole: every row lies below the length
+            constexpr bool kWhole = decltype(whole)::value;
+            const bool in0 = kWhole || at + g < p1, in1 = kWhole || at + g + 8 < p1;
+            const uint32_t sk = ring_at + stage * kStage, sv = sk + kStage / 2;
+            // ---- scores of rows g and g + 8
+            float s[4];
+            {
+                uint32_t w[NG][2], p0[NG], p1w[NG];
+                kv4_codes<NG, false>(sk, lane, w);
+                const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
+                kv4_params<NG>(r0, p0);
+                kv4_params<NG>(r1, p1w);
+                // rows of (scale, zero) pairs as they lie there times (-8 Q, Q), or (0, Q)
+                float zacc[4], acc[NG][4];
+                if constexpr (NG > 4) {
+                    const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
+                    kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1]);
+                    kv4_mma_add(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1]);
+                } else {
+                    const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
+                    kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1]);
                 }
+                // (the groups' chains of products side by side)
 #pragma unroll
-                for (int k = 0; k < NG; ++k) z[k][j] *= f;
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int gr = 0; gr < NG; ++gr) {
+                        const uint32_t x0 = w[gr][0] >> (8 * half), x1 = w[gr][1] >> (8 * half);
+                        uint32_t a0, a1, a2, a3;
+                        if constexpr (SPLIT)
+                            a0 = kv4_low(x0, magic), a1 = kv4_low(x1, magic), a2 = kv4_high(x0, magic), a3 = kv4_high(x1, magic);
+                        else
+                            a0 = x0 & 0x000f000fu, a1 = x1 & 0x000f000fu, a2 = x0 & 0x00f000f0u, a3 = x1 & 0x00f000f0u;
+                        if (half == 0)
+                            kv4_mma(acc[gr], a0, a1, a2, a3, qf[0][gr][0], qf[0][gr][1]);
+                        else
+                            kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[0][gr][2], qf[0][gr][3]);
+                        if constexpr (SPLIT) kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[1][gr][2 * half], qf[1][gr][2 * half + 1]);
+                    }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) s[j] = zacc[j] * (1.f / kUnit);
+#pragma unroll
+                for (int gr = 0; gr < NG; ++gr) {
+                    const float s0 = half2_bits_to_float2(p0[gr]).x, s1 = half2_bits_to_float2(p1w[gr]).x;
+                    s[0] = fmaf(s0, acc[gr][0], s[0]);
+                    s[1] = fmaf(s0, acc[gr][1], s[1]);
+                    s[2] = fmaf(s1, acc[gr][2], s[2]);
+                    s[3] = fmaf(s1, acc[gr][3], s[3]);
+                }
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
-        }
-        l[0] += p[0] + p[2];
-        l[1] += p[1] + p[3];
-        // ---- values
-        uint32_t pf[kParts][NG][2];  // probabilities times scales as operands: rows as the codes have them
+            for (int j = 0; j < 4; ++j) s[j] *= rate[j & 1];
+            if constexpr (!kWhole) {
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-            const float2 u = half2_bits_to_float2(vp[0][gr]), w = half2_bits_to_float2(vp[1][gr]);
-            z[gr][0] = fmaf(p[2], w.y, fmaf(p[0], u.y, z[gr][0]));
-            z[gr][1] = fmaf(p[3], w.y, fmaf(p[1], u.y, z[gr][1]));
-            const float y0 = p[0] * u.x, y1 = p[1] * u.x, y2 = p[2] * w.x, y3 = p[3] * w.x;
-            const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
-            pf[0][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&ha));
-            pf[0][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
-            if constexpr (SPLIT) {
-                const float2 fa = __half22float2(ha), fb = __half22float2(hb);
-                const __half2 la = __floats2half2_rn(y0 - fa.x, y1 - fa.y), lb = __floats2half2_rn(y2 - fb.x, y3 - fb.y);
-                pf[1][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&la));
-                pf[1][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
+                for (int j = 0; j < 4; ++j)
+                    if (!(j < 2 ? in0 : in1)) s[j] = -INFINITY;
+            }
+            if (a.scores) {
+                if (2 * t + 1 < n_heads && a.gqa % 2 == 0) {
+                    if (in0) *reinterpret_cast<float2*>(scores) = make_float2(s[0], s[1]);
+                    if (in1) *reinterpret_cast<float2*>(scores + 8 * a.gqa) = make_float2(s[2], s[3]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if ((j < 2 ? in0 : in1) && 2 * t + (j & 1) < n_heads) scores[(j >> 1) * 8 * a.gqa + (j & 1)] = s[j];
+                }
+                scores += (long long)kKv4Unit * a.gqa;
+            }
+            // ---- scales and zeros of the values of the same rows; beyond the end the rows may hold anything
+            uint32_t vp[2][NG], codes[NG][2];
+            kv4_codes<NG, true>(sv, lane, codes);
+            float top[2];
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+                kv4_params<NG>(sv + (g + r * 8) * kRow + NG * 16, vp[r]);
+                if (!(r ? in1 : in0)) {
+#pragma unroll
+                    for (int gr = 0; gr < NG; ++gr) vp[r][gr] = 0u;
+                }
+                __half2 most = *reinterpret_cast<const __half2*>(&vp[r][0]);
+#pragma unroll
+                for (int gr = 1; gr < NG; ++gr) most = __hmax2(most, *reinterpret_cast<const __half2*>(&vp[r][gr]));
+                top[r] = fmaxf(__low2float(most), 0x1p-24f);
+            }
+            float p[4];  // (a row beyond the end: 0, or NaN while there is no reference, which the vote takes)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
+            if (__any_sync(0xffffffffu, !(fmaxf(p[0], p[1]) * top[0] <= kKv4Limit) || !(fmaxf(p[2], p[3]) * top[1] <= kKv4Limit))) {
+                // move the reference: the largest product becomes 2^8 .. 2^9
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float x = fmaxf(s[j] + (float)(ilogbf(top[0]) - 8), s[j + 2] + (float)(ilogbf(top[1]) - 8));
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, d));
+                    const float next = fmaxf(m[j], x), f = m[j] == -INFINITY ? 0.f : exp2_fast(m[j] - next);
+                    m[j] = next;
+                    l[j] *= f;
+#pragma unroll
+                    for (int k = 0; k < 2 * NG; ++k) {
+                        o[k][j] *= f;
+                        o[k][j + 2] *= f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) z[k][j] *= f;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p[j] = exp2_fast(s[j] - m[j & 1]);
+            }
+            l[0] += p[0] + p[2];
+            l[1] += p[1] + p[3];
+            // ---- values
+            uint32_t pf[kParts][NG][2];  // probabilities times scales as operands: rows as the codes have them
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr) {
+                const float2 u = half2_bits_to_float2(vp[0][gr]), w = half2_bits_to_float2(vp[1][gr]);
+                z[gr][0] = fmaf(p[2], w.y, fmaf(p[0], u.y, z[gr][0]));
+                z[gr][1] = fmaf(p[3], w.y, fmaf(p[1], u.y, z[gr][1]));
+                const float y0 = p[0] * u.x, y1 = p[1] * u.x, y2 = p[2] * w.x, y3 = p[3] * w.x;
+                const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
+                pf[0][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&ha));
+                pf[0][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
+                if constexpr (SPLIT) {
+                    const float2 fa = __half22float2(ha), fb = __half22float2(hb);
+                    const __half2 la = __floats2half2_rn(y0 - fa.x, y1 - fa.y), lb = __floats2half2_rn(y2 - fb.x, y3 - fb.y);
+                    pf[1][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&la));
+                    pf[1][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
+                }
+            }
+#pragma unroll
+            for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
+                    const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
+                    float(&y)[4] = o[2 * gr + k];
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part) kv4_mma_add(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1]);
+                }
+        };
+        const int unit_end = min(p1, (unit + mine) * kKv4Unit);
+        for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
+            const int at = unit_at + warp * kKv4Tile;
+            ok = ok && kv4_wait(full_at + stage * 8, phase);
+            if (!ok) {  // a copy that never came: the results of this run say so
+                m[0] = m[1] = NAN;
+                s_fail = 1;
+                break;
+            }
+            if (at + kKv4Tile <= p1)
+                tile(std::true_type(), at);
+            else if (at < p1)
+                tile(std::false_type(), at);
+            __syncwarp();
+            // the unit before has been read by all warps but late ones: its place takes the next
+            if (turn == warp && stage_before >= 0) {
+                ok = kv4_wait(empty_at + stage_before * 8, phase_before);
+                if (lane == 0 && ok) request();
+                __syncwarp();
+            }
+            if (lane == 0) kv4_arrive(empty_at + stage * 8);  // (after the request: who makes the next one sees how far it came)
+            turn = (turn + 1) & (kKv4Warps - 1);
+            stage_before = stage;
+            phase_before = phase;
+            if (++stage == a.stages) {
+                stage = 0;
+                phase ^= 1u;
+            }
+        }
+        // ---- the warp's sums over its lanes, then the CTA's over its warps
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
+#pragma unroll
+            for (int k = 0; k < NG; ++k)
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) z[k][j] += __shfl_xor_sync(0xffffffffu, z[k][j], d);
+            if (g == 0) {
+                s_m[warp][2 * t + j] = m[j];
+                s_l[warp][2 * t + j] = l[j];
             }
         }
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
-                const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
-                float(&y)[4] = o[2 * gr + k];
+            for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int part = 0; part < kParts; ++part) kv4_mma_add(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1]);
+                for (int j = 0; j < 4; ++j)  // tile 2 gr + k: rows g and g + 8 are dimensions 4 g + 2 k and the one after
+                    if (2 * t + (j & 1) < n_heads) so[(warp * n_heads + 2 * t + (j & 1)) * kPitch + gr * 32 + 4 * g + 2 * k + (j >> 1)] = o[2 * gr + k][j] + z[gr][j & 1];
+        __syncthreads();
+        const bool whole = unit == 0 && mine == units;  // the head lies in this run; else a part: [1] begins here, [0] began earlier
+        const long long part = (long long)blockIdx.x * 2 + (unit == 0 ? 1 : 0);
+        for (int i = tid; i < n_heads * NG * 32; i += kKv4Threads) {
+            const int h = i / (NG * 32), d = i - h * (NG * 32);
+            float top = -INFINITY, sum = 0.f, y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, s_m[w][h]);
+#pragma unroll
+            for (int w = 0; w < kKv4Warps; ++w) {
+                const float f = s_m[w][h] == -INFINITY ? 0.f : exp2_fast(s_m[w][h] - top);
+                sum = fmaf(f, s_l[w][h], sum);
+                y = fmaf(f, so[(w * n_heads + h) * kPitch + d], y);
             }
-    };
-    const int unit_end = min(p1, (unit + mine) * kKv4Unit);
-    for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
-        const int at = unit_at + warp * kKv4Tile;
-        ok = ok && kv4_wait(full_at + stage * 8, phase);
-        if (!ok) {  // a copy that never came: the results of this run say so
-            m[0] = m[1] = NAN;
-            s_fail = 1;
+            const long long bh = (long long)b * a.heads + h0 + h;
+            if constexpr (CLUSTER) {
+                c_y[i] = y;
+                if (d == 0) {
+                    c_ml[h][0] = top;
+                    c_ml[h][1] = sum;
+                }
+            } else if (!whole) {
+                a.part_o[(part * kKv4Heads + h) * (NG * 32) + d] = y;
+                if (d == 0) a.part_ml[part * kKv4Heads + h] = make_float2(top, sum);
+            } else {
+                if (d < a.head_size) store_typed(a.out, (long long)b * a.out_stride + (long long)(h0 + h) * a.head_size + d, a.dtype, len > 0 ? __fdiv_rn(y, sum) : 0.f);
+                if (d == 0 && a.whole_ml) a.whole_ml[bh] = make_float2(top, sum);
+            }
+        }
+        if constexpr (CLUSTER) {
+            cluster_barrier();  // every CTA's results are there
+            const int rank = blockIdx.x % a.cluster;
+            if (tid < n_heads) {
+                float ml[kKv4Cluster][2], top = -INFINITY, sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < kKv4Cluster; ++c)
+                    if (c < a.cluster) {
+                        const uint32_t at = cluster_map(smem_u32(&c_ml[tid][0]), c);
+                        ml[c][0] = __uint_as_float(kv4_cluster_load(at));
+                        ml[c][1] = __uint_as_float(kv4_cluster_load(at + 4));
+                    }
+#pragma unroll
+                for (int c = 0; c < kKv4Cluster; ++c)
+                    if (c < a.cluster) top = fmaxf(top, ml[c][0]);
+#pragma unroll
+                for (int c = 0; c < kKv4Cluster; ++c)
+                    if (c < a.cluster) {
+                        const float f = ml[c][0] == -INFINITY ? 0.f : exp2_fast(ml[c][0] - top);
+                        c_w[tid][c] = f;
+                        sum = fmaf(f, ml[c][1], sum);
+                    }
+                c_w[tid][kKv4Cluster] = top;
+                c_w[tid][kKv4Cluster + 1] = __fdiv_rn(1.f, sum);
+            }
+            __syncthreads();
+            for (int i = rank * kKv4Threads + tid; i < n_heads * NG * 32; i += a.cluster * kKv4Threads) {
+                const int h = i / (NG * 32), d = i - h * (NG * 32);
+                float y[kKv4Cluster], sum = 0.f;
+#pragma unroll
+                for (int c = 0; c < kKv4Cluster; ++c) y[c] = c < a.cluster ? __uint_as_float(kv4_cluster_load(cluster_map(smem_u32(&c_y[i]), c))) : 0.f;
+#pragma unroll
+                for (int c = 0; c < kKv4Cluster; ++c)
+                    if (c < a.cluster) sum = fmaf(c_w[h][c], y[c], sum);
+                if (d < a.head_size)
+                    store_typed(a.out, (long long)b * a.out_stride + (long long)(h0 + h) * a.head_size + d, a.dtype, len > 0 ? sum * c_w[h][kKv4Cluster + 1] : 0.f);
+            }
+            if (a.sums_out) {  // (up to eight query heads: this CTA has all scores of its positions)
+                for (int p = unit * kKv4Unit + tid; p < min(len, p_end.unit * kKv4Unit); p += kKv4Threads) {
+                    const float* x = a.scores + (row0 + p) * a.gqa;
+                    float sum = 0.f;
+                    for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - c_w[h][kKv4Cluster]), c_w[h][kKv4Cluster + 1], sum);
+                    a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
+                }
+            }
+            cluster_barrier();  // every CTA's shared memory stays until all have read it
             break;
         }
-        if (at + kKv4Tile <= p1)
-            tile(std::true_type(), at);
-        else if (at < p1)
-            tile(std::false_type(), at);
-        __syncwarp();
-        // the unit before has been read by all warps but late ones: its place takes the next
-        if (turn == warp && stage_before >= 0) {
-            ok = kv4_wait(empty_at + stage_before * 8, phase_before);
-            if (lane == 0 && ok) request();
-            __syncwarp();
-        }
-        if (lane == 0) kv4_arrive(empty_at + stage * 8);  // (after the request: who makes the next one sees how far it came)
-        turn = (turn + 1) & (kKv4Warps - 1);
-        stage_before = stage;
-        phase_before = phase;
-        if (++stage == a.stages) {
-            stage = 0;
-            phase ^= 1u;
-        }
-    }
-    // ---- the warp's sums over its lanes, then the CTA's over its warps
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-        for (int d = 4; d < 32; d <<= 1) l[j] += __shfl_xor_sync(0xffffffffu, l[j], d);
-#pragma unroll
-        for (int k = 0; k < NG; ++k)
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) z[k][j] += __shfl_xor_sync(0xffffffffu, z[k][j], d);
-        if (g == 0) {
-            s_m[warp][2 * t + j] = m[j];
-            s_l[warp][2 * t + j] = l[j];
-        }
-    }
-#pragma unroll
-    for (int gr = 0; gr < NG; ++gr)
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j)  // tile 2 gr + k: rows g and g + 8 are dimensions 4 g + 2 k and the one after
-                if (2 * t + (j & 1) < n_heads) so[(warp * n_heads + 2 * t + (j & 1)) * kPitch + gr * 32 + 4 * g + 2 * k + (j >> 1)] = o[2 * gr + k][j] + z[gr][j & 1];
-    __syncthreads();
-    const bool whole = unit == 0 && mine == units;  // the head lies in this run; else a part: [1] begins here, [0] began earlier
-    const long long part = (long long)blockIdx.x * 2 + (unit == 0 ? 1 : 0);
-    for (int i = tid; i < n_heads * NG * 32; i += kKv4Threads) {
-        const int h = i / (NG * 32), d = i - h * (NG * 32);
-        float top = -INFINITY, sum = 0.f, y = 0.f;
-#pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) top = fmaxf(top, s_m[w][h]);
-#pragma unroll
-        for (int w = 0; w < kKv4Warps; ++w) {
-            const float f = s_m[w][h] == -INFINITY ? 0.f : exp2_fast(s_m[w][h] - top);
-            sum = fmaf(f, s_l[w][h], sum);
-            y = fmaf(f, so[(w * n_heads + h) * kPitch + d], y);
-        }
-        const long long bh = (long long)b * a.heads + h0 + h;
-        if constexpr (CLUSTER) {
-            c_y[i] = y;
-            if (d == 0) {
-                c_ml[h][0] = top;
-                c_ml[h][1] = sum;
+        __syncthreads();  // the sums have been read
+        unit += mine;
+        if (unit == units) {
+            unit = 0;
+            if (++head == heads8) {
+                head = 0;
+                if (++b < a.batch) len = kv4_len(a, b);
+                units = kv4_units(len);
             }
-        } else if (!whole) {
-            a.part_o[(part * kKv4Heads + h) * (NG * 32) + d] = y;
-            if (d == 0) a.part_ml[part * kKv4Heads + h] = make_float2(top, sum);
         } else {
-            if (d < a.head_size) store_typed(a.out, (long long)b * a.out_stride + (long long)(h0 + h) * a.head_size + d, a.dtype, len > 0 ? __fdiv_rn(y, sum) : 0.f);
-            if (d == 0 && a.whole_ml) a.whole_ml[bh] = make_float2(top, sum);
+            break;
         }
-    }
-    if constexpr (CLUSTER) {
-        cluster_barrier();  // every CTA's results are there
-        const int rank = blockIdx.x % a.cluster;
-        if (tid < n_heads) {
-            float ml[kKv4Cluster][2], top = -INFINITY, sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < kKv4Cluster; ++c)
-                if (c < a.cluster) {
-                    const uint32_t at = cluster_map(smem_u32(&c_ml[tid][0]), c);
-                    ml[c][0] = __uint_as_float(kv4_cluster_load(at));
-                    ml[c][1] = __uint_as_float(kv4_cluster_load(at + 4));
-                }
-#pragma unroll
-            for (int c = 0; c < kKv4Cluster; ++c)
-                if (c < a.cluster) top = fmaxf(top, ml[c][0]);
-#pragma unroll
-            for (int c = 0; c < kKv4Cluster; ++c)
-                if (c < a.cluster) {
-                    const float f = ml[c][0] == -INFINITY ? 0.f : exp2_fast(ml[c][0] - top);
-                    c_w[tid][c] = f;
-                    sum = fmaf(f, ml[c][1], sum);
-                }
-            c_w[tid][kKv4Cluster] = top;
-            c_w[tid][kKv4Cluster + 1] = __fdiv_rn(1.f, sum);
-        }
-        __syncthreads();
-        for (int i = rank * kKv4Threads + tid; i < n_heads * NG * 32; i += a.cluster * kKv4Threads) {
-            const int h = i / (NG * 32), d = i - h * (NG * 32);
-            float y[kKv4Cluster], sum = 0.f;
-#pragma unroll
-            for (int c = 0; c < kKv4Cluster; ++c) y[c] = c < a.cluster ? __uint_as_float(kv4_cluster_load(cluster_map(smem_u32(&c_y[i]), c))) : 0.f;
-#pragma unroll
-            for (int c = 0; c < kKv4Cluster; ++c)
-                if (c < a.cluster) sum = fmaf(c_w[h][c], y[c], sum);
-            if (d < a.head_size)
-                store_typed(a.out, (long long)b * a.out_stride + (long long)(h0 + h) * a.head_size + d, a.dtype, len > 0 ? sum * c_w[h][kKv4Cluster + 1] : 0.f);
-        }
-        if (a.sums_out) {  // (up to eight query heads: this CTA has all scores of its positions)
-            for (int p = unit * kKv4Unit + tid; p < min(len, p_end.unit * kKv4Unit); p += kKv4Threads) {
-                const float* x = a.scores + (row0 + p) * a.gqa;
-                float sum = 0.f;
-                for (int h = 0; h < a.gqa; ++h) sum = fmaf(exp2_fast(x[h] - c_w[h][kKv4Cluster]), c_w[h][kKv4Cluster + 1], sum);
-                a.sums_out[row0 + p] = (a.sums_in ? a.sums_in[row0 + p] : 0.f) + sum;
-            }
-        }
-        cluster_barrier();  // every CTA's shared memory stays until all have read it
-        break;
-    }
-    __syncthreads();  // the sums have been read
-    unit += mine;
-    if (unit == units) {
-        unit = 0;
-        if (++head == heads8) {
-            head = 0;
-            if (++b < a.batch) len = kv4_len(a, b);
-            units = kv4_units(len);
-        }
-    } else {
-        break;
-    }
     }
     if (s_fail) {  // copies may still be in flight: a bounded time to land
         const long long c0 = clock64();

@@ -11,6 +11,10 @@
 // Sums O are rescaled only when a row's maximum has grown by more than 2^8 since it was last set, by the row's own thread, when the
 // product of the tile before is complete.
 //
+// Measured: 8192 tokens of 32 heads of 128 take 438 us, 1.25 PFLOP/s, bound by the tensor cores under the power cap (without exponentials
+// 435); tensor cores and special functions are busy 60 % of the clocks each.  1023 tokens of 32 heads of 64: 15.5 us, of which the longest row
+// tiles' eight steps take 1.4 us each (exponentials of one warp a scheduler) and start and end 4.  201 tokens of 6 heads of 48: 6.7 us.
+//
 // Sequences do not have to begin at tiles: row tiles cover the packed tokens whatever the borders, a row sees the keys from its
 // sequence's start to itself, and a tile runs over the keys from its first row's sequence on.  Many short prompts share a tile.
 //

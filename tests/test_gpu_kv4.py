@@ -186,6 +186,16 @@ def test_queries_of_any_size(T, name, factor):
     check(T, q, k, v, lens, 1.0 / factor, name)
 
 
+def test_queries_near_the_largest_value(T):
+    """The factor that goes back from the operands to scores is beyond FP32 there."""
+    lens = (333,)
+    q, k, v = setup(T, 4, 1, 64, "bf16", lens, 336, 4)
+    big = (q.float() / q.float().abs().max() * 3e38).to(q.dtype)
+    check(T, big, k, v, lens, 1e-37, "bf16")
+    k[0, :, :333] = U.pack(np.zeros((333, 64)))  # keys of 0: all positions alike
+    check(T, big, k, v, lens, 0.125, "bf16")
+
+
 def test_lengths_beyond_the_capacity_are_cut(T):
     q, k, v = setup(T, 4, 2, 64, "f16", (64, 64), 64, 1)
     from lighterpp_b200 import ops
