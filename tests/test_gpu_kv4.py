@@ -428,3 +428,78 @@ def test_prompt_steps_eviction_and_steps_behind_one_another(T):
     for _ in range(5):
         step(64)
     assert np.all(np.abs(sums.double().cpu().numpy() - ref_sums) <= ref_bound)
+
+
+def test_a_cache_beyond_32_bits(T):
+    """A head's rows, scores and slots far behind the first 2^32 bytes, and more positions than an FP32 sum counts.  All rows are 0 but a few."""
+    from lighterpp_b200 import ops
+    if T.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    rng = np.random.default_rng(12)
+    heads, kv, size, cap, keep, scale = 8, 2, 128, 1 << 26, 64, 0.125
+    n, some = cap - 4, np.array([0, 5, (1 << 25) + 1, cap - 100, cap - 5])
+    kc, vc = (T.zeros((1, kv, cap, U.row_bytes(size)), dtype=T.uint8, device="cuda") for _ in range(2))
+    q = T.from_numpy(rng.standard_normal((1, heads, size)).astype(np.float32)).cuda().half()
+    q64 = q.double().cpu().numpy()[0].reshape(kv, heads // kv, size)
+    k = q64.mean(1)[None] * rng.uniform(4, 6, (len(some), kv, 1))  # keys along a head's queries: scores that some 10^7 others do not hide
+    k, v = (T.from_numpy(x.astype(np.float32)).cuda().half() for x in (k, rng.standard_normal((len(some), kv, size))))
+    slots = T.from_numpy(some).cuda()
+    ops.cuda_kv4_write(kc, vc, k, v, slots)
+    k_rows, v_rows = (U.pack(x.double().cpu().numpy()) for x in (k, v))
+    assert np.array_equal(kc[0][:, slots].transpose(0, 1).cpu().numpy(), k_rows) and np.array_equal(vc[0][:, slots].transpose(0, 1).cpu().numpy(), v_rows)
+    assert T.count_nonzero(kc[0, 1, 1 << 25:]) <= 3 * U.row_bytes(size)
+    back = T.zeros_like(k), T.zeros_like(v)
+    ops.cuda_kv4_read(*back, kc, vc, slots)
+    for x, rows in zip(back, (k_rows, v_rows)):
+        assert np.array_equal(x.cpu().numpy(), U.unpack(rows, size)[0].astype(np.float16))
+    out, sums = T.zeros_like(q), T.zeros((1, kv, cap), device="cuda")
+    ops.cuda_kv4_attention(out, q, kc, vc, T.tensor([n], dtype=T.int32, device="cuda"), scale, sums, sums)
+    u = 2.0 ** -24
+    for h in range(kv):
+        (kh, ks, kz), (vh, _, vz) = U.unpack(k_rows[:, h], size), U.unpack(v_rows[:, h], size)
+        x = q64[h] @ kh.T * scale
+        total = (n - len(some)) + np.exp(x).sum(-1, keepdims=True)
+        p = np.exp(x) / total
+        # a score's rounding as in kv4_util, that of its exponential and of the sum's members; sums of 3542 tiles in a lane (148 SMs, two CTAs each),
+        # five lanes' steps, eight warps and at most 300 parts behind one another
+        dp = 2 * ((size + 16) * u * (np.abs(q64[h]) @ (16 * ks + np.abs(kz)).T) * scale + (np.abs(x).max() + 8) * 2 * u) + 4000 * u
+        want = p @ vh
+        bound = (p * dp) @ (np.abs(vh - vz) + np.abs(vz)) + 2.0 ** -11 * (p @ np.abs(vh - vz))
+        got = out[0, h * 4:h * 4 + 4].double().cpu().numpy()
+        assert np.all(np.abs(got - want) <= bound + 2.0 ** -11 * (np.abs(want) + bound) + 2.0 ** -25)
+        assert np.all(np.abs(sums[0, h, slots].double().cpu().numpy() - p.sum(0)) <= (p * dp).sum(0) + 8 * u * p.sum(0))
+        other = (1 / total).sum()
+        assert abs(float(sums[0, h, cap - 50]) - other) <= (dp.max() + 8 * u) * other
+        assert not sums[0, h, n:].any()
+    ko, vo = (T.zeros((1, kv, keep, U.row_bytes(size)), dtype=T.uint8, device="cuda") for _ in range(2))
+    so, kept, lo = T.zeros((1, kv, keep), device="cuda"), T.zeros((1, kv, keep), dtype=T.int32, device="cuda"), T.zeros(1, dtype=T.int32, device="cuda")
+    ops.cuda_kv4_evict(ko, vo, so, kept, lo, kc, vc, sums, T.tensor([n], dtype=T.int32, device="cuda"), keep, 1)
+    first = sorted(set(range(62)) | {int(s) for s in some})  # all others weigh the same: the lowest positions stay
+    first = [r for r in first if r in some or first.index(r) < 61][:61] + [int(s) for s in some[2:]]
+    for h in range(kv):
+        assert list(kept[0, h].cpu().numpy()) == first
+        at = [first.index(int(s)) for s in some]
+        assert np.array_equal(ko[0, h, at].cpu().numpy(), k_rows[:, h]) and np.array_equal(vo[0, h, at].cpu().numpy(), v_rows[:, h])
+
+
+def test_two_streams_at_once(T):
+    """Calls of either stream have scratch of their own."""
+    from lighterpp_b200 import ops
+    sets = []
+    for seed, lens in ((1, (5000, 9, 2000)), (2, (17, 4097, 4999))):
+        q, k, v = setup(T, 16, 2, 128, "f16", lens, 5000, seed)
+        kc, vc, dl = T.from_numpy(k).cuda(), T.from_numpy(v).cuda(), T.tensor(lens, dtype=T.int32, device="cuda")
+        out, sums = T.zeros_like(q), T.zeros((3, 2, 5000), device="cuda")
+        ops.cuda_kv4_attention(out, q, kc, vc, dl, 0.09, None, sums)
+        sets.append((q, kc, vc, dl, out, sums, T.cuda.Stream()))
+    T.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for q, kc, vc, dl, _, _, stream in sets:
+            with T.cuda.stream(stream):
+                out, sums = T.zeros_like(q), T.zeros((3, 2, 5000), device="cuda")
+                ops.cuda_kv4_attention(out, q, kc, vc, dl, 0.09, None, sums)
+                got.append((out, sums))
+    T.cuda.synchronize()
+    for i, (out, sums) in enumerate(got):
+        assert T.equal(out, sets[i % 2][4]) and T.equal(sums, sets[i % 2][5])

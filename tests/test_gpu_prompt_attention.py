@@ -232,3 +232,25 @@ def test_prompts_into_the_cache_and_on(T):
             p = T.softmax(q[i, h].double() @ K.T * 0.125, -1)
             more = (p * T.expm1(2 * dx)) @ V.abs() + 2.0 ** -11 * (p @ V.abs())
             assert bool(((got[b, h].double() - want[i, h]).abs() <= bound[i, h] + 2 * more + 2.0 ** -10 * (p @ V.abs())).all())
+
+
+def test_strides_beyond_32_bits(T):
+    """Tokens 64 MB apart: the same bits as from tensors without gaps, a value that is not a number among them."""
+    from lighterpp_b200 import ops
+    if T.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    n, heads, kv, size, apart = 130, 4, 2, 64, 1 << 25
+    q, k, v = inputs(T, n, heads, kv, size, "f16", 5)
+    v[100, 1, 7] = float("nan")
+    want = T.zeros_like(q)
+    ops.cuda_prompt_attention(want, q, k, v, offsets(T, (129, 1)), 0.125)
+    room = T.empty(n * apart, dtype=T.float16, device="cuda")
+
+    def place(at, x):
+        view = room.as_strided(x.shape, (apart, size, 1), at)
+        return view.copy_(x)
+
+    views = [place(0, T.zeros_like(q)), place(256, q), place(512, k), place(640, v)]
+    ops.cuda_prompt_attention(*views, offsets(T, (129, 1)), 0.125)
+    assert T.equal(views[0].contiguous().view(T.int16), want.view(T.int16))
+    assert bool(want[100:129, 2:, 7].isnan().all()) and int(want.isnan().sum()) == 29 * 2
