@@ -325,8 +325,9 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
     // CTAs of a head: up to eight (a portable cluster), while they all run at once and have some hundred rows each
     a.cluster = 1;
     while (a.cluster < kKv4EvictCluster && 2ll * a.cluster * (long long)heads <= sms && capacity >= 1024ll * a.cluster) a.cluster *= 2;
-    lpp_status st = launch_op_cluster(kv4_select_kernel, dim3(a.cluster, n_kv_heads, batch), kKv4EvictThreads, 0, a.cluster, false, S(stream), a);
-    if (st != LPP_OK) return launched("lpp_op_kv4_evict: the launch failed", st);
+    const bool few = keep <= kKv4EvictMove * a.cluster;
+    lpp_status st = launch_op_cluster(few ? kv4_select_kernel<true> : kv4_select_kernel<false>, dim3(a.cluster, n_kv_heads, batch), kKv4EvictThreads, 0, a.cluster, false, S(stream), a);
+    if (few || st != LPP_OK) return launched("lpp_op_kv4_evict: the launch failed", st);
     const dim3 grid(blocks(std::min<int64_t>(keep, capacity), kKv4MoveRows), n_kv_heads, batch);
     auto move = [&](auto kernel) { return launch_behind(kernel, grid, kKv4MoveRows, 0, S(stream), a); };
     switch (row / 20) {  // groups of a row

@@ -1065,12 +1065,13 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // equals; a NaN counts as -infinity), in their order.  A cluster of CTAs takes a head, every CTA a run of its rows: the smallest sum that
 // stays is found digit by digit (histograms of 8 bits of the sums' order, every CTA adding up all of the cluster's through distributed
 // shared memory), then every CTA knows where its kept rows begin in the new cache and lists them.  A second kernel, of many small CTAs,
-// moves them: bound by the rows' bytes where they are many, by the meetings of the cluster where they are few.  (Digits of 11 bits added
+// moves many of them: bound by the rows' bytes where they are many, by the meetings of the cluster where they are few.  (Digits of 11 bits added
 // up by remote atomics in one CTA: passes of 3 - 8 us each instead of 1.4.  Rows moved by the cluster that lists them, two sequences of
 // 32768 and 20011 positions to 12000: 30 us, its SMs being too few for the bandwidth; now 26.)
 // 512 threads: two CTAs fit an SM (of 1024, sixteen clusters of eight did not fit the GPU at once, and the last ran alone).
 constexpr int kKv4EvictThreads = 512, kKv4EvictCluster = 8;
 constexpr int kKv4EvictKeep = 8;  // rows of a thread whose ranks stay in registers
+constexpr int kKv4EvictMove = 256;  // new rows a CTA up to which one kernel does it all
 
 struct Kv4EvictArgs {
     const unsigned char *k, *v;
@@ -1088,6 +1089,26 @@ __device__ __forceinline__ uint32_t kv4_rank(float x) {
     const uint32_t u = x != x ? 0xff800000u : __float_as_uint(x + 0.f);  // (-0 becomes 0)
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
+// Rows first .. first + n - 1 of the new cache, by one CTA
+template <typename V, int UNITS>
+__device__ __forceinline__ void kv4_move_rows(const Kv4EvictArgs& a, long long head, int first, int n) {
+    const int* kept = a.kept + head * a.keep + first;
+    const V *k = reinterpret_cast<const V*>(a.k) + head * a.capacity * UNITS, *v = reinterpret_cast<const V*>(a.v) + head * a.capacity * UNITS;
+    V *ko = reinterpret_cast<V*>(a.k_out) + (head * a.capacity_out + first) * UNITS, *vo = reinterpret_cast<V*>(a.v_out) + (head * a.capacity_out + first) * UNITS;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < n * UNITS; i += kKv4EvictThreads) {
+        const int row = i / UNITS;
+        const long long from = (long long)kept[row] * UNITS + (i - row * UNITS);
+        const V x = k[from], y = v[from];
+        ko[i] = x;
+        vo[i] = y;
+    }
+    for (int i = threadIdx.x; i < n; i += kKv4EvictThreads) a.sums_out[head * a.capacity_out + first + i] = a.sums[head * a.capacity + kept[i]];
+}
+// MOVE: the CTAs also move the rows that they list, and there is no second kernel, whose launch takes the host 2.3 us.  For few rows.  (2048
+// to 1024 positions, eight heads: calls behind one another 8.7 us, with two kernels 11; four sequences of 4096 to 1024 in a graph 9.4, 11.7;
+// 32768 to 2048, as many as are moved so, 11.6 and 11.1.)
+template <bool MOVE>
 static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_select_kernel(const Kv4EvictArgs a) {
     __shared__ uint32_t hist[4][256], parts[2][256];  // hist: a pass each
     __shared__ uint32_t counts[kKv4EvictCluster][2], warp_sums[32], s_digit, s_left, s_all;
@@ -1199,6 +1220,7 @@ static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_select_kernel(
     uint32_t at = 0, equal = 0;
     for (int c = 0; c < cta; ++c) at += counts[c][0], equal += counts[c][1];
     at += min(equal, left);
+    const int first = (int)at;
     auto place = [&](int i, uint32_t r) {
         bool more, same;
         judge(i, r, more, same);
@@ -1217,6 +1239,17 @@ static __global__ void __launch_bounds__(kKv4EvictThreads, 2) kv4_select_kernel(
     for (int j = 0; j < kKv4EvictKeep; ++j)
         if (row0 + j * kKv4EvictThreads < row1) place(row0 + tid + j * kKv4EvictThreads, rank[j]);  // (the same for the whole CTA)
     for (int i0 = row0 + kKv4EvictKeep * kKv4EvictThreads; i0 < row1; i0 += kKv4EvictThreads) place(i0 + tid, rank_of(i0 + tid));
+    if constexpr (MOVE) {
+        __syncthreads();  // the list is there
+        const int n = (int)at - first;
+        switch (a.row_bytes) {
+            case kv4_row_bytes(1): kv4_move_rows<uint32_t, 5>(a, head, first, n); break;
+            case kv4_row_bytes(2): kv4_move_rows<uint2, 5>(a, head, first, n); break;
+            case kv4_row_bytes(3): kv4_move_rows<uint32_t, 15>(a, head, first, n); break;
+            case kv4_row_bytes(4): kv4_move_rows<uint4, 5>(a, head, first, n); break;
+            default: kv4_move_rows<uint4, 10>(a, head, first, n);
+        }
+    }
 }
 
 // V: bytes a thread moves at once (16, 8 or 4, by the row's size), UNITS of them a row.  A CTA takes 256 rows, a thread UNITS pieces of the

@@ -320,6 +320,17 @@ def test_evict(T, size, kv, lens, cap, keep, recent):
     evict(T, size, kv, lens, cap, keep, recent, sums)
 
 
+@pytest.mark.parametrize("size", [20, 64, 96, 128, 200])
+@pytest.mark.parametrize("cap,keep,recent", [(600, 256, 20), (600, 257, 20), (2052, 1024, 0), (2052, 1025, 30)])
+def test_evict_of_few_and_of_many_rows(T, size, cap, keep, recent):
+    """Either side of what one kernel moves; sums that leave most of the rows to one end of the cache."""
+    rng = np.random.default_rng(size + keep)
+    sums = rng.random((1, 3, cap)).astype(np.float32)
+    sums[0, 1] *= np.linspace(0, 1, cap) ** 4
+    sums[0, 2] *= np.linspace(1, 0, cap) ** 4
+    evict(T, size, 3, (cap - 1,), cap, keep, recent, sums)
+
+
 @pytest.mark.parametrize("kind", ["equal", "few", "wild", "close"])
 def test_evict_of_equal_and_odd_sums(T, kind):
     rng = np.random.default_rng(4)
@@ -367,6 +378,29 @@ def test_evict_captured_and_replayed(T):
             rows = U.keep_rows(w[0, h], n, keep, recent)
             assert int(lo) == len(rows) and list(kept[0, h, :len(rows)].cpu().numpy()) == rows
             assert np.array_equal(ko[0, h, :len(rows)].cpu().numpy(), k[0, h, rows]) and np.array_equal(vo[0, h, :len(rows)].cpu().numpy(), k[0, h, rows][:, ::-1])
+
+
+def test_evict_of_many_rows_captured_and_replayed(T):
+    from lighterpp_b200 import ops
+    rng = np.random.default_rng(8)
+    cap, keep, row = 4096, 2100, U.row_bytes(64)
+    k = rng.integers(0, 256, (1, 2, cap, row), dtype=np.uint8)
+    kc, sums, lens = T.from_numpy(k).cuda(), T.zeros((1, 2, cap), device="cuda"), T.full((1,), cap, dtype=T.int32, device="cuda")
+    ko, vo, so = T.zeros((1, 2, keep, row), dtype=T.uint8, device="cuda"), T.zeros((1, 2, keep, row), dtype=T.uint8, device="cuda"), T.zeros((1, 2, keep), device="cuda")
+    kept, lo = T.zeros((1, 2, keep), dtype=T.int32, device="cuda"), T.zeros(1, dtype=T.int32, device="cuda")
+    graph = T.cuda.CUDAGraph()
+    ops.cuda_kv4_evict(ko, vo, so, kept, lo, kc, kc, sums, lens, keep, 3)
+    with T.cuda.graph(graph):
+        ops.cuda_kv4_evict(ko, vo, so, kept, lo, kc, kc, sums, lens, keep, 3)
+    for n in (4096, 2101, 5):
+        w = rng.random((1, 2, cap)).astype(np.float32)
+        sums.copy_(T.from_numpy(w))
+        lens.fill_(n)
+        graph.replay()
+        for h in range(2):
+            rows = U.keep_rows(w[0, h], n, keep, 3)
+            assert int(lo) == len(rows) and list(kept[0, h, :len(rows)].cpu().numpy()) == rows
+            assert np.array_equal(ko[0, h, :len(rows)].cpu().numpy(), k[0, h, rows]) and T.equal(ko[0, h, :len(rows)], vo[0, h, :len(rows)])
 
 
 def test_a_longer_cache_takes_everything(T):
