@@ -367,8 +367,9 @@ lpp_status lpp_op_sample_static(float* d_logits, int vocab_size, float temperatu
  * q and out are [token][n_heads][head_size], k and v [token][n_kv_heads][head_size], F16 or BF16, *_stride elements from one token to the
  * next (a multiple of 8, at least a token's elements), on 16-byte boundaries; head sizes are multiples of 8 up to 128.  The arrays hold n_tokens tokens:
  * results of those from d_offsets[n_sequences] on are left as they were, and their queries, keys and values are not looked at.  Scores and
- * sums are FP32, probabilities are rounded to the type.  What is not finite reaches the tokens that see it and no others.  The results
- * overlap none of the inputs. */
+ * sums are FP32, probabilities are rounded to the type.  What is not finite reaches the tokens that see it and no others: an infinite
+ * value makes the results of its dimension infinite, whatever its weight has become, a NaN or both signs no numbers.  The results overlap none
+ * of the inputs. */
 lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k, const void* d_v, const int* d_offsets, int n_sequences, int n_tokens,
                                    int n_heads, int n_kv_heads, int head_size, int64_t out_stride, int64_t q_stride, int64_t k_stride,
                                    int64_t v_stride, float scale, int dtype, void* stream);

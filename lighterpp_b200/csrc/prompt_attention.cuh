@@ -20,7 +20,9 @@
 //
 // Keys of tokens that a row does not see are masked after the product; their values meet probabilities of 0, which hides everything but
 // NaN and infinity.  So two warps look through the value tiles that some row sees only in part, zero what is not finite, and the rows
-// that do see it get it added to their results at the end.
+// that do see it get it added to their results at the end.  In a tile that all rows see it goes through the product, where an infinity whose
+// probability has become 0 leaves a NaN.  So a row whose sum is not finite looks for what it saw (at its end; other rows pay 0.1 us
+// for the look at their sums): an infinity makes a result infinite, a NaN or infinities of both signs make it no number, wherever tiles are cut.
 #pragma once
 #include "common.cuh"
 #include "umma.cuh"
@@ -453,6 +455,7 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
         const bool mine = token < t_end;
         T* dst = reinterpret_cast<T*>(a.out) + (long long)token * a.out_stride + (long long)head * a.head_size;
         const float inv = ok ? __fdiv_rn(1.f, l) : NAN;
+        float lost[4] = {};  // NaN: a sum is not finite
 #pragma unroll
         for (int c = 0; c < HS; c += 32) {
             uint32_t o[32];
@@ -460,6 +463,8 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
             tc_wait_ld();
             pin16(o);
             pin16(o + 16);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) lost[i & 3] = __fmaf_rn(__uint_as_float(o[i]), 0.f, lost[i & 3]);
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
                 if (mine && c + i < a.head_size) {
@@ -482,6 +487,17 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
                 }
             }
         }
+        if (ok && mine && l < INFINITY && !((lost[0] + lost[1]) + (lost[2] + lost[3]) == 0.f))  // (no sum of probabilities: all is NaN)
+            for (int d = 0; d < a.head_size; ++d) {
+                if (fabsf(to_float(dst[d])) < INFINITY) continue;
+                const T* v = reinterpret_cast<const T*>(a.v) + (long long)kvh * a.head_size + d;
+                float seen = 0.f;
+                for (int j = first; j <= i_row && seen == seen; ++j) {
+                    const float y = to_float(v[(long long)j * a.v_stride]);
+                    if (!(fabsf(y) < INFINITY)) seen += y;
+                }
+                if (seen != 0.f) dst[d] = from_float<T>(seen);  // (0: finite values whose sum is beyond the type)
+            }
     }
     // ---------------- common exit
     __syncwarp();

@@ -254,3 +254,46 @@ def test_strides_beyond_32_bits(T):
     ops.cuda_prompt_attention(*views, offsets(T, (129, 1)), 0.125)
     assert T.equal(views[0].contiguous().view(T.int16), want.view(T.int16))
     assert bool(want[100:129, 2:, 7].isnan().all()) and int(want.isnan().sum()) == 29 * 2
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv,size", [(4, 2, 64), (3, 3, 128), (4, 2, 128), (2, 1, 40)])
+@pytest.mark.parametrize("before", [0, 1, 77, 128])
+def test_values_that_are_infinite_whatever_their_weight(T, name, heads, kv, size, before):
+    """An infinite value whose weight has become 0 in the type, and what becomes of it, do not go by where key tiles are cut: results are
+    infinite wherever the prompt lies, not numbers where both signs are seen, and those of other dimensions as without."""
+    from lighterpp_b200 import ops
+    n = 700
+    q, k, v = inputs(T, before + n, heads, kv, size, name, 9)
+    weak = [before + i for i in (0, 5, 126, 200, 399)]
+    q[:, :, 0], k[:, :, 0] = 40.0, 0.0
+    k[weak, :, 0] = -40.0  # their scores lie 288 powers of two below the others
+    lengths = ((before, n) if before else (n,))
+    clean = T.zeros_like(q)
+    ops.cuda_prompt_attention(clean, q, k, v, offsets(T, lengths), 0.125)
+    v[weak[1], 0, 3] = float("inf")
+    v[weak[2], 0, 5] = float("-inf")
+    v[weak[3], 0, 3] = float("-inf")
+    v[weak[4], 0, 7] = float("nan")
+    out = T.zeros_like(q)
+    ops.cuda_prompt_attention(out, q, k, v, offsets(T, lengths), 0.125)
+    want = clean.clone()
+    g = heads // kv
+    want[weak[1]:, :g, 3] = float("inf")
+    want[weak[3]:, :g, 3] = float("nan")
+    want[weak[2]:, :g, 5] = float("-inf")
+    want[weak[4]:, :g, 7] = float("nan")
+    same = (out == want) | (out.isnan() & want.isnan())
+    assert bool(same.all()), (~same).nonzero()[:5].tolist()
+
+
+@pytest.mark.parametrize("name", ["f16", "bf16"])
+def test_values_near_the_largest(T, name):
+    """Finite values near the type's largest: results are their weighted means, which no part on the way takes beyond FP32."""
+    from lighterpp_b200 import ops
+    q, k, v = inputs(T, 300, 2, 1, 64, name, 10)
+    v[:] = 60000.0 if name == "f16" else 1e33
+    out = T.zeros_like(q)
+    ops.cuda_prompt_attention(out, q, k, v, offsets(T, (300,)), 0.125)
+    want, bound = reference(T, q, k, v, (300,), 0.125)
+    close(T, out, want, bound)
