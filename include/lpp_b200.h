@@ -397,7 +397,8 @@ lpp_status lpp_op_kv4_read(void* d_k, void* d_v, const void* d_k_cache, const vo
 /* Attention of one query token per sequence over the first d_lens[b] positions (clamped to [0, capacity]) of the 4-bit cache:
  * out[b][h] = sum_j softmax_j(scale q[b][h] . k[b][h / (n_heads / n_kv_heads)][j]) v[...][j]; zeros for a sequence of no positions.
  * q and out are [batch][n_heads][head_size] of dtype, *_stride elements from one sequence to the next.  FP32 queries and results are worked
- * with in FP32 precision, others with probabilities rounded to FP16.
+ * with in FP32 precision in every group of 32 dimensions, whatever the groups' sizes; of the others a query's elements are held to 2^-27 of its
+ * largest one, and probabilities times scales are rounded to FP16 (2^-11 of themselves, or 2^-33 of the largest one of the head).
  * d_sums_out (may be NULL) gets the running sums of attention weight that lpp_op_kv4_evict goes by, [batch][n_kv_heads][capacity]:
  * d_sums_in (NULL = zeros; may be the same array) plus, per position, the sum of the softmax over the query heads of the key/value
  * head.  Positions from the length on are left as they were.

@@ -268,12 +268,13 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.rate = scale * 1.4426950408889634f;
     return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
                         constexpr int NG = ng.value;
-                        constexpr int most = (227 * 1024) / kKv4Ctas<NG> - 1024 * (NG + 2);  // shared memory of a CTA beside its fixed arrays
-                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads)), room = most - sums;
+                        const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads));
                         // as many units in flight as the shared memory holds beside the warps' sums; a short cache has no more
                         auto go = [&](auto parts, auto clusters) {
-                            constexpr auto kernel = kv4_attn_kernel<NG, parts.value == 2, clusters.value == 1>;
-                            a.stages = std::min(clusters.value ? kKv4ClusterUnits : kKv4MaxStages, room / kKv4StageBytes<NG>);
+                            constexpr bool split = parts.value == 2;
+                            constexpr auto kernel = kv4_attn_kernel<NG, split, clusters.value == 1>;
+                            constexpr int most = (227 * 1024) / kKv4Ctas<NG> - 1024 * (NG + 2) - (split ? 512 * NG : 0);  // shared memory of a CTA beside its fixed arrays
+                            a.stages = std::min(clusters.value ? kKv4ClusterUnits : kKv4MaxStages, (most - sums) / kKv4StageBytes<NG>);
                             const int smem = a.stages * kKv4StageBytes<NG> + sums;
                             if (!allow_smem<kernel>(most)) return LPP_ERR_CUDA;
                             return launch_op_cluster(kernel, dim3(clusters.value ? P.cluster * batch * n_kv_heads * a.head_tiles : P.runs), kKv4Threads, smem,

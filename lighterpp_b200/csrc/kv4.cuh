@@ -255,8 +255,12 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
 // 24 us of issue slots, their 168 MB 26 us.  Four warps a scheduler fill 63 % of the slots: 43.5 us (3.9 TB/s); 32769 positions with sums
 // 23 us, of which starting and merging take 5 and the second kernel 4.
 //
-// SPLIT: FP32 queries and FP32 results go in as two FP16 operands each (hi + lo), the sums of either added up, and the keys' codes are
-// n - 8 too, with (0, Q_g): sums of n and 8 Q_g that cancel would cost two bits of the scores.
+// SPLIT, for FP32 queries and results, whose groups may differ in size: queries go in as two FP16 operands (hi + lo) with a power of two of
+// every group, which scale_g's factor takes back; the keys' codes are n - 8 too, and zero_g Q_g is added in FP32 (sums of n and 8 Q_g that cancel
+// would cost two bits of the scores).  Probabilities times scales go in as three BF16 operands, which are all of an FP32 number wherever it lies;
+// two FP16 ones, under the one reference of all groups, lost bits of groups 2^-11 below the largest, and the low half of those 2^-22 below.
+// (FP32, 131071 positions of eight heads of 128:
+// 55 us with those, now 66; of heads of 64 35.5 and 40; 641 positions 6.4 and 6.65.)
 constexpr int kKv4Warps = 8, kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tile = 16;     // positions of a warp's tile
 constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
@@ -369,6 +373,12 @@ __device__ __forceinline__ void kv4_mma_add(float (&d)[4], uint32_t a0, uint32_t
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// d += a . b in BF16
+__device__ __forceinline__ void kv4_mma_add_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {  // 8 x 8 matrix of 16-bit elements spread over a warp
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -446,6 +456,21 @@ __device__ __forceinline__ uint32_t kv4_high(uint32_t x, const Kv4Magic& c) {
     const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&b), *reinterpret_cast<const __half2*>(&c.f), *reinterpret_cast<const __half2*>(&c.off));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
+// (n - 8) in BF16 of the codes in bits 0-3 and 16-19: 128 + n - 136
+__device__ __forceinline__ uint32_t kv4_bf16(uint32_t x, uint32_t exponent /* 0x43004300 */) {
+    uint32_t b;
+    asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xea;" : "=r"(b) : "r"(x), "r"(exponent));
+    const uint32_t off = 0x43084308u;
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&b), *reinterpret_cast<const __nv_bfloat162*>(&off));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// The upper eight bits of the significands of x and y as a pair of BF16 numbers; x and y keep the rest.  Three times, and there is none.
+__device__ __forceinline__ uint32_t kv4_part(float& x, float& y) {
+    const uint32_t u = __float_as_uint(x), w = __float_as_uint(y);
+    x = __fsub_rn(x, __uint_as_float(u & 0xffff0000u));
+    y = __fsub_rn(y, __uint_as_float(w & 0xffff0000u));
+    return __byte_perm(u, w, 0x7632);
+}
 
 // Barriers by address in shared memory (as pointers, their address is put together again at every use)
 __device__ __forceinline__ bool kv4_try_wait(uint32_t bar, uint32_t parity) {
@@ -486,6 +511,8 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
     __shared__ uint64_t full[kKv4MaxStages], empty[kKv4MaxStages];
     __shared__ Kv4Ahead ahead;
     __shared__ int s_fail;
+    // SPLIT: of every warp, group and pair of heads 2 t, 2 t + 1: factors of the group's scores, and sums Q of its queries
+    __shared__ float4 s_q[SPLIT ? kKv4Warps : 1][SPLIT ? NG : 1][4];
     __shared__ float c_y[CLUSTER ? kKv4Heads * NG * 32 : 1], c_ml[kKv4Heads][2];                  // this CTA's sums, reference and sum of probabilities
     __shared__ float c_w[CLUSTER ? kKv4Heads : 1][kKv4Cluster + 2];                               // weights of the CTAs; reference, 1 / sum of all
     pdl_wait();
@@ -574,36 +601,52 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
 
     Kv4Magic magic;
     magic.hide();
+    uint32_t magic_bf16 = 0x43004300u;
+    asm volatile("" : "+r"(magic_bf16));
 
     while (CLUSTER || b < p_end.b || (b == p_end.b && (head < p_end.head || (head == p_end.head && unit < p_end.unit)))) {
         const int kvh = head / a.head_tiles, tile8 = head - kvh * a.head_tiles;
         const int h0 = kvh * a.gqa + tile8 * kKv4Heads, n_heads = min(kKv4Heads, a.gqa - tile8 * kKv4Heads);
         const long long row0 = ((long long)b * a.kv_heads + kvh) * a.capacity;
         const int mine = (b == p_end.b && head == p_end.head ? p_end.unit : units) - unit, p1 = len;
-        // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest 2^6 .. 2^7 (eight times
-        // their sums over a group stay in the FP16 range)
+        // queries: head g of the tile, dimensions 8 t .. 8 t + 7 of every group, times a power of two that makes the largest (SPLIT: of the group)
+        // 2^6 .. 2^7 (eight times their sums over a group stay in the FP16 range)
         uint32_t qf[kParts][NG][4];
-        float rate[2];  // factor of the scores, heads 2 t and 2 t + 1
+        float rate[2];  // (not SPLIT) factor of the scores, heads 2 t and 2 t + 1
         uint32_t zf[NG > 4 ? 2 : 1][2];  // operand of (scale, zero), head g: (-8 Q, Q) of group t, and of the rest of Q after FP16 (more than 4 groups: group t + 4)
         {
-            float x[NG][8], top = 0.f;
+            float x[NG][8], tops[NG], top = 0.f;
             const bool some = g < n_heads;
 #pragma unroll
-            for (int i = 0; i < NG; ++i)
+            for (int i = 0; i < NG; ++i) {
+                tops[i] = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int d = i * 32 + t * 8 + j;
                     x[i][j] = some && d < a.head_size ? load_typed(a.q, (long long)b * a.q_stride + (long long)(h0 + g) * a.head_size + d, a.dtype) : 0.f;
-                    top = fmaxf(top, fabsf(x[i][j]));
+                    tops[i] = fmaxf(tops[i], fabsf(x[i][j]));
                 }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                if constexpr (SPLIT) {
+                    tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 1));
+                    tops[i] = fmaxf(tops[i], __shfl_xor_sync(0xffffffffu, tops[i], 2));
+                }
+                top = fmaxf(top, tops[i]);
+            }
+            if constexpr (!SPLIT) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            }
             // exponents of 2 in two halves, either within the normal range
-            const int e = top > 0.f && top < INFINITY ? 6 - ilogbf(top) : 0, e0 = e / 2, e1 = e - e0;
-            const float f0 = __int_as_float((127 + e0) << 23), f1 = __int_as_float((127 + e1) << 23);
+            auto exponent = [](float y) { return y > 0.f && y < INFINITY ? 6 - ilogbf(y) : 0; };
+            auto power = [](int e) { return __int_as_float((127 + e) << 23); };
+            // back from the operands' factors: 2^24 / 2^e (finite: beyond, scores are alike, or so far apart that one position wins)
+            auto back_from = [&](int e) { return fminf(power(-(e / 2)) * a.rate * power(-(e - e / 2)) * kUnit, 3.402823466e38f); };
+            const int e_all = exponent(top);
             float sums[NG];
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
+                const int e = SPLIT ? exponent(tops[i]) : e_all;
+                const float f0 = power(e / 2), f1 = power(e - e / 2);
                 float sum = 0.f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {  // register j: dimensions j and j + 4; odd ones meet codes times 16 (SPLIT: none)
@@ -613,24 +656,30 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                     const __half2 hi = __floats2half2_rn(u * f, w * f);
                     const float2 hf = __half22float2(hi);
                     qf[0][i][j] = *reinterpret_cast<const uint32_t*>(&hi);
-                    sum += (hf.x + hf.y) * (sixteenth ? 16.f : 1.f);
                     if constexpr (SPLIT) {
-                        const __half2 lo = __floats2half2_rn(u * f - hf.x, w * f - hf.y);
-                        const float2 lf = __half22float2(lo);
+                        const __half2 lo = __floats2half2_rn(u - hf.x, w - hf.y);
                         qf[1][i][j] = *reinterpret_cast<const uint32_t*>(&lo);
-                        sum += lf.x + lf.y;
+                        sum += u + w;
+                    } else {
+                        sum += (hf.x + hf.y) * (sixteenth ? 16.f : 1.f);
                     }
                 }
                 sum += __shfl_xor_sync(0xffffffffu, sum, 1);
                 sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 sums[i] = sum;
+                if constexpr (SPLIT)
+                    if ((i & 3) == t) {
+                        float* to = reinterpret_cast<float*>(&s_q[warp][i][g >> 1]) + (g & 1);
+                        to[0] = back_from(e);
+                        to[2] = sum;
+                    }
             }
-            // back from the operands' factors: 2^24 / 2^e (finite: beyond, scores are alike, or so far apart that one position wins)
-            const float back = fminf(__int_as_float((127 - e0) << 23) * __int_as_float((127 - e1) << 23) * a.rate * kUnit, 3.402823466e38f);
+            if constexpr (SPLIT) {
+                __syncwarp();
+            } else {
+                const float back = back_from(e_all);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int from = (2 * t + j) * 4;
-                rate[j] = __shfl_sync(0xffffffffu, back, from);
+                for (int j = 0; j < 2; ++j) rate[j] = __shfl_sync(0xffffffffu, back, (2 * t + j) * 4);
             }
             float own[NG > 4 ? 2 : 1] = {};
 #pragma unroll
@@ -639,7 +688,7 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
 #pragma unroll
             for (int i = 0; i < (NG > 4 ? 2 : 1); ++i) {
                 const __half hi = __float2half_rn(own[i]), lo = __float2half_rn(own[i] - __half2float(hi));
-                const __half times = __float2half_rn(SPLIT ? 0.f : -8.f);
+                const __half times = __float2half_rn(-8.f);
                 const __half2 both = __halves2half2(__hmul(hi, times), hi), rest = __halves2half2(__hmul(lo, times), lo);
                 zf[0][i] = *reinterpret_cast<const uint32_t*>(&both);
                 zf[NG > 4 ? 1 : 0][NG > 4 ? i : 1] = *reinterpret_cast<const uint32_t*>(&rest);
@@ -667,15 +716,16 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                 const uint32_t r0 = sk + g * kRow + NG * 16, r1 = r0 + 8 * kRow;  // scales and zeros
                 kv4_params<NG>(r0, p0);
                 kv4_params<NG>(r1, p1w);
-                // rows of (scale, zero) pairs as they lie there times (-8 Q, Q), or (0, Q)
                 float zacc[4], acc[NG][4];
-                if constexpr (NG > 4) {
-                    const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
-                    kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1]);
-                    kv4_mma_add(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1]);
-                } else {
-                    const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
-                    kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1]);
+                if constexpr (!SPLIT) {  // rows of (scale, zero) pairs as they lie there times (-8 Q, Q)
+                    if constexpr (NG > 4) {
+                        const uint32_t a0 = lds32(r0 + t * 4), a1 = lds32(r1 + t * 4), a2 = lds32(r0 + 16 + t * 4), a3 = lds32(r1 + 16 + t * 4);
+                        kv4_mma(zacc, a0, a1, a2, a3, zf[0][0], zf[0][1]);
+                        kv4_mma_add(zacc, a0, a1, a2, a3, zf[1][0], zf[1][1]);
+                    } else {
+                        const uint32_t a0 = t < NG ? lds32(r0 + t * 4) : 0u, a1 = t < NG ? lds32(r1 + t * 4) : 0u;
+                        kv4_mma(zacc, a0, a1, a0, a1, zf[0][0], zf[0][1]);
+                    }
                 }
                 // (the groups' chains of products side by side)
 #pragma unroll
@@ -695,18 +745,28 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
                         if constexpr (SPLIT) kv4_mma_add(acc[gr], a0, a1, a2, a3, qf[1][gr][2 * half], qf[1][gr][2 * half + 1]);
                     }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) s[j] = zacc[j] * (1.f / kUnit);
+                for (int j = 0; j < 4; ++j) s[j] = SPLIT ? 0.f : zacc[j] * (1.f / kUnit);
 #pragma unroll
                 for (int gr = 0; gr < NG; ++gr) {
-                    const float s0 = half2_bits_to_float2(p0[gr]).x, s1 = half2_bits_to_float2(p1w[gr]).x;
-                    s[0] = fmaf(s0, acc[gr][0], s[0]);
-                    s[1] = fmaf(s0, acc[gr][1], s[1]);
-                    s[2] = fmaf(s1, acc[gr][2], s[2]);
-                    s[3] = fmaf(s1, acc[gr][3], s[3]);
+                    const float2 u0 = half2_bits_to_float2(p0[gr]), u1 = half2_bits_to_float2(p1w[gr]);
+                    if constexpr (SPLIT) {
+                        const float4 f = s_q[warp][gr][t];
+                        s[0] = fmaf(f.x, fmaf(u0.x, acc[gr][0], u0.y * f.z), s[0]);
+                        s[1] = fmaf(f.y, fmaf(u0.x, acc[gr][1], u0.y * f.w), s[1]);
+                        s[2] = fmaf(f.x, fmaf(u1.x, acc[gr][2], u1.y * f.z), s[2]);
+                        s[3] = fmaf(f.y, fmaf(u1.x, acc[gr][3], u1.y * f.w), s[3]);
+                    } else {
+                        s[0] = fmaf(u0.x, acc[gr][0], s[0]);
+                        s[1] = fmaf(u0.x, acc[gr][1], s[1]);
+                        s[2] = fmaf(u1.x, acc[gr][2], s[2]);
+                        s[3] = fmaf(u1.x, acc[gr][3], s[3]);
+                    }
                 }
             }
+            if constexpr (!SPLIT) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] *= rate[j & 1];
+                for (int j = 0; j < 4; ++j) s[j] *= rate[j & 1];
+            }
             if constexpr (!kWhole) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -766,33 +826,43 @@ static __global__ void __launch_bounds__(kKv4Threads, kKv4Ctas<NG>) kv4_attn_ker
             l[0] += p[0] + p[2];
             l[1] += p[1] + p[3];
             // ---- values
-            uint32_t pf[kParts][NG][2];  // probabilities times scales as operands: rows as the codes have them
+            uint32_t pf[NG][2];  // probabilities times scales as operands: rows as the codes have them
 #pragma unroll
             for (int gr = 0; gr < NG; ++gr) {
                 const float2 u = half2_bits_to_float2(vp[0][gr]), w = half2_bits_to_float2(vp[1][gr]);
                 z[gr][0] = fmaf(p[2], w.y, fmaf(p[0], u.y, z[gr][0]));
                 z[gr][1] = fmaf(p[3], w.y, fmaf(p[1], u.y, z[gr][1]));
-                const float y0 = p[0] * u.x, y1 = p[1] * u.x, y2 = p[2] * w.x, y3 = p[3] * w.x;
-                const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
-                pf[0][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&ha));
-                pf[0][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
+                float y0 = p[0] * u.x, y1 = p[1] * u.x, y2 = p[2] * w.x, y3 = p[3] * w.x;
                 if constexpr (SPLIT) {
-                    const float2 fa = __half22float2(ha), fb = __half22float2(hb);
-                    const __half2 la = __floats2half2_rn(y0 - fa.x, y1 - fa.y), lb = __floats2half2_rn(y2 - fb.x, y3 - fb.y);
-                    pf[1][gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&la));
-                    pf[1][gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&lb));
+                    uint32_t part[3][2];
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) {
+                        part[i][0] = transpose8(kv4_part(y0, y1));
+                        part[i][1] = transpose8(kv4_part(y2, y3));
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
+                        const uint32_t a0 = kv4_bf16(xa, magic_bf16), a1 = kv4_bf16(xa >> 4, magic_bf16), a2 = kv4_bf16(xb, magic_bf16), a3 = kv4_bf16(xb >> 4, magic_bf16);
+#pragma unroll
+                        for (int i = 0; i < 3; ++i) kv4_mma_add_bf16(o[2 * gr + k], a0, a1, a2, a3, part[i][0], part[i][1]);
+                    }
+                } else {
+                    const __half2 ha = __floats2half2_rn(y0, y1), hb = __floats2half2_rn(y2, y3);
+                    pf[gr][0] = transpose8(*reinterpret_cast<const uint32_t*>(&ha));
+                    pf[gr][1] = transpose8(*reinterpret_cast<const uint32_t*>(&hb));
                 }
             }
+            if constexpr (!SPLIT) {
 #pragma unroll
-            for (int gr = 0; gr < NG; ++gr)
+                for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
-                    const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
-                    float(&y)[4] = o[2 * gr + k];
-#pragma unroll
-                    for (int part = 0; part < kParts; ++part) kv4_mma_add(y, a0, a1, a2, a3, pf[part][gr][0], pf[part][gr][1]);
-                }
+                    for (int k = 0; k < 2; ++k) {
+                        const uint32_t xa = codes[gr][0] >> (8 * k), xb = codes[gr][1] >> (8 * k);
+                        const uint32_t a0 = kv4_low(xa, magic), a1 = kv4_high(xa, magic), a2 = kv4_low(xb, magic), a3 = kv4_high(xb, magic);
+                        kv4_mma_add(o[2 * gr + k], a0, a1, a2, a3, pf[gr][0], pf[gr][1]);
+                    }
+            }
         };
         const int unit_end = min(p1, (unit + mine) * kKv4Unit);
         for (int unit_at = unit * kKv4Unit; unit_at < unit_end; unit_at += kKv4Unit) {
