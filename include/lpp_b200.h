@@ -359,7 +359,8 @@ lpp_status lpp_op_sample_static(float* d_logits, int vocab_size, float temperatu
 /* ---- attention operators beyond the reference's: prompts of several sequences, and a cache held in 4 bits -------------------
  *
  * No counterpart in the reference, which runs one sequence with an FP16 cache (src/model.cpp:121-209).  Device pointers, work is
- * queued on `stream`, nothing is allocated or synchronised; the current device is the one that holds the memory. */
+ * queued on `stream`, nothing is allocated or synchronised; the current device is the one that holds the memory.  A scale is positive and at most
+ * 2.3e38 (its product with log2(e) is finite). */
 
 /* Causal attention of n_sequences whole prompts that lie behind one another, d_offsets[n_sequences + 1] (on the device, ascending from
  * 0; equal neighbours are empty prompts) being their first tokens and the end of the last: for a token i of a prompt

@@ -58,6 +58,12 @@ lpp_status with_type(int dtype, F f) {
     if (dtype == LPP_BF16) return f((__nv_bfloat16*)nullptr);
     return f((float*)nullptr);
 }
+// The factor of a score in base 2, scale * log2(e); 0 where the scale has none: the product, too, is positive and finite.
+constexpr float kLog2e = 1.4426950408889634f;
+float rate_of(float scale) {
+    const float rate = scale * kLog2e;
+    return rate > 0.f && rate <= 3.402823466e38f ? rate : 0.f;
+}
 bool is_dtype(int dtype) { return dtype == LPP_F32 || dtype == LPP_F16 || dtype == LPP_BF16; }
 
 // What every call on a 4-bit cache wants of it; NULL = nothing wrong.
@@ -138,7 +144,7 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
     if (n_heads <= 0 || n_kv_heads <= 0 || n_heads % n_kv_heads || n_heads > 65535) return refuse("prompt attention: the key/value heads divide the heads");
     if (head_size <= 0 || head_size % 8 || head_size > 128) return refuse("prompt attention: head sizes are multiples of 8 up to 128");
     if (dtype != LPP_F16 && dtype != LPP_BF16) return refuse("prompt attention: F16 or BF16");
-    if (!(scale > 0.f) || scale > 3.4e38f) return refuse("prompt attention: the scale is positive and finite");
+    if (rate_of(scale) == 0.f) return refuse("prompt attention: the scale is positive, and finite with a factor of log2(e)");
     if (n_sequences == 0 || n_tokens == 0) return LPP_OK;
     if (!d_out || !d_q || !d_k || !d_v || !d_offsets) return refuse("prompt attention: null pointer");
     if (((uintptr_t)d_out | (uintptr_t)d_q | (uintptr_t)d_k | (uintptr_t)d_v) & 15 || (uintptr_t)d_offsets & 3)
@@ -177,7 +183,7 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
         a.pair_heads = Shape::kTiles == 2 && a.gqa % 2 == 0;
         const int cta_rows = a.pair_heads ? kPaRows : Shape::kTiles * kPaRows, per_tile = a.pair_heads ? n_heads / 2 : n_heads;
         a.tiles = (n_tokens + cta_rows - 1) / cta_rows;
-        a.rate = scale * 1.4426950408889634f;
+        a.rate = rate_of(scale);
         if ((long long)a.tiles * per_tile > 0x7fffffffll) return LPP_ERR_TOO_LARGE;
         if (!allow_smem<prompt_attention_kernel<HS, T>>(Shape::kSmem)) return LPP_ERR_CUDA;
         return launch_op(prompt_attention_kernel<HS, T>, dim3(a.tiles * per_tile), Shape::kThreads, Shape::kSmem, S(stream), q_map, k_map, v_map, a);
@@ -233,7 +239,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     if (((uintptr_t)d_out | (uintptr_t)d_q) & (element - 1) || ((uintptr_t)d_lens | (uintptr_t)d_sums_in | (uintptr_t)d_sums_out) & 3)
         return refuse("4-bit attention: a pointer is not aligned to its type");
     if (out_stride < (int64_t)n_heads * head_size || q_stride < (int64_t)n_heads * head_size) return refuse("4-bit attention: a sequence's heads overlap the next one's");
-    if (!(scale > 0.f) || scale > 3.4e38f) return refuse("4-bit attention: the scale is positive and finite");
+    if (rate_of(scale) == 0.f) return refuse("4-bit attention: the scale is positive, and finite with a factor of log2(e)");
     if (d_sums_in && !d_sums_out) return refuse("4-bit attention: sums go in but not out");
     const int sms = sm_count();
     if (sms <= 0) return refuse("4-bit attention: no CUDA device", LPP_ERR_NO_DEVICE);
@@ -265,7 +271,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
     a.runs = P.runs;
     a.cluster = P.cluster;
     a.dtype = dtype;
-    a.rate = scale * 1.4426950408889634f;
+    a.rate = rate_of(scale);
     return launched("lpp_op_kv4_attention: the launch failed", with_groups(groups, [&](auto ng) {
                         constexpr int NG = ng.value;
                         const int sums = kv4_sums_bytes<NG>(std::min(a.gqa, kKv4Heads));

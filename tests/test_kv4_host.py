@@ -131,3 +131,10 @@ def test_plain_rows_hold_what_the_text_says():
     assert np.all(np.abs(y - x) <= s * (0.5 + 16 * 2.0 ** -11) + np.abs(z) * 2.0 ** -11 + 2.0 ** -24)
     const = U.unpack(U.pack(np.full((1, 40), 0.25)), 40)[0]
     assert np.all(const == 0.25)
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.4e38])
+def test_a_scale_beyond_fp32_in_base_2_is_refused(scale):
+    """scale * log2(e) would be infinite, and the scores of zeros no numbers."""
+    assert attention(scale=scale) == 1
+    assert b"scale" in E.load_library().lpp_last_error()

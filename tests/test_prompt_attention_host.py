@@ -30,3 +30,10 @@ def test_tensors_that_do_not_fit_are_refused():
     q = torch.zeros(4, 4, 64, dtype=torch.float16)
     with pytest.raises(ValueError):  # of the host
         ops.cuda_prompt_attention(torch.zeros_like(q), q, q, q, torch.zeros(2, dtype=torch.int32), 0.1)
+
+
+@pytest.mark.parametrize("scale", [3e38, 2.4e38])
+def test_a_scale_beyond_fp32_in_base_2_is_refused(scale):
+    """scale * log2(e) would be infinite, and masked scores no numbers."""
+    assert call(scale=scale) == 1
+    assert b"scale" in E.load_library().lpp_last_error()
