@@ -379,8 +379,9 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
  * The 4-bit cache of a layer is two arrays (keys, values) [batch][n_kv_heads][capacity] of rows of
  * lpp_op_kv4_row_bytes(head_size) bytes, on 16-byte boundaries, capacity a multiple of 4.  A row holds groups of 32 dimensions
  * (ceil(head_size / 32) of them; 8 where that is 5 to 7), lo and hi being the least and the largest value of a group:
- *     scale = fp16((hi - lo) / 15), zero = fp16(lo + 8 scale), code = clamp(round((x - zero) / scale) + 8, 0, 15)
- * (half to even; 8 where scale is 0), and the code stands for zero + scale (code - 8).  First the codes of all groups, two a
+ *     scale = fp16(fp32((hi - lo) / 15)), zero = fp16(fp32(lo + 8 scale)), code = clamp(round((x - zero) / scale) + 8, 0, 15)
+ * (exact quotients and sums, rounded to FP32 and from there to FP16; half to even; code 8 where scale is 0), and the code stands for
+ * zero + scale (code - 8).  First the codes of all groups, two a
  * byte, the lower dimension in the lower half; then (scale, zero) of every group.  A NaN is written as 0, a value beyond the FP16
  * range as +-65504.  Dimensions that the head does not have carry code 8. */
 

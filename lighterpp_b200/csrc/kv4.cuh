@@ -4,8 +4,9 @@
 //
 // A row holds the keys (or values) of one head at one position in groups of 32 dimensions.  With lo and hi the least and the largest
 // value of a group:
-//     scale = fp16((hi - lo) / 15),  zero = fp16(lo + 8 scale),  code = clamp(round((x - zero) / scale) + 8, 0, 15)   (half to even;
-// 8 where scale is 0), and the code stands for zero + scale (code - 8).  The bytes of a row: 16 per group with two codes each (the lower
+//     scale = fp16(fp32((hi - lo) / 15)),  zero = fp16(fp32(lo + 8 scale)),  code = clamp(round((x - zero) / scale) + 8, 0, 15)
+// (exact quotients and sums rounded to FP32, then to FP16: of FP32 values a few groups in 100,000 get a neighbour of what one rounding
+// would give, which its codes then go by; half to even; code 8 where scale is 0), and the code stands for zero + scale (code - 8).  The bytes of a row: 16 per group with two codes each (the lower
 // dimension in the lower half), then 4 per group with scale and zero.  The dimensions that fill the last group up have code 8 and
 // count neither for lo nor for hi.  A NaN is written as 0, values beyond the FP16 range as +-65504.
 #pragma once

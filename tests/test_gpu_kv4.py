@@ -537,3 +537,25 @@ def test_two_streams_at_once(T):
     T.cuda.synchronize()
     for i, (out, sums) in enumerate(got):
         assert T.equal(out, sets[i % 2][4]) and T.equal(sums, sets[i % 2][5])
+
+
+def test_scale_and_zero_by_way_of_fp32(T):
+    """Groups whose scale, or zero, is another FP16 number when the exact one is rounded without the step over FP32."""
+    from lighterpp_b200 import ops
+    rng = np.random.default_rng(1)
+    lo, hi = -np.abs(rng.standard_normal(400000)).astype(np.float32) * 3, np.abs(rng.standard_normal(400000)).astype(np.float32) * 3
+    lo[0], hi[0] = float.fromhex("-0x1.750b5ap+1"), float.fromhex("0x1.42314ap+0")
+    exact = (hi.astype(np.float64) - lo.astype(np.float64)) / 15
+    by_way = exact.astype(np.float32).astype(np.float16)
+    zero = lo.astype(np.float64) + 8 * by_way.astype(np.float64)
+    some = np.flatnonzero((exact.astype(np.float16) != by_way) | (zero.astype(np.float16) != zero.astype(np.float32).astype(np.float16)))
+    assert 0 in some and len(some) > 10
+    x = np.linspace(lo[some], hi[some], 32, axis=-1).astype(np.float32)
+    x[:, 0], x[:, -1] = lo[some], hi[some]
+    x = np.ascontiguousarray(np.clip(x, lo[some][:, None], hi[some][:, None])[:, None])
+    n = len(some)
+    cap = -(-n // 4) * 4
+    kc, vc = (T.zeros((1, 1, cap, 20), dtype=T.uint8, device="cuda") for _ in range(2))
+    xs = T.from_numpy(x).cuda()
+    ops.cuda_kv4_write(kc, vc, xs, xs, T.arange(n, device="cuda"))
+    assert np.array_equal(kc.cpu().numpy()[0, 0, :n], U.pack(x.astype(np.float64))[:, 0])
