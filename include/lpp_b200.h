@@ -383,13 +383,14 @@ lpp_status lpp_op_prompt_attention(void* d_out, const void* d_q, const void* d_k
  * (exact quotients and sums, rounded to FP32 and from there to FP16; half to even; code 8 where scale is 0), and the code stands for
  * zero + scale (code - 8).  First the codes of all groups, two a
  * byte, the lower dimension in the lower half; then (scale, zero) of every group.  A NaN is written as 0, a value beyond the FP16
- * range as +-65504.  Dimensions that the head does not have carry code 8. */
+ * range as +-65504; as scale and zero are rounded, a group that comes near +-65504 may stand for up to 65568: finite in FP32 and BF16, while an
+ * FP16 number read back, or an FP16 result of attention, is an infinity from 65520 on.  Dimensions that the head does not have carry code 8. */
 
 int64_t lpp_op_kv4_row_bytes(int head_size); /* -1: head sizes are 1 to 256 */
 
 /* Writes n_tokens rows of keys and values [token][n_kv_heads][head_size] (dtype F32, F16 or BF16; *_stride elements from one token to
  * the next) at the slots d_slots[token] = sequence * capacity + position.  A token whose slot lies outside [0, batch *
- * capacity) is left out.  The slots of one call differ from one another; n_tokens * n_kv_heads is at most 2^27.  lpp_op_kv4_read gets rows back as values; where the slot lies
+ * capacity) is left out.  The slots of one call differ from one another; n_tokens * n_kv_heads is at most 2^27.  lpp_op_kv4_read gets rows back as values, rounded to dtype; where the slot lies
  * outside, the token's place is left as it was. */
 lpp_status lpp_op_kv4_write(void* d_k_cache, void* d_v_cache, const void* d_k, const void* d_v, const int64_t* d_slots, int n_tokens, int batch,
                             int n_kv_heads, int64_t capacity, int head_size, int64_t k_stride, int64_t v_stride, int dtype, void* stream);

@@ -261,7 +261,8 @@ def cuda_kv4_write(d_k_cache, d_v_cache, d_k, d_v, d_slots):
 
 
 def cuda_kv4_read(d_k, d_v, d_k_cache, d_v_cache, d_slots):
-    """The values that the cache holds at ``d_slots``; a token whose slot is negative, or beyond the cache, is left as it was."""
+    """The values that the cache holds at ``d_slots``, rounded to the type of ``d_k`` (F16 has infinities from 65520 on, which rows written from
+    numbers near 65504 may reach); a token whose slot is negative, or beyond the cache, is left as it was."""
     caches, rows = (d_k_cache, d_v_cache), (d_k, d_v)
     _kv4_rows("cuda_kv4_read", _KV4_READ, rows, caches, d_k, d_v, caches, d_slots)
 

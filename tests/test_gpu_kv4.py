@@ -559,3 +559,30 @@ def test_scale_and_zero_by_way_of_fp32(T):
     xs = T.from_numpy(x).cuda()
     ops.cuda_kv4_write(kc, vc, xs, xs, T.arange(n, device="cuda"))
     assert np.array_equal(kc.cpu().numpy()[0, 0, :n], U.pack(x.astype(np.float64))[:, 0])
+
+
+def test_held_values_beyond_fp16(T):
+    """scale and zero are rounded, so a group that reaches +-65504 may stand for a little more: FP32 and BF16 get it as it is, FP16 rounded
+    to what it has, an infinity from 65520 on."""
+    from lighterpp_b200 import ops
+    x = np.zeros((4, 1, 32), dtype=np.float32)
+    x[0, 0, 0] = 65504
+    x[1, 0, :2] = 65504, -65504
+    x[2, 0, :2] = np.inf, -1
+    x[3, 0, :2] = -np.inf, 60000
+    rows = U.pack(x.astype(np.float64))
+    held = U.unpack(rows, 32)[0]
+    assert held[0, 0, 0] == 65520 and held[1, 0, 0] == 65536
+    kc, vc = (T.zeros((1, 1, 4, 20), dtype=T.uint8, device="cuda") for _ in range(2))
+    slots = T.arange(4, device="cuda")
+    xs = T.from_numpy(x).cuda()
+    ops.cuda_kv4_write(kc, vc, xs, xs, slots)
+    assert np.array_equal(kc.cpu().numpy()[0, 0], rows[:, 0])
+    for name in TYPES:
+        k, v = (T.zeros((4, 1, 32), dtype=dtype(T, name), device="cuda") for _ in range(2))
+        ops.cuda_kv4_read(k, v, kc, vc, slots)
+        assert T.equal(k.cpu(), T.from_numpy(held.astype(np.float32)).to(k.dtype)) and T.equal(k, v)
+        assert bool(k.isfinite().all()) == (name != "f16")
+        out = T.zeros((1, 1, 32), dtype=dtype(T, name), device="cuda")
+        ops.cuda_kv4_attention(out, T.zeros_like(out), kc, vc, T.tensor([1], dtype=T.int32, device="cuda"), 1.0)  # one position: its values
+        assert T.equal(out[0, 0].cpu(), T.from_numpy(held[0, 0].astype(np.float32)).to(out.dtype))
