@@ -586,3 +586,18 @@ def test_held_values_beyond_fp16(T):
         out = T.zeros((1, 1, 32), dtype=dtype(T, name), device="cuda")
         ops.cuda_kv4_attention(out, T.zeros_like(out), kc, vc, T.tensor([1], dtype=T.int32, device="cuda"), 1.0)  # one position: its values
         assert T.equal(out[0, 0].cpu(), T.from_numpy(held[0, 0].astype(np.float32)).to(out.dtype))
+
+
+@pytest.mark.parametrize("kind", ["random", "few"])
+@pytest.mark.parametrize("batch,kv,n,cap,keeps", [(1, 1, 39999, 40000, (1, 2048, 2049, 20000)), (1, 2, 70001, 70004, (2000, 50000)), (10, 8, 5000, 5000, (256, 257, 4500)),
+                                                  (40, 4, 4700, 4800, (100, 3000))])
+def test_evict_of_more_rows_than_a_thread_holds(T, kind, batch, kv, n, cap, keeps):
+    """More than 4096 rows a CTA: a cluster over one long head, and heads that get a CTA each."""
+    rng = np.random.default_rng(cap + batch)
+    if kind == "random":
+        sums = rng.random((batch, kv, cap)).astype(np.float32)
+        sums[..., ::3] *= np.linspace(0, 1, cap, dtype=np.float32)[::3]
+    else:  # equals among what is kept and what goes, before and behind the rows that a thread holds
+        sums = rng.choice(np.float32([0.25, 0.5, 0.5 + 2.0 ** -24, 1.0]), (batch, kv, cap))
+    for keep in keeps:
+        evict(T, 32, kv, (n,) + tuple(int(x) for x in rng.integers(0, n + 1, batch - 1)), cap, keep, min(keep, 33), sums, seed=keep)
