@@ -416,7 +416,7 @@ lpp_status lpp_op_kv4_attention(void* scratch, int64_t scratch_bytes, void* d_ou
  * than `keep` keeps, head by head, its `recent` last rows (recent <= keep) and of the others those with the largest sums, the lowest
  * position first among equals, a NaN counting as -infinity; a shorter one keeps everything.  Rows stay in their order.  d_kept
  * [batch][n_kv_heads][keep] gets the old positions, d_sums_out [batch][n_kv_heads][capacity_out] their sums, d_lens_out [batch]
- * the new lengths min(length, keep); what lies behind them is left as it was. */
+ * the new lengths min(length, keep); what lies behind them is left as it was.  The results overlap neither one another nor what is read. */
 lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int* d_kept, int* d_lens_out, const void* d_k_cache,
                             const void* d_v_cache, const float* d_sums, const int* d_lens, int batch, int n_kv_heads, int64_t capacity,
                             int64_t capacity_out, int head_size, int keep, int recent, void* stream);

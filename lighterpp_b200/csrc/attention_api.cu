@@ -301,16 +301,20 @@ lpp_status lpp_op_kv4_evict(void* d_k_out, void* d_v_out, float* d_sums_out, int
     if (!d_sums_out || !d_kept || !d_lens_out || !d_sums || !d_lens) return refuse("eviction: null pointer");
     if (((uintptr_t)d_sums_out | (uintptr_t)d_kept | (uintptr_t)d_lens_out | (uintptr_t)d_sums | (uintptr_t)d_lens) & 3) return refuse("eviction: a pointer is not aligned to its type");
     if (keep <= 0 || keep > capacity_out || recent < 0 || recent > keep) return refuse("eviction: 0 <= recent <= keep <= capacity of the new cache, keep > 0");
-    // rows move to other places while others are read: the old and the new cache are two
-    auto apart = [](const void* x, size_t nx, const void* y, size_t ny) { return (uintptr_t)x + nx <= (uintptr_t)y || (uintptr_t)y + ny <= (uintptr_t)x; };
+    // rows move to other places, and are listed, while sums and other rows are read: what is written overlaps nothing else
     const int row = kv4_row_bytes(kv4_held_groups(head_size));
-    const size_t heads = (size_t)batch * n_kv_heads, in = heads * capacity * row, out = heads * capacity_out * row;
-    const void *ins[2] = {d_k_cache, d_v_cache}, *outs[2] = {d_k_out, d_v_out};
-    for (const void* i : ins)
-        for (const void* o : outs)
-            if (!apart(i, in, o, out)) return refuse("eviction: the new cache overlaps the old one");
-    if (!apart(d_k_out, out, d_v_out, out) || !apart(d_sums, heads * capacity * 4, d_sums_out, heads * capacity_out * 4) || !apart(d_lens, (size_t)batch * 4, d_lens_out, (size_t)batch * 4))
-        return refuse("eviction: the new cache overlaps the old one");
+    const size_t heads = (size_t)batch * n_kv_heads, in = heads * capacity, out = heads * capacity_out;
+    struct Range {
+        const void* at;
+        size_t bytes;
+    };
+    const Range ranges[] = {{d_k_out, out * row},  {d_v_out, out * row}, {d_sums_out, out * 4}, {d_kept, heads * keep * 4}, {d_lens_out, (size_t)batch * 4},  // written
+                            {d_k_cache, in * row}, {d_v_cache, in * row}, {d_sums, in * 4},     {d_lens, (size_t)batch * 4}};
+    for (int w = 0; w < 5; ++w)
+        for (int r = w + 1; r < 9; ++r) {
+            const uintptr_t x = (uintptr_t)ranges[w].at, y = (uintptr_t)ranges[r].at;
+            if (x + ranges[w].bytes > y && y + ranges[r].bytes > x) return refuse("eviction: a result overlaps another one, or what is read");
+        }
     const int sms = sm_count();
     if (sms <= 0) return refuse("eviction: no CUDA device", LPP_ERR_NO_DEVICE);
     Kv4EvictArgs a = {};

@@ -138,3 +138,17 @@ def test_a_scale_beyond_fp32_in_base_2_is_refused(scale):
     """scale * log2(e) would be infinite, and the scores of zeros no numbers."""
     assert attention(scale=scale) == 1
     assert b"scale" in E.load_library().lpp_last_error()
+
+
+@pytest.mark.parametrize("wrong", [dict(kept=8 * P), dict(kept=8 * P + 2 * 64 * 4 - 4), dict(kept=9 * P), dict(kept=6 * P), dict(kept=P + 4), dict(so=4 * P), dict(so=7 * P), dict(so=9 * P),
+                                   dict(so=2 * P), dict(lo=4 * P + 8), dict(lo=8 * P), dict(lo=7 * P + 40), dict(lo=3 * P), dict(ko=8 * P), dict(vo=9 * P)])
+def test_evict_into_what_it_reads_or_writes_elsewhere_is_refused(wrong):
+    """Kept positions over the sums that are still being looked at would be counted one way and written another."""
+    assert evict(**wrong) == 1
+
+
+def test_evict_of_arrays_side_by_side_is_not_refused():
+    """Arrays that touch do not overlap (the call gets as far as the device)."""
+    if __import__("torch").cuda.is_available():
+        pytest.skip("addresses that stand for pointers are not followed")
+    assert evict(kept=8 * P + 2 * 64 * 4, lo=4 * P - 4, so=9 * P + 4) == 7  # no device here
