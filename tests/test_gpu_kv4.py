@@ -601,3 +601,11 @@ def test_evict_of_more_rows_than_a_thread_holds(T, kind, batch, kv, n, cap, keep
         sums = rng.choice(np.float32([0.25, 0.5, 0.5 + 2.0 ** -24, 1.0]), (batch, kv, cap))
     for keep in keeps:
         evict(T, 32, kv, (n,) + tuple(int(x) for x in rng.integers(0, n + 1, batch - 1)), cap, keep, min(keep, 33), sums, seed=keep)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("heads,kv,lens,cap", [(16, 2, (3000, 511), 3000), (24, 2, (2600,), 2600), (32, 2, (513, 2300), 2400), (12, 2, (2500,), 2500), (3, 1, (5000,), 5000)])
+def test_sums_of_groups_of_any_size(T, name, heads, kv, lens, cap):
+    """Heads that lie in several runs, with groups of 8, 12, 16, 6 and 3 query heads: scores are taken up in fours, or one by one."""
+    q, k, v = setup(T, heads, kv, 64, name, lens, cap, heads)
+    check(T, q, k, v, lens, 0.125, name)
