@@ -609,3 +609,25 @@ def test_sums_of_groups_of_any_size(T, name, heads, kv, lens, cap):
     """Heads that lie in several runs, with groups of 8, 12, 16, 6 and 3 query heads: scores are taken up in fours, or one by one."""
     q, k, v = setup(T, heads, kv, 64, name, lens, cap, heads)
     check(T, q, k, v, lens, 0.125, name)
+
+
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), float("-inf")])
+@pytest.mark.parametrize("n,cap", [(600, 600), (4000, 4000)])
+def test_queries_that_are_not_finite_spoil_their_own_head_only(T, name, bad, n, cap):
+    from lighterpp_b200 import ops
+    q, k, v = setup(T, 8, 2, 64, name, (n, n), cap, 13, garbage=False)
+    q[0, 2, 5] = bad
+    kc, vc = T.from_numpy(k).cuda(), T.from_numpy(v).cuda()
+    out, sums = T.zeros_like(q), T.zeros((2, 2, cap), device="cuda")
+    ops.cuda_kv4_attention(out, q, kc, vc, T.tensor([n, n], dtype=T.int32, device="cuda"), 0.125, None, sums)
+    q[0, 2, 5] = 0.0
+    ref, bound, want_sums, sums_bound = U.attention(q.double().cpu().numpy(), k, v, (n, n), 0.125, name != "f32")
+    got, got_sums = out.double().cpu().numpy(), sums.double().cpu().numpy()
+    assert np.isnan(got[0, 2]).all() and np.isnan(got_sums[0, 0]).all()
+    ok = np.ones((2, 8), dtype=bool)
+    ok[0, 2] = False
+    bound = bound + half_step(name) * (np.abs(ref) + bound) + 2.0 ** -25
+    assert np.all(np.abs(got - ref)[ok] <= bound[ok])
+    for b, h in ((0, 1), (1, 0), (1, 1)):
+        assert np.all(np.abs(got_sums - want_sums)[b, h] <= (sums_bound + 2.0 ** -24 * want_sums)[b, h])
