@@ -267,7 +267,7 @@ def cuda_kv4_read(d_k, d_v, d_k_cache, d_v_cache, d_slots):
     _kv4_rows("cuda_kv4_read", _KV4_READ, rows, caches, d_k, d_v, caches, d_slots)
 
 
-@functools.lru_cache(maxsize=None)
+@functools.lru_cache(maxsize=256)  # (a host whose capacities keep changing does not gather them all)
 def _kv4_scratch_bytes(device, *sizes):
     with torch.cuda.device(device):
         return _lib().lpp_op_kv4_attention_scratch_bytes(*sizes)

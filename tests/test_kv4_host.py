@@ -152,3 +152,7 @@ def test_evict_of_arrays_side_by_side_is_not_refused():
     if __import__("torch").cuda.is_available():
         pytest.skip("addresses that stand for pointers are not followed")
     assert evict(kept=8 * P + 2 * 64 * 4, lo=4 * P - 4, so=9 * P + 4) == 7  # no device here
+
+
+def test_sizes_asked_for_are_not_gathered_without_end():
+    assert 0 < ops._kv4_scratch_bytes.cache_info().maxsize < 10000
