@@ -11,9 +11,11 @@
 // Sums O are rescaled only when a row's maximum has grown by more than 2^8 since it was last set, by the row's own thread, when the
 // product of the tile before is complete.
 //
-// Measured: 8192 tokens of 32 heads of 128 take 438 us, 1.25 PFLOP/s, bound by the tensor cores under the power cap (without exponentials
-// 435); tensor cores and special functions are busy 60 % of the clocks each.  1023 tokens of 32 heads of 64: 15.5 us, of which the longest row
-// tiles' eight steps take 1.4 us each (exponentials of one warp a scheduler) and start and end 4.  201 tokens of 6 heads of 48: 6.7 us.
+// Measured from graphs: 8192 tokens of 32 heads of 128 take 438 - 480 us (up to 1.25 PFLOP/s; 507 - 518 in calls without a pause, under the power
+// cap).  The products are 475,000 clocks an SM of that, 242 us at the full clock; tensor cores and special functions are busy 60 % of the clocks
+// each, and without any exponentials it is 435 us, so the rest is the hand-over between the row tiles and the clock under the cap, which have not been
+// told apart.  1023 tokens of 32 heads of 64: 15.5 - 17 us, of which the longest row tiles' eight steps take 1.4 us each (exponentials of one
+// warp a scheduler) and start and end 4.  201 tokens of 6 heads of 48: 6.8 us.
 //
 // Sequences do not have to begin at tiles: row tiles cover the packed tokens whatever the borders, a row sees the keys from its
 // sequence's start to itself, and a tile runs over the keys from its first row's sequence on.  Many short prompts share a tile.
@@ -226,6 +228,11 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
     const int k0 = s_start[0], n_tiles = (t_end - 1 - k0) / kPaKeys + 1, last_start = s_start[t_end - 1 - t0];
     // some row of the CTA sees only a part of key tile `it`
     auto partial = [&](int it) { return k0 + it * kPaKeys < last_start || k0 + it * kPaKeys + kPaKeys - 1 > t0; };
+    // the signs' places of the numbers of a pair that are not finite: an exponent of ones carries into them
+    auto odd_of = [](uint32_t w) {
+        constexpr bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+        return ((w & (bf16 ? 0x7f807f80u : 0x7c007c00u)) + (bf16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+    };
     auto wait = [](uint64_t* bar, int phase) { return __all_sync(0xffffffffu, mbar_wait_bounded(bar, (uint32_t)phase & 1u, nullptr)) != 0; };
 
     if (warp >= Shape::kSoftWarps) {
@@ -301,7 +308,6 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
             if (!ok) s_fail = 1;
         } else {
             // ---------------- values that are not finite
-            constexpr uint32_t kExp = std::is_same<T, __nv_bfloat16>::value ? 0x7f807f80u : 0x7c007c00u, kOne = std::is_same<T, __nv_bfloat16>::value ? 0x00800080u : 0x04000400u;
             constexpr int kAhead = 8, kStep = kPaCheckWarps * 32;
             static_assert(kTile / 16 % (kAhead * kStep) == 0, "a tile is a whole number of rounds");
             for (int it = 0; it < n_tiles; ++it) {
@@ -322,12 +328,12 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
                     for (int k = 0; k < kAhead; ++k) {
                         uint32_t odd = 0;
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) odd |= ((w[k][j] & kExp) + kOne) & 0x80008000u;  // an exponent of ones carries into the sign's place
+                        for (int j = 0; j < 4; ++j) odd |= odd_of(w[k][j]);
                         if (odd) {
                             s_odd = 1;
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                const uint32_t o = ((w[k][j] & kExp) + kOne) & 0x80008000u;
+                                const uint32_t o = odd_of(w[k][j]);
                                 if (o & 0x8000u) w[k][j] &= 0xffff0000u;
                                 if (o & 0x80000000u) w[k][j] &= 0x0000ffffu;
                             }
@@ -487,17 +493,47 @@ static __global__ void __launch_bounds__(PaShape<HS>::kThreads, PaShape<HS>::kCt
                 }
             }
         }
-        if (ok && mine && l < INFINITY && !((lost[0] + lost[1]) + (lost[2] + lost[3]) == 0.f))  // (no sum of probabilities: all is NaN)
-            for (int d = 0; d < a.head_size; ++d) {
-                if (fabsf(to_float(dst[d])) < INFINITY) continue;
+        // (no sum of probabilities: all is NaN).  The lanes look through 128 tokens at once, eight dimensions each, and hand what they find around.
+        const bool search = ok && mine && l < INFINITY && !((lost[0] + lost[1]) + (lost[2] + lost[3]) == 0.f);
+        if (__any_sync(0xffffffffu, search)) {
+            const int j0 = __reduce_min_sync(0xffffffffu, search ? first : t_end), j1 = __reduce_max_sync(0xffffffffu, search ? i_row : 0);
+            for (int d = 0; d < a.head_size; d += 8) {
+                bool look = false;
+                if (search)
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) look = look || !(fabsf(to_float(dst[d + i])) < INFINITY);
+                if (!__any_sync(0xffffffffu, look)) continue;
                 const T* v = reinterpret_cast<const T*>(a.v) + (long long)kvh * a.head_size + d;
-                float seen = 0.f;
-                for (int j = first; j <= i_row && seen == seen; ++j) {
-                    const float y = to_float(v[(long long)j * a.v_stride]);
-                    if (!(fabsf(y) < INFINITY)) seen += y;
+                float seen[8] = {};
+                for (int j = j0; j <= j1; j += 128) {
+                    uint4 y[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int at = j + 32 * k + lane;
+                        y[k] = at <= j1 ? *reinterpret_cast<const uint4*>(v + (long long)at * a.v_stride) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        unsigned odd = __ballot_sync(0xffffffffu, (odd_of(y[k].x) | odd_of(y[k].y) | odd_of(y[k].z) | odd_of(y[k].w)) != 0u);
+                        for (; odd; odd &= odd - 1u) {
+                            const int from = __ffs((int)odd) - 1, at = j + 32 * k + from;
+                            const uint32_t w[4] = {__shfl_sync(0xffffffffu, y[k].x, from), __shfl_sync(0xffffffffu, y[k].y, from), __shfl_sync(0xffffffffu, y[k].z, from),
+                                                   __shfl_sync(0xffffffffu, y[k].w, from)};
+                            if (!look || at < first || at > i_row) continue;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 f = unpack2<T>(w[i]);
+                                if (!(fabsf(f.x) < INFINITY)) seen[2 * i] += f.x;
+                                if (!(fabsf(f.y) < INFINITY)) seen[2 * i + 1] += f.y;
+                            }
+                        }
+                    }
                 }
-                if (seen != 0.f) dst[d] = from_float<T>(seen);  // (0: finite values whose sum is beyond the type)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (seen[i] != 0.f) dst[d + i] = from_float<T>(seen[i]);  // (0: finite values whose sum is beyond the type)
             }
+        }
     }
     // ---------------- common exit
     __syncwarp();
