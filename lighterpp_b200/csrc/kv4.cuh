@@ -254,14 +254,15 @@ __device__ __forceinline__ uint32_t kv4_cluster_load(uint32_t a) {
 //
 // Bound by the instructions around the products, about 400 a warp for 16 positions of 128 dimensions: 131071 positions of eight heads are
 // 24 us of issue slots, their 168 MB 26 us.  Four warps a scheduler fill 63 % of the slots: 43.5 us (3.9 TB/s); 32769 positions with sums
-// 23 us, of which starting and merging take 5 and the second kernel 4.
+// 23 us, of which starting and merging take 5 and the second kernel 4.  131071 positions of eight heads of 64, whose rows of 40 bytes are no
+// multiple of 16 (no ldmatrix, see kv4_codes): 31 us for 84 MB.
 //
 // SPLIT, for FP32 queries and results, whose groups may differ in size: queries go in as two FP16 operands (hi + lo) with a power of two of
 // every group, which scale_g's factor takes back; the keys' codes are n - 8 too, and zero_g Q_g is added in FP32 (sums of n and 8 Q_g that cancel
 // would cost two bits of the scores).  Probabilities times scales go in as three BF16 operands, which are all of an FP32 number wherever it lies;
 // two FP16 ones, under the one reference of all groups, lost bits of groups 2^-11 below the largest, and the low half of those 2^-22 below.
-// (FP32, 131071 positions of eight heads of 128:
-// 55 us with those, now 66; of heads of 64 35.5 and 40; 641 positions 6.4 and 6.65.)
+// About 610 instructions a warp for 16 positions: 131071 positions of eight heads of 128 66 us (with two FP16 operands 55), of heads of 64 40 us
+// (35.5); 641 positions of 2048 6.65 us (6.4).
 constexpr int kKv4Warps = 8, kKv4Threads = kKv4Warps * 32;
 constexpr int kKv4Tile = 16;     // positions of a warp's tile
 constexpr int kKv4Unit = kKv4Warps * kKv4Tile;
@@ -1150,6 +1151,9 @@ static __global__ void __launch_bounds__(kKv4FinishThreads) kv4_finish_kernel(co
 // up by remote atomics in one CTA: passes of 3 - 8 us each instead of 1.4.  Rows moved by the cluster that lists them, two sequences of
 // 32768 and 20011 positions to 12000: 30 us, its SMs being too few for the bandwidth; now 26.)
 // 512 threads: two CTAs fit an SM (of 1024, sixteen clusters of eight did not fit the GPU at once, and the last ran alone).
+// A head has as many CTAs, up to eight, as give every CTA of the call an SM: of sequences of eight heads two get clusters of eight, four clusters of four,
+// nine of two, more a CTA a head, whose sums beyond 4096 rows are read again in every pass.  1, 2, 3, 9 and 16 sequences of 32768 positions to
+// 12000: 19.5, 27.6, 40.5, 94 and 152 us, their bytes 5 us a sequence.
 constexpr int kKv4EvictThreads = 512, kKv4EvictCluster = 8;
 constexpr int kKv4EvictKeep = 8;  // rows of a thread whose ranks stay in registers
 constexpr int kKv4EvictMove = 256;  // new rows a CTA up to which one kernel does it all
